@@ -60,7 +60,7 @@ extern "C" {
 #define KF_API
 #endif
 
-#define KF_ABI_VERSION 7 /* 7: kf_filter_backward_tapes, kf_set_option / kf_get_option.  6: kf_smoother_from_filter. \
+#define KF_ABI_VERSION 8 /* 8: kf_linear_attention, _backward, _step, kf_orthogonalise.  7: kf_filter_backward_tapes, kf_set_option / kf_get_option.  6: kf_smoother_from_filter. \
                           * 5: KF_FLAG_STEADY_STATE; the block kernel's steady-state phase off by default below 1536 steps; kf_workspace_bytes_for(KF_WS_FORWARD) covers the split pipeline. \
                           * 2: KF_FLAG_H_DIAGONAL, KF_KERNEL_MFMA, kf_dare, kf_simulate_statespace, workspace use by smoother/backward; \
                             3: kf_workspace_bytes_for, kf_forward_kernel_name_ws; every entry point runs on the handle's device; \
@@ -479,6 +479,70 @@ KF_API int kf_simulate_statespace(kf_handle* h, int64_t B, int32_t n_sims, int32
                            const double* R, const double* H, const double* Q, const double* x0,
                            const double* z_state, const double* z_obs, double* states,
                            double* obs, int32_t* info, void* stream);
+
+/* ---- sequence layers --------------------------------------------------------------------
+ * The linear state space recurrence as a layer of a sequence model, and the update its weight matrices are trained with.  These
+ * entry points take the element type of their data with them (the filters above are fp64 throughout). */
+enum {
+  KF_DTYPE_F64 = 0,  /* kf_orthogonalise only */
+  KF_DTYPE_F32 = 1,
+  KF_DTYPE_BF16 = 2,
+  KF_DTYPE_F16 = 3
+};
+
+/* Sizes, types and layouts of the kf_linear_attention entry points.  q, k: [B][T][G][K], v: [B][T][H][V]; head h reads the queries
+ * and keys of group h / (H / G).  Strides are in elements, for the axes batch, token, head (group) in this order; the last axis is
+ * contiguous.  A stride of 0 repeats a row.  1 <= K, V <= 128, H a multiple of G, B H < 2^31. */
+typedef struct kf_attention_dims {
+  int64_t B, T;
+  int32_t G, H, K, V;
+  int32_t dtype;           /* KF_DTYPE_F32, _BF16 or _F16: q, k, v, o and their gradients */
+  int32_t decay_per_token; /* log_decay is [B][T][H] (kf_linear_attention_step: [B][H]); 0: [H] */
+  double scale;            /* s below */
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  int64_t g_o_stride[3];   /* kf_linear_attention_backward only */
+} kf_attention_dims;
+
+/* Bytes of workspace kf_linear_attention (backward == 0) or kf_linear_attention_backward (!= 0) needs for these sizes. */
+KF_API int kf_linear_attention_workspace(kf_handle* h, const kf_attention_dims* dims, int backward, size_t* bytes);
+
+/* Linear attention with a decay for each head, over whole sequences:
+ *     S_t = exp(log_decay_t) S_{t-1} + k_t v_t',   o_t = s S_t' q_t,   S_0 = s0 (NULL: zero)
+ * o [B][T][H][V]; sT [B][H][K][V] fp32, the state behind each sequence's last token (may be NULL; may be s0).  log_decay is fp32 and
+ * meant to be <= 0; anything below -1e4, -infinity included, is a reset of the state.  lengths [B] int32 (NULL: all T): tokens from
+ * lengths[b] on (clamped to 0 .. T) are not read, o is zero there and the state stays.  The state, its sums and the decays are held
+ * in 32 bits; o is rounded once more than the state where dtype is 16 bits wide (see kf_attention.hip). */
+KF_API int kf_linear_attention(kf_handle* h, const kf_attention_dims* dims, const void* q, const void* k, const void* v,
+                               const float* log_decay, const float* s0, const int32_t* lengths, void* o, float* sT,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradient: of <g_o, o> + <g_sT, sT> (g_sT NULL: zero) with respect to q, k, v (contiguous, in dtype; summed over the heads of a
+ * group), log_decay (fp32, shaped like it) and s0 (fp32; NULL: not wanted).  Nothing of the forward call is needed.  Rows behind a
+ * sequence's end are zero.  The same inputs give the same bits (no atomics). */
+KF_API int kf_linear_attention_backward(kf_handle* h, const kf_attention_dims* dims, const void* q, const void* k, const void* v,
+                                        const float* log_decay, const float* s0, const int32_t* lengths, const void* g_o,
+                                        const float* g_sT, void* g_q, void* g_k, void* g_v, float* g_log_decay, float* g_s0,
+                                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token of each of B sequences whose states live in a pool, state [n_slots][H][K][V] fp32: row b reads and advances slot slots[b]
+ * (int32; NULL: slot b, and n_slots >= B).  The new states go to state_out (may be `state`; slots that no row names are not touched).
+ * dims->T and the token strides are not read.  A negative slot marks an empty row of the batch: o is zero, nothing else happens.  A
+ * slot >= n_slots does the same and sets info[b] = 1 (info may be NULL; 0 otherwise).  Rows that name the same slot are consecutive
+ * tokens of that sequence, in the order of the rows. */
+KF_API int kf_linear_attention_step(kf_handle* h, const kf_attention_dims* dims, const void* q, const void* k, const void* v,
+                                    const float* log_decay, const int32_t* slots, int64_t n_slots, const float* state,
+                                    float* state_out, void* o, int32_t* info, void* stream);
+
+/* Orthogonalised updates: each of n matrices M [n][rows][cols] moved towards its orthogonal factor by Newton-Schulz products,
+ *     X = M / (|M|_F + eps);   for each step (a, b, c):   A = X X',   X <- a X + (b A + c A A) X
+ * (on the transpose where rows > cols).  coefficients: HOST double[n_steps][3].  The singular values of X start in [0, 1] and each
+ * goes through the polynomials a s + b s^3 + c s^5; a list that can carry one of them above 1.9 is refused (KF_ERR_ARG).
+ * X: the type and shape of M, not overlapping it.  1 <= n_steps <= 16.  The same inputs give the same bits. */
+#define KF_ORTHOGONALISE_STEPS_MAX 16
+KF_API int kf_orthogonalise_workspace(kf_handle* h, int64_t n, int32_t rows, int32_t cols, int32_t dtype, size_t* bytes);
+KF_API int kf_orthogonalise(kf_handle* h, int64_t n, int32_t rows, int32_t cols, int32_t dtype, int32_t n_steps,
+                            const double* coefficients, double eps, const void* M, void* X, void* workspace,
+                            size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

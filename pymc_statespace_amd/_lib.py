@@ -12,7 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # KF_LIB_PATH: developer override for A/B experiments with instrumented builds of the same ABI
 LIB_PATH = os.environ.get("KF_LIB_PATH") or os.path.join(_HERE, "libkf_hip.so")
 
-KF_ABI_VERSION = 7
+KF_ABI_VERSION = 8
 
 KF_FILTER = {"standard": 0, "cholesky": 1, "univariate": 2, "single": 3}
 KF_FLAG_MVN_CONST_EXACT = 1 << 0
@@ -34,6 +34,8 @@ EXPORTS = (
     "kf_set_forward_kernel", "kf_forward_kernel_name", "kf_forward_kernel_name_ws", "kf_last_forward_kernel",
     "kf_workspace_bytes", "kf_workspace_bytes_for", "kf_filter_forward", "kf_filter_backward", "kf_filter_backward_tapes", "kf_filter_value_and_grad", "kf_smoother", "kf_smoother_from_filter",
     "kf_assemble", "kf_lyapunov", "kf_conditional_simulation", "kf_dare", "kf_dare_backward", "kf_simulate_statespace",
+    "kf_linear_attention_workspace", "kf_linear_attention", "kf_linear_attention_backward", "kf_linear_attention_step",
+    "kf_orthogonalise_workspace", "kf_orthogonalise",
 )
 
 
@@ -41,6 +43,18 @@ class KfDims(C.Structure):
     _fields_ = [
         ("B", C.c_int64), ("T", C.c_int32), ("p", C.c_int32), ("m", C.c_int32), ("r", C.c_int32),
         ("filter", C.c_int32), ("flags", C.c_uint32),
+    ]
+
+
+KF_DTYPE = {"float64": 0, "float32": 1, "bfloat16": 2, "float16": 3}
+KF_ORTHOGONALISE_STEPS_MAX = 16
+
+
+class KfAttentionDims(C.Structure):
+    _fields_ = [
+        ("B", C.c_int64), ("T", C.c_int64), ("G", C.c_int32), ("H", C.c_int32), ("K", C.c_int32), ("V", C.c_int32),
+        ("dtype", C.c_int32), ("decay_per_token", C.c_int32), ("scale", C.c_double),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("g_o_stride", C.c_int64 * 3),
     ]
 
 
@@ -125,6 +139,16 @@ def load():
     lib.kf_simulate_statespace.argtypes = [vp, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                            dp, dp, dp, dp, dp, dp, dp, dp, dp, dp, ip, vp]
     lib.kf_simulate_statespace.restype = C.c_int
+    ad, sz = C.POINTER(KfAttentionDims), C.c_size_t
+    lib.kf_linear_attention_workspace.argtypes = [vp, ad, C.c_int, C.POINTER(sz)]
+    lib.kf_linear_attention.argtypes = [vp, ad] + [dp] * 8 + [vp, sz, vp]
+    lib.kf_linear_attention_backward.argtypes = [vp, ad] + [dp] * 13 + [vp, sz, vp]
+    lib.kf_linear_attention_step.argtypes = [vp, ad] + [dp] * 4 + [ip, C.c_int64] + [dp] * 3 + [ip, vp]
+    lib.kf_orthogonalise_workspace.argtypes = [vp, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.POINTER(sz)]
+    lib.kf_orthogonalise.argtypes = [vp, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_double),
+                                     C.c_double, vp, vp, vp, sz, vp]
+    for name in EXPORTS[-6:]:
+        getattr(lib, name).restype = C.c_int
     if lib.kf_abi_version() != KF_ABI_VERSION:
         raise KfLibraryMissing(f"{LIB_PATH}: ABI version {lib.kf_abi_version()} != {KF_ABI_VERSION}")
     _lib = lib

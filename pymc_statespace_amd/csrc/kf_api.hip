@@ -1,10 +1,12 @@
 // kf_api.hip -- the extern "C" surface declared in include/kf.h: argument checks,
 // kernel selection, launches.  No allocation, no synchronisation, no host copies here
 // (safe to capture in a hipGraph).
+#include <math.h>
 #include <stdlib.h>
 
 #include "kf_internal.h"
 #include "kf_b4_split.h"
+#include "kf_sequence.h"
 
 static thread_local char g_err[256] = "";
 
@@ -1550,4 +1552,231 @@ extern "C" int kf_simulate_statespace(kf_handle* h, int64_t B, int32_t n_sims, i
   KF_ON_DEVICE(h);
   return kf_launch_simulate_statespace(h, B, n_sims, n, p, m, r, T, Z, R, H, Q, x0, z_state, z_obs, states, obs, info,
                                        (hipStream_t)stream);
+}
+
+// ------------------------------------------------------------------------------------------------ sequence layers
+// Checks the sizes and strides and copies them; `which` names the entry point in the error text.
+static int attention_args(kf_handle* h, const kf_attention_dims* d, const char* which, KfAttnArgs* a) {
+  if (!h) return KF_ERR_ARG;
+  if (!d) {
+    KF_SET_ERR(h, "%s: dims is NULL", which);
+    return KF_ERR_ARG;
+  }
+  if (d->B < 1 || d->T < 1 || d->G < 1 || d->H < 1 || d->K < 1 || d->V < 1) {
+    KF_SET_ERR(h, "%s: sizes must be positive (B=%ld T=%ld G=%d H=%d K=%d V=%d)", which, (long)d->B, (long)d->T, d->G, d->H, d->K, d->V);
+    return KF_ERR_ARG;
+  }
+  if (d->H % d->G) {
+    KF_SET_ERR(h, "%s: H=%d is not a multiple of G=%d", which, d->H, d->G);
+    return KF_ERR_ARG;
+  }
+  if (d->K > 128 || d->V > 128) {
+    KF_SET_ERR(h, "%s: K=%d, V=%d: at most 128 each (a wider V is several heads)", which, d->K, d->V);
+    return KF_ERR_UNSUPPORTED;
+  }
+  if (d->dtype != KF_DTYPE_F32 && d->dtype != KF_DTYPE_BF16 && d->dtype != KF_DTYPE_F16) {
+    KF_SET_ERR(h, "%s: dtype %d is none of KF_DTYPE_F32, _BF16, _F16", which, d->dtype);
+    return KF_ERR_UNSUPPORTED;
+  }
+  // (a sequence of 2^31 tokens would not fit the memory in any type; its bound keeps every product of sizes below in 63 bits)
+  if (d->B > 0x7fffffffL / d->H || d->T > 0x7fffffffL || d->B * d->T > (1L << 40) / d->H) {
+    KF_SET_ERR(h, "%s: B=%ld T=%ld H=%d: B H must be below 2^31, B T H below 2^40", which, (long)d->B, (long)d->T, d->H);
+    return KF_ERR_UNSUPPORTED;
+  }
+  if (!(fabs(d->scale) <= 3.0e38)) {
+    KF_SET_ERR(h, "%s: scale must be a finite fp32 number", which);
+    return KF_ERR_ARG;
+  }
+  for (int i = 0; i < 3; ++i)
+    if (d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0) {
+      KF_SET_ERR(h, "%s: strides must not be negative", which);
+      return KF_ERR_ARG;
+    }
+  memset(a, 0, sizeof(*a));
+  a->B = d->B; a->T = d->T; a->G = d->G; a->H = d->H; a->K = d->K; a->V = d->V;
+  a->dtype = d->dtype; a->per_token = d->decay_per_token != 0; a->scale = (float)d->scale;
+  for (int i = 0; i < 3; ++i) {
+    a->qs[i] = d->q_stride[i]; a->ks[i] = d->k_stride[i]; a->vs[i] = d->v_stride[i]; a->gs[i] = d->g_o_stride[i];
+  }
+  return KF_OK;
+}
+
+static int workspace_ok(kf_handle* h, const char* which, size_t need, const void* ws, size_t bytes) {
+  if (need && (!ws || bytes < need)) {
+    KF_SET_ERR(h, "%s: workspace of %zu bytes, %zu needed", which, ws ? bytes : (size_t)0, need);
+    return KF_ERR_WORKSPACE;
+  }
+  if (need && ((uintptr_t)ws & 15)) {
+    KF_SET_ERR(h, "%s: the workspace must be aligned to 16 bytes", which);
+    return KF_ERR_ARG;
+  }
+  return KF_OK;
+}
+
+extern "C" int kf_linear_attention_workspace(kf_handle* h, const kf_attention_dims* dims, int backward, size_t* bytes) {
+  KfAttnArgs a;
+  const int rc = attention_args(h, dims, "kf_linear_attention_workspace", &a);
+  if (rc) return rc;
+  if (!bytes) {
+    KF_SET_ERR(h, "kf_linear_attention_workspace: bytes is NULL");
+    return KF_ERR_ARG;
+  }
+  *bytes = kf_attention_workspace(h, a, backward != 0);
+  return KF_OK;
+}
+
+extern "C" int kf_linear_attention(kf_handle* h, const kf_attention_dims* dims, const void* q, const void* k, const void* v,
+                                   const float* log_decay, const float* s0, const int32_t* lengths, void* o, float* sT,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  KfAttnArgs a;
+  int rc = attention_args(h, dims, "kf_linear_attention", &a);
+  if (rc) return rc;
+  if (!q || !k || !v || !log_decay || !o) {
+    KF_SET_ERR(h, "kf_linear_attention: q, k, v, log_decay and o must be non-NULL");
+    return KF_ERR_ARG;
+  }
+  rc = workspace_ok(h, "kf_linear_attention", kf_attention_workspace(h, a, false), workspace, workspace_bytes);
+  if (rc) return rc;
+  KF_ON_DEVICE(h);
+  a.q = q; a.k = k; a.v = v; a.log_decay = log_decay; a.s0 = s0; a.lengths = lengths; a.o = o; a.sT = sT;
+  return kf_launch_attention(h, a, workspace, (hipStream_t)stream);
+}
+
+extern "C" int kf_linear_attention_backward(kf_handle* h, const kf_attention_dims* dims, const void* q, const void* k, const void* v,
+                                            const float* log_decay, const float* s0, const int32_t* lengths, const void* g_o,
+                                            const float* g_sT, void* g_q, void* g_k, void* g_v, float* g_log_decay, float* g_s0,
+                                            void* workspace, size_t workspace_bytes, void* stream) {
+  KfAttnArgs a;
+  int rc = attention_args(h, dims, "kf_linear_attention_backward", &a);
+  if (rc) return rc;
+  if (!q || !k || !v || !log_decay || !g_o || !g_q || !g_k || !g_v || !g_log_decay) {
+    KF_SET_ERR(h, "kf_linear_attention_backward: only s0, lengths, g_sT and g_s0 may be NULL");
+    return KF_ERR_ARG;
+  }
+  if (dims->g_o_stride[0] < 0 || dims->g_o_stride[1] < 0 || dims->g_o_stride[2] < 0) {
+    KF_SET_ERR(h, "kf_linear_attention_backward: strides must not be negative");
+    return KF_ERR_ARG;
+  }
+  rc = workspace_ok(h, "kf_linear_attention_backward", kf_attention_workspace(h, a, true), workspace, workspace_bytes);
+  if (rc) return rc;
+  KF_ON_DEVICE(h);
+  a.q = q; a.k = k; a.v = v; a.log_decay = log_decay; a.s0 = s0; a.lengths = lengths; a.g_o = g_o; a.g_sT = g_sT;
+  a.g_q = g_q; a.g_k = g_k; a.g_v = g_v; a.g_decay = g_log_decay; a.g_s0 = g_s0;
+  return kf_launch_attention_backward(h, a, workspace, (hipStream_t)stream);
+}
+
+extern "C" int kf_linear_attention_step(kf_handle* h, const kf_attention_dims* dims, const void* q, const void* k, const void* v,
+                                        const float* log_decay, const int32_t* slots, int64_t n_slots, const float* state,
+                                        float* state_out, void* o, int32_t* info, void* stream) {
+  KfAttnArgs c;
+  kf_attention_dims d1;
+  if (dims) {
+    d1 = *dims;
+    d1.T = 1;
+    for (int64_t* st : {d1.q_stride, d1.k_stride, d1.v_stride}) st[1] = 0;
+  }
+  const int rc = attention_args(h, dims ? &d1 : nullptr, "kf_linear_attention_step", &c);
+  if (rc) return rc;
+  if (!q || !k || !v || !log_decay || !state || !state_out || !o) {
+    KF_SET_ERR(h, "kf_linear_attention_step: only slots and info may be NULL");
+    return KF_ERR_ARG;
+  }
+  if (n_slots < 1 || n_slots > 0x7fffffffL || (!slots && n_slots < c.B)) {
+    KF_SET_ERR(h, "kf_linear_attention_step: n_slots=%ld for B=%ld rows%s", (long)n_slots, (long)c.B, slots ? "" : " without slots");
+    return KF_ERR_ARG;
+  }
+  KF_ON_DEVICE(h);
+  KfAttnStepArgs a;
+  a.B = c.B; a.n_slots = n_slots; a.G = c.G; a.H = c.H; a.K = c.K; a.V = c.V; a.dtype = c.dtype; a.per_row = c.per_token; a.scale = c.scale;
+  a.q = q; a.k = k; a.v = v; a.log_decay = log_decay; a.slots = slots; a.state = state; a.state_out = state_out; a.o = o; a.info = info;
+  a.qs[0] = c.qs[0]; a.qs[1] = c.qs[2]; a.ks[0] = c.ks[0]; a.ks[1] = c.ks[2]; a.vs[0] = c.vs[0]; a.vs[1] = c.vs[2];
+  return kf_launch_attention_step(h, a, (hipStream_t)stream);
+}
+
+static int orthogonalise_args(kf_handle* h, int64_t n, int32_t rows, int32_t cols, int32_t dtype, const char* which, KfOrthArgs* a) {
+  if (!h) return KF_ERR_ARG;
+  if (n < 1 || rows < 1 || cols < 1) {
+    KF_SET_ERR(h, "%s: sizes must be positive (n=%ld rows=%d cols=%d)", which, (long)n, rows, cols);
+    return KF_ERR_ARG;
+  }
+  if (n > 65535 * 64L || rows > (1 << 17) || cols > (1 << 24) || (rows > cols && (rows > (1 << 24) || cols > (1 << 17))) ||
+      (double)n * rows * cols > 1.0e12) {
+    KF_SET_ERR(h, "%s: n=%ld rows=%d cols=%d is too large", which, (long)n, rows, cols);
+    return KF_ERR_UNSUPPORTED;
+  }
+  if (dtype < KF_DTYPE_F64 || dtype > KF_DTYPE_F16) {
+    KF_SET_ERR(h, "%s: dtype %d is none of KF_DTYPE_*", which, dtype);
+    return KF_ERR_UNSUPPORTED;
+  }
+  memset(a, 0, sizeof(*a));
+  a->n = n; a->rows = rows; a->cols = cols; a->dtype = dtype;
+  return KF_OK;
+}
+
+extern "C" int kf_orthogonalise_workspace(kf_handle* h, int64_t n, int32_t rows, int32_t cols, int32_t dtype, size_t* bytes) {
+  KfOrthArgs a;
+  const int rc = orthogonalise_args(h, n, rows, cols, dtype, "kf_orthogonalise_workspace", &a);
+  if (rc) return rc;
+  if (!bytes) {
+    KF_SET_ERR(h, "kf_orthogonalise_workspace: bytes is NULL");
+    return KF_ERR_ARG;
+  }
+  *bytes = kf_orthogonalise_ws(h, a);
+  return KF_OK;
+}
+
+// The largest |a s + b s^3 + c s^5| over 0 <= s <= top: at top or where the derivative a + 3 b u + 5 c u^2 (u = s^2) vanishes.
+static double quintic_top(const double* p, double top) {
+  const double a = p[0], b = p[1], c = p[2];
+  double best = fabs(top * (a + top * top * (b + c * top * top)));
+  double u[2];
+  int n = 0;
+  if (c != 0.0) {
+    const double disc = 9 * b * b - 20 * a * c;
+    if (disc >= 0) {
+      u[n++] = (-3 * b + sqrt(disc)) / (10 * c);
+      u[n++] = (-3 * b - sqrt(disc)) / (10 * c);
+    }
+  } else if (b != 0.0) {
+    u[n++] = -a / (3 * b);
+  }
+  for (int i = 0; i < n; ++i)
+    if (u[i] > 0 && u[i] < top * top) {
+      const double s = sqrt(u[i]);
+      best = fmax(best, fabs(s * (a + u[i] * (b + c * u[i]))));
+    }
+  return best;
+}
+
+extern "C" int kf_orthogonalise(kf_handle* h, int64_t n, int32_t rows, int32_t cols, int32_t dtype, int32_t n_steps,
+                                const double* coefficients, double eps, const void* M, void* X, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  KfOrthArgs a;
+  int rc = orthogonalise_args(h, n, rows, cols, dtype, "kf_orthogonalise", &a);
+  if (rc) return rc;
+  if (n_steps < 1 || n_steps > KF_ORTHOGONALISE_STEPS_MAX || !coefficients || !M || !X || M == X || !(eps >= 0.0 && eps < 1e300)) {
+    KF_SET_ERR(h, "kf_orthogonalise: needs 1 <= n_steps <= %d, coefficients, M, X apart from M, and a finite eps >= 0",
+               KF_ORTHOGONALISE_STEPS_MAX);
+    return KF_ERR_ARG;
+  }
+  double top = 1.0;
+  for (int s = 0; s < n_steps; ++s) {
+    for (int i = 0; i < 3; ++i) {
+      a.coef[s][i] = coefficients[3 * s + i];
+      if (!(fabs(a.coef[s][i]) <= 1e3)) {
+        KF_SET_ERR(h, "kf_orthogonalise: coefficient %d of step %d is not a number within 1000", i, s);
+        return KF_ERR_ARG;
+      }
+    }
+    top = quintic_top(a.coef[s], top);
+    if (!(top <= 1.9)) {
+      KF_SET_ERR(h, "kf_orthogonalise: step %d can carry a singular value to %g (at most 1.9)", s, top);
+      return KF_ERR_ARG;
+    }
+  }
+  a.steps = n_steps; a.eps = eps; a.M = M; a.X = X;
+  rc = workspace_ok(h, "kf_orthogonalise", kf_orthogonalise_ws(h, a), workspace, workspace_bytes);
+  if (rc) return rc;
+  KF_ON_DEVICE(h);
+  return kf_launch_orthogonalise(h, a, workspace, (hipStream_t)stream);
 }
