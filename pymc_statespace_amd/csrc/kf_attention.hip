@@ -8,52 +8,6 @@ namespace {
 
 constexpr int MAXD = 128;  // the largest K and V
 
-// one workgroup per (sequence, head, 64 columns of V): a thread holds one column of the state
-template <typename T>
-__global__ __launch_bounds__(64) void attention_forward_kernel(KfAttnArgs a) {
-  __shared__ float sq[MAXD], sk[MAXD];
-  const long bh = blockIdx.x;
-  const long b = bh / a.H;
-  const int h = (int)(bh - b * a.H), g = h / (a.H / a.G);
-  const int c = blockIdx.y * 64 + threadIdx.x;
-  const bool on = c < a.V;
-  const long n = kf_row_length(a.lengths, b, a.T);
-  float S[MAXD];
-#pragma unroll
-  for (int i = 0; i < MAXD; ++i) S[i] = (a.s0 && on && i < a.K) ? a.s0[(bh * a.K + i) * a.V + c] : 0.f;
-  const T* q = (const T*)a.q + b * a.qs[0] + g * a.qs[2];
-  const T* k = (const T*)a.k + b * a.ks[0] + g * a.ks[2];
-  const T* v = (const T*)a.v + b * a.vs[0] + h * a.vs[2];
-  T* o = (T*)a.o;
-  for (long t = 0; t < a.T; ++t) {
-    const long at = ((b * a.T + t) * a.H + h) * a.V + c;
-    if (t >= n) {
-      if (on) o[at] = kf_from_float<T>(0.f);
-      continue;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < MAXD; i += 64) {
-      sq[i] = i < a.K ? kf_to_float(q[t * a.qs[1] + i]) : 0.f;
-      sk[i] = i < a.K ? kf_to_float(k[t * a.ks[1] + i]) : 0.f;
-    }
-    __syncthreads();
-    const float d = expf(kf_clamp_log_decay(a.per_token ? a.log_decay[(b * a.T + t) * a.H + h] : a.log_decay[h]));
-    const float vt = on ? kf_to_float(v[t * a.vs[1] + c]) : 0.f;
-    float r = 0.f;
-#pragma unroll
-    for (int i = 0; i < MAXD; ++i) {
-      S[i] = d * S[i] + sk[i] * vt;
-      r += sq[i] * S[i];
-    }
-    if (on) o[at] = kf_from_float<T>(a.scale * r);
-  }
-  if (a.sT && on) {
-#pragma unroll
-    for (int i = 0; i < MAXD; ++i)
-      if (i < a.K) a.sT[(bh * a.K + i) * a.V + c] = S[i];
-  }
-}
-
 // MODE 0: dq, forward in time, a thread per row of S.  MODE 1: dk and dS_0, backward, a thread per row of R.
 // MODE 2: dv, backward, a thread per column of R.  dq, dk per head in 32 bits (summed over a group's heads afterwards).
 template <typename T, int MODE>
@@ -250,13 +204,6 @@ __global__ __launch_bounds__(64) void attention_step_kernel(KfAttnStepArgs a) {
 }
 
 template <typename T>
-int forward_t(kf_handle* h, const KfAttnArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL(attention_forward_kernel<T>, dim3((unsigned)(a.B * a.H), (a.V + 63) / 64), dim3(64), 0, stream, a);
-  KF_HIP_CHECK(h, hipGetLastError());
-  return KF_OK;
-}
-
-template <typename T>
 int backward_t(kf_handle* h, const KfAttnArgs& a, void* ws, hipStream_t stream) {
   const size_t rows = (size_t)a.B * a.T * a.H;
   char* w = (char*)ws;
@@ -286,18 +233,10 @@ int step_t(kf_handle* h, const KfAttnStepArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-size_t kf_attention_workspace(const kf_handle*, const KfAttnArgs& a, bool backward) {
-  if (!backward) return 0;
+size_t kf_attention_workspace(const kf_handle* h, const KfAttnArgs& a, bool backward) {
+  if (!backward) return kf_attention_forward_workspace(h, a);
   const size_t rows = (size_t)a.B * a.T * a.H;
   return 2 * kf_seq_round(rows * a.K * 4) + 2 * kf_seq_round((size_t)a.B * a.H * 4);
-}
-
-int kf_launch_attention(kf_handle* h, const KfAttnArgs& a, void*, hipStream_t stream) {
-  switch (a.dtype) {
-    case KF_DTYPE_F32: return forward_t<float>(h, a, stream);
-    case KF_DTYPE_BF16: return forward_t<__hip_bfloat16>(h, a, stream);
-    default: return forward_t<__half>(h, a, stream);
-  }
 }
 
 int kf_launch_attention_backward(kf_handle* h, const KfAttnArgs& a, void* ws, hipStream_t stream) {

@@ -38,6 +38,7 @@ struct KfAttnStepArgs {
 };
 
 size_t kf_attention_workspace(const kf_handle* h, const KfAttnArgs& a, bool backward);
+size_t kf_attention_forward_workspace(const kf_handle* h, const KfAttnArgs& a);
 int kf_launch_attention(kf_handle* h, const KfAttnArgs& a, void* ws, hipStream_t stream);
 int kf_launch_attention_backward(kf_handle* h, const KfAttnArgs& a, void* ws, hipStream_t stream);
 int kf_launch_attention_step(kf_handle* h, const KfAttnStepArgs& a, hipStream_t stream);
