@@ -511,7 +511,7 @@ KF_API int kf_linear_attention_workspace(kf_handle* h, const kf_attention_dims* 
  * o [B][T][H][V]; sT [B][H][K][V] fp32, the state behind each sequence's last token (may be NULL; may be s0).  log_decay is fp32 and
  * meant to be <= 0; anything below -1e4, -infinity included, is a reset of the state.  lengths [B] int32 (NULL: all T): tokens from
  * lengths[b] on (clamped to 0 .. T) are not read, o is zero there and the state stays.  The state, its sums and the decays are held
- * in 32 bits; o is rounded once more than the state where dtype is 16 bits wide (see kf_attention.hip). */
+ * in 32 bits; o is rounded once more than the state where dtype is 16 bits wide (see kf_attention_forward.hip). */
 KF_API int kf_linear_attention(kf_handle* h, const kf_attention_dims* dims, const void* q, const void* k, const void* v,
                                const float* log_decay, const float* s0, const int32_t* lengths, void* o, float* sT,
                                void* workspace, size_t workspace_bytes, void* stream);

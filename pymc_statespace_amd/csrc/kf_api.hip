@@ -1621,7 +1621,7 @@ extern "C" int kf_linear_attention_workspace(kf_handle* h, const kf_attention_di
     KF_SET_ERR(h, "kf_linear_attention_workspace: bytes is NULL");
     return KF_ERR_ARG;
   }
-  *bytes = kf_attention_workspace(h, a, backward != 0);
+  *bytes = backward ? kf_attention_backward_workspace(h, a) : kf_attention_forward_workspace(h, a);
   return KF_OK;
 }
 
@@ -1635,7 +1635,7 @@ extern "C" int kf_linear_attention(kf_handle* h, const kf_attention_dims* dims, 
     KF_SET_ERR(h, "kf_linear_attention: q, k, v, log_decay and o must be non-NULL");
     return KF_ERR_ARG;
   }
-  rc = workspace_ok(h, "kf_linear_attention", kf_attention_workspace(h, a, false), workspace, workspace_bytes);
+  rc = workspace_ok(h, "kf_linear_attention", kf_attention_forward_workspace(h, a), workspace, workspace_bytes);
   if (rc) return rc;
   KF_ON_DEVICE(h);
   a.q = q; a.k = k; a.v = v; a.log_decay = log_decay; a.s0 = s0; a.lengths = lengths; a.o = o; a.sT = sT;
@@ -1657,7 +1657,7 @@ extern "C" int kf_linear_attention_backward(kf_handle* h, const kf_attention_dim
     KF_SET_ERR(h, "kf_linear_attention_backward: strides must not be negative");
     return KF_ERR_ARG;
   }
-  rc = workspace_ok(h, "kf_linear_attention_backward", kf_attention_workspace(h, a, true), workspace, workspace_bytes);
+  rc = workspace_ok(h, "kf_linear_attention_backward", kf_attention_backward_workspace(h, a), workspace, workspace_bytes);
   if (rc) return rc;
   KF_ON_DEVICE(h);
   a.q = q; a.k = k; a.v = v; a.log_decay = log_decay; a.s0 = s0; a.lengths = lengths; a.g_o = g_o; a.g_sT = g_sT;

@@ -1,0 +1,578 @@
+// kf_attention_backward.hip -- the gradient of linear attention with a decay for each head, in chunks of C tokens.
+//
+// With S_0 the state at a chunk's start, R = dL/dS behind its last token, G_i the log decays summed through token i, E the chunk's
+// whole decay, D_ij = e^{G_i - G_j} for j <= i, A_ij = q_i . k_j, B_ij = do_i . v_j:
+//     dq_i = s [ e^{G_i} S_0 do_i + sum_j D_ij B_ij k_j ]
+//     dk_j = e^{G_C - G_j} R v_j + s sum_i D_ij B_ij q_i
+//     dv_j = e^{G_C - G_j} R' k_j + s sum_i D_ij A_ij do_i
+//     dL/d log a_t = sum_{i >= t} (sum_j W_ij + q_i . dq_i|state) - sum_{j >= t} sum_i W_ij + sum_{j < t} k_j . dk_j|state + E <R, S_0>
+// with W_ij = s D_ij A_ij B_ij: what passes through the decay of token t.  All of it from this chunk's own numbers (the shorter form,
+// a running sum of q.dq - k.dk over the whole sequence, loses what those sums share).  Then R <- E R + sum_i s e^{G_i} q_i do_i'.
+//
+// Launches: (1) where the time axis is cut into segments, what each segment adds to S and to R; (2) S at every chunk's start, kept
+// in the layout of the operand it becomes; (3) the chunks of each segment from its last to its first, R in registers; (4) sums over
+// the heads that share queries and keys, and over tokens for fixed decays.
+#include "kf_attention_chunk.h"
+
+namespace {
+
+// K and V are padded to one size D; a workgroup has D / 16 waves, wave w has columns 16 w .. of K (in dv: of V).
+template <typename A> constexpr int chunk_of() { return A::PAD == 8 ? 64 : 32; }  // fp32 tiles are twice as wide: half as many tokens
+
+struct Split {
+  long works;
+  int segments, seg_chunks;
+  long chunks;
+  int vec_q, vec_k, vec_v, vec_g;
+  float *adds_s, *adds_r, *factors;  // [B H][segments - 1][D D], [B H][segments] (each segment's whole decay)
+  kf_u32x4* starts;                  // S_0 of every chunk: [B H][chunks][D / 32][2][threads]
+  float *part_q, *part_k;            // [B][T][H][K], where heads share q and k
+  double* part_decay;                // [B H][segments], where decays are fixed
+};
+
+template <int C, typename A, typename T, int D>
+struct Stage {  // C rows of a tensor through registers into LDS
+  static constexpr int N = C * D / 8 / (4 * D), LD = D + A::PAD;
+  typename A::frag r[N];
+  __device__ __forceinline__ void load(const T* p, long stride, long t0, long n, int dim, bool vec) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int x = threadIdx.x + 4 * D * u, row = x / (D / 8), col = 8 * (x % (D / 8));
+      r[u] = KfLoad8<A, T>::load(p + (t0 + row) * stride + col, t0 + row < n ? dim - col : 0, vec);
+    }
+  }
+  __device__ __forceinline__ void put(typename A::elem* s) const {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int x = threadIdx.x + 4 * D * u;
+      A::put8(s + (x / (D / 8)) * LD + 8 * (x % (D / 8)), r[u]);
+    }
+  }
+};
+
+// One sweep over a segment's chunks of acc[v][k] <- E acc + sum_t weight_t y_t x_t': S (x = k, y = v, forward in time) or R (x = q,
+// y = do, backward).  STARTS: S, started from the segments before, kept at every chunk's start; else what the segment adds.
+template <typename A, typename T, int D, bool STARTS>
+__global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Split sp) {
+  constexpr int C = chunk_of<A>(), LD = D + A::PAD, NT = D / 16, TH = 4 * D;
+  typedef typename A::elem E;
+  __shared__ __attribute__((aligned(16))) E sX[C * LD];
+  __shared__ __attribute__((aligned(16))) E sY[C * LD];
+  __shared__ KfChunkDecay<C> dec[2];
+  const long work = kf_xcd_work(sp.works);
+  if (work >= sp.works) return;
+  const int segs = STARTS ? sp.segments : sp.segments - 1;
+  long rest = work;
+  bool back = false;
+  if (!STARTS) {
+    back = rest & 1;
+    rest >>= 1;
+  }
+  const int h = (int)(rest % a.H);
+  rest /= a.H;
+  const int s0 = (int)(rest % segs);
+  const long b = rest / segs;
+  const int seg = back ? s0 + 1 : s0;  // (nothing is behind the last segment, nothing before the first)
+  const long bh = b * a.H + h;
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, i = l & 15, g = l >> 4;
+  const long n = kf_row_length(a.lengths, b, a.T);
+  const int grp = h / (a.H / a.G);
+  const T* x = back ? (const T*)a.q + b * a.qs[0] + grp * a.qs[2] : (const T*)a.k + b * a.ks[0] + grp * a.ks[2];
+  const T* y = back ? (const T*)a.g_o + b * a.gs[0] + h * a.gs[2] : (const T*)a.v + b * a.vs[0] + h * a.vs[2];
+  const long xs = back ? a.qs[1] : a.ks[1], ys = back ? a.gs[1] : a.vs[1];
+  const bool vx = back ? sp.vec_q : sp.vec_k, vy = back ? sp.vec_g : sp.vec_v;
+  const float* ld = a.log_decay + (a.per_token ? b * a.T * a.H + h : (long)h);
+  const long c0 = (long)seg * sp.seg_chunks, c1 = c0 + sp.seg_chunks < sp.chunks ? c0 + sp.seg_chunks : sp.chunks;
+  const long live = (n + C - 1) / C, last = c1 < live ? c1 : live;  // chunks that hold tokens: c0 .. last - 1
+
+  kf_f32x4 acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    acc[t] = kf_f32x4{0, 0, 0, 0};
+    const int kk = 16 * w + i;
+    if (STARTS && a.s0 && kk < a.K) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (16 * t + 4 * g + r < a.V) acc[t][r] = a.s0[(bh * a.K + kk) * a.V + 16 * t + 4 * g + r];
+    }
+  }
+  if (STARTS) {
+    for (int s = 0; s < seg; ++s) {
+      const float f = sp.factors[bh * sp.segments + s];
+      const kf_f32x4* u = reinterpret_cast<const kf_f32x4*>(sp.adds_s) + (bh * (sp.segments - 1) + s) * (D * D / 4) + tid;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t] = acc[t] * f + u[t * TH];
+    }
+  }
+  float through = 1.f;
+  Stage<C, A, T, D> rx, ry;
+  float rg = 0.f;
+  const long steps = last > c0 ? last - c0 : 0;
+  auto at = [&](long s) { return back ? last - 1 - s : c0 + s; };
+  auto decay_of = [&](long c) { return l < C && c * C + l < n ? (a.per_token ? ld[(c * C + l) * a.H] : ld[0]) : 0.f; };
+  if (steps) {
+    rx.load(x, xs, at(0) * C, n, a.K, vx);
+    ry.load(y, ys, at(0) * C, n, a.V, vy);
+    if (w == 0) dec[0].fill(decay_of(at(0)), l < C && at(0) * C + l < n);
+  }
+  for (long s = 0; s < steps; ++s) {
+    if (STARTS) {
+      kf_u32x4* out = sp.starts + (bh * sp.chunks + at(s)) * (D / 32 * 2 * TH) + tid;
+#pragma unroll
+      for (int u = 0; u < D / 32; ++u) {
+        KfSplit<A> f;
+        f.set(acc[2 * u], acc[2 * u + 1]);
+        out[(2 * u) * TH] = f.piece(0);
+        out[(2 * u + 1) * TH] = f.piece(1);
+      }
+      if (s + 1 == steps && seg == sp.segments - 1) break;  // the state behind the last token is not asked for
+    }
+    rx.put(sX);
+    ry.put(sY);
+    __syncthreads();
+    const bool more = s + 1 < steps;
+    const int wd = (int)((s + 1) % NT);  // the wave that computes the next chunk's decays
+    if (more) {
+      rx.load(x, xs, at(s + 1) * C, n, a.K, vx);
+      ry.load(y, ys, at(s + 1) * C, n, a.V, vy);
+      if (w == wd) rg = decay_of(at(s + 1));
+    }
+    const KfChunkDecay<C>& d = dec[s & 1];
+    const float fe = d.from_start[C - 1];
+    through *= fe;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] *= fe;
+#pragma unroll
+    for (int u = 0; u < C / 32; ++u) {
+      float wt[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int tok = 32 * u + 16 * (e >> 2) + 4 * g + (e & 3);
+        wt[e] = back ? d.from_start[tok] * a.scale : d.to_end[tok];
+      }
+      KfWeighted<A> xw;
+      xw.set(A::col(sX + 32 * u * LD + 16 * w, LD, i, g), wt);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t] = xw.mma_right(A::col(sY + 32 * u * LD + 16 * t, LD, i, g), acc[t]);
+    }
+    if (more && w == wd) dec[(s + 1) & 1].fill(rg, l < C && at(s + 1) * C + l < n);
+    __syncthreads();
+  }
+  if (!STARTS) {
+    kf_f32x4* u = reinterpret_cast<kf_f32x4*>(back ? sp.adds_r : sp.adds_s) + (bh * (sp.segments - 1) + s0) * (D * D / 4) + tid;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) u[t * TH] = acc[t];
+    // (each segment's decay from one of the sweeps that pass through it: the first from S, the others from R)
+    if (tid == 0 && (back || s0 == 0)) sp.factors[bh * sp.segments + seg] = through;
+  }
+}
+
+template <typename A, typename T, int D>
+__global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a, Split sp) {
+  constexpr int C = chunk_of<A>(), LD = D + A::PAD, LP = C + A::PAD, NT = D / 16, CT = C / 16, TH = 4 * D;
+  typedef typename A::elem E;
+  typedef typename A::frag F;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  E* sQ = (E*)smem;
+  E* sK = sQ + C * LD;
+  E* sV = sK + C * LD;
+  E* sG = sV + C * LD;
+  E* sR = sG + C * LD;   // R as an operand, [k][v]
+  E* sP = sR + D * LD;   // s D A, [i][j]
+  E* sB = sP + C * LP;   // s D B
+  KfChunkDecay<C>* dec = (KfChunkDecay<C>*)(sB + C * LP);
+  float* rs = (float*)(dec + 2);  // [CT][C]: sums of W over the columns of one tile
+  float* cs = rs + CT * C;        // [CT][C]: over the rows
+  float* xs = cs + CT * C;        // [NT][C]: q . dq|state, this wave's columns of K
+  float* ys = xs + NT * C;        // [NT][C]: k . dk|state
+  float* cr = ys + NT * C;        // [NT]: <R, S_0>
+
+  const long work = kf_xcd_work(sp.works);
+  if (work >= sp.works) return;
+  long rest = work;
+  const int h = (int)(rest % a.H);
+  rest /= a.H;
+  const int seg = (int)(rest % sp.segments);
+  const long b = rest / sp.segments;
+  const long bh = b * a.H + h;
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, i = l & 15, g = l >> 4;
+  const long n = kf_row_length(a.lengths, b, a.T);
+  const int grp = h / (a.H / a.G);
+  const T* q = (const T*)a.q + b * a.qs[0] + grp * a.qs[2];
+  const T* k = (const T*)a.k + b * a.ks[0] + grp * a.ks[2];
+  const T* v = (const T*)a.v + b * a.vs[0] + h * a.vs[2];
+  const T* go = (const T*)a.g_o + b * a.gs[0] + h * a.gs[2];
+  const float* ld = a.log_decay + (a.per_token ? b * a.T * a.H + h : (long)h);
+  const long c0 = (long)seg * sp.seg_chunks, c1 = c0 + sp.seg_chunks < sp.chunks ? c0 + sp.seg_chunks : sp.chunks;
+  const long live = (n + C - 1) / C, last = c1 < live ? c1 : live;
+  const bool shared_heads = a.G != a.H;
+
+  kf_f32x4 R[NT];  // rows v, columns k
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    R[t] = kf_f32x4{0, 0, 0, 0};
+    const int kk = 16 * w + i;
+    if (a.g_sT && kk < a.K) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (16 * t + 4 * g + r < a.V) R[t][r] = a.g_sT[(bh * a.K + kk) * a.V + 16 * t + 4 * g + r];
+    }
+  }
+  for (int s = sp.segments - 1; s > seg; --s) {
+    const float f = sp.factors[bh * sp.segments + s];
+    const kf_f32x4* u = reinterpret_cast<const kf_f32x4*>(sp.adds_r) + (bh * (sp.segments - 1) + s - 1) * (D * D / 4) + tid;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) R[t] = R[t] * f + u[t * TH];
+  }
+
+  // gradients of rows behind the sequence's end
+  {
+    const long lo = (last > c0 ? last : c0) * C, hi = c1 * C < a.T ? c1 * C : a.T;
+    for (long t = lo + tid / D; t < hi; t += 4) {
+      const int c = tid % D;
+      const long row = (b * a.T + t) * a.H + h;
+      if (c < a.V) ((T*)a.g_v)[row * a.V + c] = kf_from_float<T>(0.f);
+      if (c < a.K) {
+        if (shared_heads) {
+          sp.part_q[row * a.K + c] = 0.f;
+          sp.part_k[row * a.K + c] = 0.f;
+        } else {
+          ((T*)a.g_q)[row * a.K + c] = kf_from_float<T>(0.f);
+          ((T*)a.g_k)[row * a.K + c] = kf_from_float<T>(0.f);
+        }
+      }
+      if (a.per_token && c == 0) a.g_decay[row] = 0.f;
+    }
+  }
+  for (int x = tid; x < 2 * C * LP; x += TH) sP[x] = E(0);  // tiles above the diagonal stay zero
+
+  Stage<C, A, T, D> rq, rk, rv, rd;
+  float rg = 0.f;
+  kf_u32x4 S0[D / 32][2];
+  auto load = [&](long c) {
+    rq.load(q, a.qs[1], c * C, n, a.K, sp.vec_q);
+    rk.load(k, a.ks[1], c * C, n, a.K, sp.vec_k);
+    rv.load(v, a.vs[1], c * C, n, a.V, sp.vec_v);
+    rd.load(go, a.gs[1], c * C, n, a.V, sp.vec_g);
+  };
+  auto load_start = [&](long c) {
+    const kf_u32x4* in = sp.starts + (bh * sp.chunks + c) * (D / 32 * 2 * TH) + tid;
+#pragma unroll
+    for (int u = 0; u < D / 32; ++u) {
+      S0[u][0] = in[(2 * u) * TH];
+      S0[u][1] = in[(2 * u + 1) * TH];
+    }
+  };
+  auto decay_of = [&](long c) { return l < C && c * C + l < n ? (a.per_token ? ld[(c * C + l) * a.H] : ld[0]) : 0.f; };
+  if (last > c0) {
+    load(last - 1);
+    load_start(last - 1);
+    if (w == 0) dec[0].fill(decay_of(last - 1), l < C && (last - 1) * C + l < n);
+  }
+  double decay_sum = 0.;
+  int turn = 0;
+  for (long c = last - 1; c >= c0; --c, turn ^= 1) {
+    const long t0 = c * C;
+    rq.put(sQ);
+    rk.put(sK);
+    rv.put(sV);
+    rd.put(sG);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) A::put4(sR + (16 * w + i) * LD + 16 * t + 4 * g, R[t]);
+    __syncthreads();
+    const bool more = c > c0;
+    if (more) {
+      load(c - 1);
+      if (w == 0) rg = decay_of(c - 1);
+    }
+    const KfChunkDecay<C>& d = dec[turn];
+
+    // scores: tile (it, jt) of A and B, rows j, columns i
+    for (int x = w; x < CT * (CT + 1) / 2; x += NT) {
+      int it = 0;
+      while ((it + 1) * (it + 2) / 2 <= x) ++it;
+      const int jt = x - it * (it + 1) / 2, row = 16 * it + i;
+      kf_f32x4 sa = {0, 0, 0, 0}, sb = {0, 0, 0, 0};
+#pragma unroll
+      for (int u = 0; u < D / 32; ++u) {
+        sa = A::mma(A::row(sK + (16 * jt + i) * LD + 32 * u + 8 * g), A::row(sQ + row * LD + 32 * u + 8 * g), sa);
+        sb = A::mma(A::row(sV + (16 * jt + i) * LD + 32 * u + 8 * g), A::row(sG + row * LD + 32 * u + 8 * g), sb);
+      }
+      kf_f32x4 p, pb, wj;
+      float wi = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = 16 * jt + 4 * g + r;
+        const bool in = j <= row;
+        const float f = a.scale * (it == jt ? d.pair(row, j) : d.from_tile[jt < CT - 1 ? jt : 0][row] * d.to_tile_end[j]);
+        p[r] = in ? sa[r] * f : 0.f;
+        pb[r] = in ? sb[r] * f : 0.f;
+        wj[r] = in ? sa[r] * pb[r] : 0.f;
+        wi += wj[r];
+      }
+      A::put4(sP + row * LP + 16 * jt + 4 * g, p);
+      A::put4(sB + row * LP + 16 * jt + 4 * g, pb);
+      wi += __shfl_xor(wi, 16);
+      wi += __shfl_xor(wi, 32);
+      if (g == 0) rs[jt * C + row] = wi;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int m = 1; m < 16; m *= 2) wj[r] += __shfl_xor(wj[r], m);
+        if (i == 0) cs[it * C + 16 * jt + 4 * g + r] = wj[r];
+      }
+    }
+
+    // through the states; rows k (dv: rows v), columns tokens
+    kf_f32x4 dq[CT], dk[CT], dv[CT];
+#pragma unroll
+    for (int t = 0; t < CT; ++t) dq[t] = dk[t] = dv[t] = kf_f32x4{0, 0, 0, 0};
+    float cross = 0.f;
+#pragma unroll
+    for (int u = 0; u < D / 32; ++u) {
+      KfSplit<A> fs, fr;
+      fs.pieces(S0[u][0], S0[u][1]);
+      fr.set(R[2 * u], R[2 * u + 1]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) cross += fs.value(e) * R[2 * u + (e >> 2)][e & 3];
+      const F fc = A::col(sR + 32 * u * LD + 16 * w, LD, i, g);  // rows v of this wave, depth k
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        dq[t] = fs.mma(A::row_t(sG + (16 * t + i) * LD + 32 * u + 4 * g), dq[t]);
+        dk[t] = fr.mma(A::row_t(sV + (16 * t + i) * LD + 32 * u + 4 * g), dk[t]);
+        dv[t] = A::mma(fc, A::row_t(sK + (16 * t + i) * LD + 32 * u + 4 * g), dv[t]);
+      }
+    }
+    if (more) load_start(c - 1);
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) cross += __shfl_xor(cross, m);
+    if (l == 0) cr[w] = cross;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      const int tok = 16 * t + i;
+      const float fi = a.scale * d.from_start[tok], fj = d.to_end[tok];
+      dq[t] *= fi;
+      dk[t] *= fj;
+      dv[t] *= fj;
+      const kf_f32x4 qv = A::get4(sQ + tok * LD + 16 * w + 4 * g), kv = A::get4(sK + tok * LD + 16 * w + 4 * g);
+      float x = 0.f, y = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x += qv[r] * dq[t][r];
+        y += kv[r] * dk[t][r];
+      }
+      x += __shfl_xor(x, 16);
+      x += __shfl_xor(x, 32);
+      y += __shfl_xor(y, 16);
+      y += __shfl_xor(y, 32);
+      if (g == 0) {
+        xs[w * C + tok] = x;
+        ys[w * C + tok] = y;
+      }
+    }
+    __syncthreads();
+
+    // inside the chunk, and R at its start
+    const float fe = d.from_start[C - 1];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) R[t] *= fe;
+#pragma unroll
+    for (int u = 0; u < C / 32; ++u) {
+      const F ck = A::col(sK + 32 * u * LD + 16 * w, LD, i, g), cq = A::col(sQ + 32 * u * LD + 16 * w, LD, i, g),
+              cg = A::col(sG + 32 * u * LD + 16 * w, LD, i, g);
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        if (2 * u <= t) dq[t] = A::mma(ck, A::row_t(sB + (16 * t + i) * LP + 32 * u + 4 * g), dq[t]);
+        if (2 * u + 1 >= t) {
+          dk[t] = A::mma(cq, A::col(sB + 32 * u * LP + 16 * t, LP, i, g), dk[t]);
+          dv[t] = A::mma(cg, A::col(sP + 32 * u * LP + 16 * t, LP, i, g), dv[t]);
+        }
+      }
+      float wt[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wt[e] = a.scale * d.from_start[32 * u + 16 * (e >> 2) + 4 * g + (e & 3)];
+      KfWeighted<A> qw;
+      qw.set(cq, wt);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) R[t] = qw.mma_right(A::col(sG + 32 * u * LD + 16 * t, LD, i, g), R[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      const long tok = t0 + 16 * t + i, row = (b * a.T + tok) * a.H + h;
+      const int c4 = 16 * w + 4 * g;
+      if (tok < a.T) {
+        if (tok >= n) dq[t] = dk[t] = dv[t] = kf_f32x4{0, 0, 0, 0};
+        kf_store4((T*)a.g_v + row * a.V + c4, dv[t], a.V - c4, a.V % 4 == 0);
+        if (shared_heads) {
+          kf_store4(sp.part_q + row * a.K + c4, dq[t], a.K - c4, a.K % 4 == 0);
+          kf_store4(sp.part_k + row * a.K + c4, dk[t], a.K - c4, a.K % 4 == 0);
+        } else {
+          kf_store4((T*)a.g_q + row * a.K + c4, dq[t], a.K - c4, a.K % 4 == 0);
+          kf_store4((T*)a.g_k + row * a.K + c4, dk[t], a.K - c4, a.K % 4 == 0);
+        }
+      }
+    }
+    if (w == 0) {
+      // d log a: token t0 + l (its sums are complete since the barrier above)
+      const bool tok = l < C;
+      double up = 0., down = 0., all = 0.;
+      if (tok) {
+        for (int x = 0; x < CT; ++x) up += (x <= (l >> 4) ? (double)rs[x * C + l] : 0.) - (x >= (l >> 4) ? (double)cs[x * C + l] : 0.);
+        for (int x = 0; x < NT; ++x) {
+          up += (double)xs[x * C + l];
+          down += (double)ys[x * C + l];
+        }
+      }
+      for (int x = 0; x < NT; ++x) all += (double)cr[x];
+      const double own = down;
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) {
+        const double su = __shfl_down(up, m), sd = __shfl_up(down, m);
+        if (l + m < 64) up += su;
+        if (l >= m) down += sd;
+      }
+      const double dg = up + (down - own) + all * (double)fe;
+      const long t = t0 + l;
+      const bool valid = tok && t < n;
+      if (a.per_token) {
+        if (tok && t < a.T) a.g_decay[(b * a.T + t) * a.H + h] = valid ? (float)dg : 0.f;
+      } else {
+        decay_sum += valid ? dg : 0.;
+      }
+      if (more) dec[turn ^ 1].fill(rg, l < C && t0 - C + l < n);
+    }
+    __syncthreads();
+  }
+  if (!a.per_token && w == 0) {
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) decay_sum += __shfl_xor(decay_sum, m);
+    if (l == 0) sp.part_decay[bh * sp.segments + seg] = decay_sum;
+  }
+  if (a.g_s0 && seg == 0) {
+    const int kk = 16 * w + i;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (kk < a.K && 16 * t + 4 * g + r < a.V) a.g_s0[(bh * a.K + kk) * a.V + 16 * t + 4 * g + r] = R[t][r];
+  }
+}
+
+// sums a group's heads into the type of q / k
+template <typename T>
+__global__ __launch_bounds__(256) void attention_group_kernel(KfAttnArgs a, const float* part_q, const float* part_k) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const long total = a.B * a.T * a.G * a.K;
+  if (i >= total) return;
+  const float* part = blockIdx.y ? part_k : part_q;
+  const int c = (int)(i % a.K);
+  const long row = i / a.K, bt = row / a.G;
+  const int g = (int)(row - bt * a.G), per = a.H / a.G;
+  float s = 0.f;
+  for (int j = 0; j < per; ++j) s += part[(bt * a.H + g * per + j) * a.K + c];
+  ((T*)(blockIdx.y ? a.g_k : a.g_q))[i] = kf_from_float<T>(s);
+}
+
+// fixed decays: sums over sequences and segments, one wave for each head
+__global__ __launch_bounds__(64) void attention_decay_kernel(KfAttnArgs a, const double* part, int segments) {
+  const int h = blockIdx.x;
+  double s = 0.;
+  for (long x = threadIdx.x; x < a.B * segments; x += 64) s += part[((x / segments) * a.H + h) * segments + x % segments];
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) s += __shfl_xor(s, m);
+  if (threadIdx.x == 0) a.g_decay[h] = (float)s;
+}
+
+struct Plan {
+  int D;
+  Split sp;
+  size_t adds, factors, starts, part, decay;
+  size_t bytes() const { return 2 * adds + factors + starts + 2 * part + decay; }
+};
+
+Plan plan(const kf_handle* h, const KfAttnArgs& a) {
+  Plan p;
+  const int most = a.K > a.V ? a.K : a.V, C = a.dtype == KF_DTYPE_BF16 ? chunk_of<KfBf16>() : chunk_of<KfF32>();
+  p.D = most <= 32 ? 32 : most <= 64 ? 64 : 128;
+  Split& s = p.sp;
+  s.chunks = (a.T + C - 1) / C;
+  const long rows = a.B * a.H, cu = h->n_cu > 0 ? h->n_cu : 256;
+  // as many workgroups as the card holds at once (by LDS: one on each compute unit for D = 128, more for smaller ones); no segment
+  // under 4 chunks
+  const long room = cu * (p.D == 128 ? 1 : p.D == 64 ? 2 : 4);
+  long segs = (room + rows - 1) / rows;
+  segs = segs > 32 ? 32 : segs;
+  segs = segs > s.chunks / 4 ? s.chunks / 4 : segs;
+  segs = segs < 1 ? 1 : segs;
+  s.seg_chunks = (int)((s.chunks + segs - 1) / segs);
+  s.segments = (int)((s.chunks + s.seg_chunks - 1) / s.seg_chunks);
+  s.works = rows * s.segments;
+  const size_t state = (size_t)p.D * p.D * 4;
+  p.adds = kf_seq_round(rows * (s.segments - 1) * state);
+  p.factors = kf_seq_round((size_t)rows * s.segments * 4);
+  p.starts = kf_seq_round((size_t)rows * s.chunks * state);
+  p.part = a.G != a.H ? kf_seq_round((size_t)a.B * a.T * a.H * a.K * 4) : 0;
+  p.decay = a.per_token ? 0 : kf_seq_round((size_t)rows * s.segments * 8);
+  return p;
+}
+
+template <typename A, typename T, int D>
+int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream) {
+  constexpr int C = chunk_of<A>(), LD = D + A::PAD, LP = C + A::PAD;
+  constexpr size_t lds = sizeof(typename A::elem) * ((4 * C + D) * LD + 2 * C * LP) + 2 * sizeof(KfChunkDecay<C>) +
+                         sizeof(float) * (2 * (C / 16) * C + 2 * (D / 16) * C + D / 16);
+  static_assert(lds <= 160 * 1024, "LDS of one workgroup");
+  const Split& s = p.sp;
+  if (s.segments > 1) {
+    Split two = s;
+    two.works = 2 * (s.works / s.segments) * (s.segments - 1);
+    hipLaunchKernelGGL((attention_sweep_kernel<A, T, D, false>), dim3(kf_xcd_grid(two.works)), dim3(4 * D), 0, stream, a, two);
+  }
+  hipLaunchKernelGGL((attention_sweep_kernel<A, T, D, true>), dim3(kf_xcd_grid(s.works)), dim3(4 * D), 0, stream, a, s);
+  KF_HIP_CHECK(h, hipFuncSetAttribute(reinterpret_cast<const void*>(attention_gradient_kernel<A, T, D>),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  hipLaunchKernelGGL((attention_gradient_kernel<A, T, D>), dim3(kf_xcd_grid(s.works)), dim3(4 * D), lds, stream, a, s);
+  if (a.G != a.H) {
+    const long total = a.B * a.T * a.G * a.K;
+    hipLaunchKernelGGL(attention_group_kernel<T>, dim3((unsigned)((total + 255) / 256), 2), dim3(256), 0, stream, a, s.part_q, s.part_k);
+  }
+  if (!a.per_token) hipLaunchKernelGGL(attention_decay_kernel, dim3(a.H), dim3(64), 0, stream, a, s.part_decay, s.segments);
+  KF_HIP_CHECK(h, hipGetLastError());
+  return KF_OK;
+}
+
+template <typename A, typename T>
+int launch_d(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream) {
+  switch (p.D) {
+    case 32: return launch<A, T, 32>(h, a, p, stream);
+    case 64: return launch<A, T, 64>(h, a, p, stream);
+    default: return launch<A, T, 128>(h, a, p, stream);
+  }
+}
+
+}  // namespace
+
+size_t kf_attention_backward_workspace(const kf_handle* h, const KfAttnArgs& a) { return plan(h, a).bytes(); }
+
+int kf_launch_attention_backward(kf_handle* h, const KfAttnArgs& a, void* ws, hipStream_t stream) {
+  Plan p = plan(h, a);
+  Split& s = p.sp;
+  const int e = a.dtype == KF_DTYPE_F32 ? 4 : 2;
+  s.vec_q = kf_rows_aligned(a.q, a.qs, 3, a.K, e);
+  s.vec_k = kf_rows_aligned(a.k, a.ks, 3, a.K, e);
+  s.vec_v = kf_rows_aligned(a.v, a.vs, 3, a.V, e);
+  s.vec_g = kf_rows_aligned(a.g_o, a.gs, 3, a.V, e);
+  char* w = (char*)ws;
+  s.adds_s = (float*)w; w += p.adds;
+  s.adds_r = (float*)w; w += p.adds;
+  s.factors = (float*)w; w += p.factors;
+  s.starts = (kf_u32x4*)w; w += p.starts;
+  s.part_q = (float*)w; w += p.part;
+  s.part_k = (float*)w; w += p.part;
+  s.part_decay = (double*)w;
+  switch (a.dtype) {
+    case KF_DTYPE_F32: return launch_d<KfF32, float>(h, a, p, stream);
+    case KF_DTYPE_F16: return launch_d<KfF32, __half>(h, a, p, stream);
+    default: return launch_d<KfBf16, __hip_bfloat16>(h, a, p, stream);
+  }
+}

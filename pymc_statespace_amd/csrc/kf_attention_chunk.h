@@ -1,4 +1,4 @@
-// kf_attention_chunk.h -- a chunk of 64 tokens of linear attention: its decays, and how the time axis is split over workgroups.
+// kf_attention_chunk.h -- a chunk of tokens of linear attention: its decays, and how the time axis is split over workgroups.
 #pragma once
 #include "kf_frag.h"
 
@@ -7,14 +7,15 @@ constexpr int KF_CHUNK = 64;
 // Decays of one chunk, G_i = sum of the log decays up to and with token i (summed in 64 bits; each exponent is rounded once).
 // No exponent is positive: pairs (i, j) in different 16-token tiles take exp(G_i - G_j) as the product of two factors <= 1 that meet
 // at the end of j's tile, so that only the tiles on the diagonal need an exponential for each pair.
+template <int C>
 struct KfChunkDecay {
-  float from_start[KF_CHUNK];  // exp(G_i): from the chunk's start through token i
-  float to_end[KF_CHUNK];      // exp(G_63 - G_j): from behind token j to the chunk's end
-  float to_tile_end[KF_CHUNK]; // exp(G_e - G_j), e the last token of j's tile
-  float from_tile[3][KF_CHUNK]; // exp(G_i - G_e), e the last token of tile 0, 1, 2 (for the tiles behind it)
-  float hi[KF_CHUNK], lo[KF_CHUNK]; // G in two floats, for the diagonal
+  float from_start[C];            // exp(G_i): from the chunk's start through token i
+  float to_end[C];                // exp(G_(C-1) - G_j): from behind token j to the chunk's end
+  float to_tile_end[C];           // exp(G_e - G_j), e the last token of j's tile
+  float from_tile[C / 16 - 1][C]; // exp(G_i - G_e), e the last token of an earlier tile
+  float hi[C], lo[C];             // G in two floats, for the diagonal
 
-  // by one whole wave; tokens that are not `live` neither decay nor write
+  // by one whole wave, lane l with token l; tokens that are not `live` (lanes from C on are not) neither decay nor write
   __device__ __forceinline__ void fill(float log_decay, bool live) {
     const int l = threadIdx.x & 63;
     double G = live ? (double)kf_clamp_log_decay(log_decay) : 0.0;
@@ -24,16 +25,18 @@ struct KfChunkDecay {
       if (l >= d) G += x;
     }
     const double end = __shfl(G, 63), tile_end = __shfl(G, l | 15);
-    from_start[l] = expf((float)G);
-    to_end[l] = expf((float)(end - G));
-    to_tile_end[l] = expf((float)(tile_end - G));
+    float d[C / 16 - 1];
 #pragma unroll
-    for (int t = 0; t < 3; ++t) {
-      const float d = (float)(G - __shfl(G, 16 * t + 15));
-      from_tile[t][l] = expf(d > 0.f ? 0.f : d);  // (a NaN stays one)
+    for (int t = 0; t < C / 16 - 1; ++t) d[t] = (float)(G - __shfl(G, 16 * t + 15));
+    if (l < C) {
+      from_start[l] = expf((float)G);
+      to_end[l] = expf((float)(end - G));
+      to_tile_end[l] = expf((float)(tile_end - G));
+#pragma unroll
+      for (int t = 0; t < C / 16 - 1; ++t) from_tile[t][l] = expf(d[t] > 0.f ? 0.f : d[t]);  // (a NaN stays one)
+      hi[l] = (float)G;
+      lo[l] = (float)(G - (double)hi[l]);
     }
-    hi[l] = (float)G;
-    lo[l] = (float)(G - (double)hi[l]);
   }
   __device__ __forceinline__ float pair(int i, int j) const { return __expf((hi[i] - hi[j]) + (lo[i] - lo[j])); }
 };

@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
   __shared__ __attribute__((aligned(16))) E sK[KF_CHUNK * LK];
   __shared__ __attribute__((aligned(16))) E sV[KF_CHUNK * LV];
   __shared__ __attribute__((aligned(16))) E sS[OUT ? VT * LK : 8];  // the state's transpose as an operand
-  __shared__ __attribute__((aligned(16))) KfChunkDecay dec[2];
+  __shared__ __attribute__((aligned(16))) KfChunkDecay<KF_CHUNK> dec[2];
 
   const long work = kf_xcd_work(sp.works);
   if (work >= sp.works) return;
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
       load(c + 1);
       if (w == (int)((c + 1) & 3)) rg = load_decay(c + 1);
     }
-    const KfChunkDecay& D = dec[c & 1];
+    const KfChunkDecay<KF_CHUNK>& D = dec[c & 1];
 
     if (OUT) {
       const int row = 16 * w + i;

@@ -36,6 +36,11 @@ struct KfBf16 {
   static __device__ __forceinline__ frag zero() { return __builtin_bit_cast(frag, kf_u32x4{0, 0, 0, 0}); }
   // row i of a [i][depth] tile, p at its first depth of this lane
   static __device__ __forceinline__ frag row(const elem* p) { return *reinterpret_cast<const frag*>(p); }
+  // the same row at depth T, p at 4 g
+  static __device__ __forceinline__ frag row_t(const elem* p) {
+    const kf_s16x4 x = *reinterpret_cast<const kf_s16x4*>(p), y = *reinterpret_cast<const kf_s16x4*>(p + 16);
+    return __builtin_bit_cast(frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
   // column i of a [depth][i] tile, p at its corner
   static __device__ __forceinline__ frag col(const elem* p, int ld, int i, int g) {
     const elem* a = p + (4 * g + (i >> 2)) * ld + 4 * (i & 3);
@@ -62,6 +67,10 @@ struct KfBf16 {
   }
   static __device__ __forceinline__ void put8(elem* p, frag x) { *reinterpret_cast<frag*>(p) = x; }
   static __device__ __forceinline__ float get(const elem* p) { return kf_float_of((unsigned)*p << 16); }
+  static __device__ __forceinline__ kf_f32x4 get4(const elem* p) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    return kf_f32x4{kf_float_of(x.x << 16), kf_float_of(x.x & 0xffff0000u), kf_float_of(x.y << 16), kf_float_of(x.y & 0xffff0000u)};
+  }
 };
 
 struct KfF32 {
@@ -76,6 +85,10 @@ struct KfF32 {
   static __device__ __forceinline__ frag zero() { return frag{0, 0, 0, 0, 0, 0, 0, 0}; }
   static __device__ __forceinline__ frag row(const elem* p) {
     const kf_f32x4 x = *reinterpret_cast<const kf_f32x4*>(p), y = *reinterpret_cast<const kf_f32x4*>(p + 4);
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  static __device__ __forceinline__ frag row_t(const elem* p) {
+    const kf_f32x4 x = *reinterpret_cast<const kf_f32x4*>(p), y = *reinterpret_cast<const kf_f32x4*>(p + 16);
     return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
   }
   static __device__ __forceinline__ frag col(const elem* p, int ld, int i, int g) {
@@ -97,6 +110,7 @@ struct KfF32 {
     put4(p + 4, __builtin_shufflevector(x, x, 4, 5, 6, 7));
   }
   static __device__ __forceinline__ float get(const elem* p) { return *p; }
+  static __device__ __forceinline__ kf_f32x4 get4(const elem* p) { return *reinterpret_cast<const kf_f32x4*>(p); }
 };
 
 // An operand times a weight for each depth, exact to 24 bits: in fp32 the product itself; in bf16 the fp32 product is cut into three
@@ -109,6 +123,7 @@ template <> struct KfWeighted<KfF32> {
     for (int e = 0; e < 8; ++e) p[e] = a[e] * w[e];
   }
   __device__ __forceinline__ kf_f32x4 mma(kf_f32x8 b, kf_f32x4 c) const { return KfF32::mma(p, b, c); }
+  __device__ __forceinline__ kf_f32x4 mma_right(kf_f32x8 a, kf_f32x4 c) const { return KfF32::mma(a, p, c); }
 };
 template <> struct KfWeighted<KfBf16> {
   kf_bf16x8 p0, p1, p2;
@@ -133,6 +148,42 @@ template <> struct KfWeighted<KfBf16> {
   __device__ __forceinline__ kf_f32x4 mma(kf_bf16x8 b, kf_f32x4 c) const {
     return KfBf16::mma(p0, b, KfBf16::mma(p1, b, KfBf16::mma(p2, b, c)));
   }
+  __device__ __forceinline__ kf_f32x4 mma_right(kf_bf16x8 a, kf_f32x4 c) const {
+    return KfBf16::mma(a, p0, KfBf16::mma(a, p1, KfBf16::mma(a, p2, c)));
+  }
+};
+
+// Accumulators of two 16 x 16 tiles as one operand: fp32 as they are; bf16 in two rounded parts, 2 x 8 bits and a sign each
+// (2^-18 of each value is lost), two products.
+template <typename A> struct KfSplit;
+template <> struct KfSplit<KfF32> {
+  static constexpr int PARTS = 2;  // 16-byte pieces
+  kf_f32x8 p;
+  __device__ __forceinline__ void set(kf_f32x4 x, kf_f32x4 y) { p = KfF32::from(x, y); }
+  __device__ __forceinline__ kf_f32x4 mma(kf_f32x8 b, kf_f32x4 c) const { return KfF32::mma(p, b, c); }
+  __device__ __forceinline__ float value(int e) const { return p[e]; }
+  __device__ __forceinline__ kf_u32x4 piece(int k) const {
+    return k ? __builtin_bit_cast(kf_u32x4, __builtin_shufflevector(p, p, 4, 5, 6, 7)) : __builtin_bit_cast(kf_u32x4, __builtin_shufflevector(p, p, 0, 1, 2, 3));
+  }
+  __device__ __forceinline__ void pieces(kf_u32x4 x, kf_u32x4 y) { p = KfF32::from(__builtin_bit_cast(kf_f32x4, x), __builtin_bit_cast(kf_f32x4, y)); }
+};
+template <> struct KfSplit<KfBf16> {
+  static constexpr int PARTS = 2;
+  kf_bf16x8 hi, lo;
+  __device__ __forceinline__ void set(kf_f32x4 x, kf_f32x4 y) {
+    hi = KfBf16::from(x, y);
+    kf_f32x4 u, v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      u[e] = x[e] - KfBf16::value(hi, e);
+      v[e] = y[e] - KfBf16::value(hi, 4 + e);
+    }
+    lo = KfBf16::from(u, v);
+  }
+  __device__ __forceinline__ kf_f32x4 mma(kf_bf16x8 b, kf_f32x4 c) const { return KfBf16::mma(hi, b, KfBf16::mma(lo, b, c)); }
+  __device__ __forceinline__ float value(int e) const { return KfBf16::value(hi, e) + KfBf16::value(lo, e); }
+  __device__ __forceinline__ kf_u32x4 piece(int k) const { return __builtin_bit_cast(kf_u32x4, k ? lo : hi); }
+  __device__ __forceinline__ void pieces(kf_u32x4 x, kf_u32x4 y) { hi = __builtin_bit_cast(kf_bf16x8, x); lo = __builtin_bit_cast(kf_bf16x8, y); }
 };
 
 // Eight consecutive elements of a global row as the arithmetic's own (the first `n` of them; n <= 0: none), zeros behind them.

@@ -37,9 +37,9 @@ struct KfAttnStepArgs {
   int32_t* info;                         // [B] or NULL
 };
 
-size_t kf_attention_workspace(const kf_handle* h, const KfAttnArgs& a, bool backward);
 size_t kf_attention_forward_workspace(const kf_handle* h, const KfAttnArgs& a);
 int kf_launch_attention(kf_handle* h, const KfAttnArgs& a, void* ws, hipStream_t stream);
+size_t kf_attention_backward_workspace(const kf_handle* h, const KfAttnArgs& a);
 int kf_launch_attention_backward(kf_handle* h, const KfAttnArgs& a, void* ws, hipStream_t stream);
 int kf_launch_attention_step(kf_handle* h, const KfAttnStepArgs& a, hipStream_t stream);
 
