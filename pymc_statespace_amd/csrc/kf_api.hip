@@ -1700,7 +1700,7 @@ static int orthogonalise_args(kf_handle* h, int64_t n, int32_t rows, int32_t col
     return KF_ERR_ARG;
   }
   if (n > 65535 * 64L || rows > (1 << 17) || cols > (1 << 24) || (rows > cols && (rows > (1 << 24) || cols > (1 << 17))) ||
-      (double)n * rows * cols > 1.0e12) {
+      (double)n * rows * cols > 4.0e11) {
     KF_SET_ERR(h, "%s: n=%ld rows=%d cols=%d is too large", which, (long)n, rows, cols);
     return KF_ERR_UNSUPPORTED;
   }
@@ -1710,6 +1710,10 @@ static int orthogonalise_args(kf_handle* h, int64_t n, int32_t rows, int32_t col
   }
   memset(a, 0, sizeof(*a));
   a->n = n; a->rows = rows; a->cols = cols; a->dtype = dtype;
+  if (n > 65535 && !kf_orthogonalise_on_chip(*a)) {  // (a launch's third axis)
+    KF_SET_ERR(h, "%s: n=%ld matrices of this size in one call (at most 65535)", which, (long)n);
+    return KF_ERR_UNSUPPORTED;
+  }
   return KF_OK;
 }
 
@@ -1768,6 +1772,7 @@ extern "C" int kf_orthogonalise(kf_handle* h, int64_t n, int32_t rows, int32_t c
         return KF_ERR_ARG;
       }
     }
+    a.top[s] = top;
     top = quintic_top(a.coef[s], top);
     if (!(top <= 1.9)) {
       KF_SET_ERR(h, "kf_orthogonalise: step %d can carry a singular value to %g (at most 1.9)", s, top);

@@ -1,9 +1,24 @@
 // kf_orthogonalise.hip -- a batch of matrices moved towards their orthogonal factors by Newton-Schulz products:
 //     X = M / (|M|_F + eps);   per step   A = X X',   X <- a X + (b A + c A A) X
-// on the transpose where there are more rows than columns, so that A has the smaller side.
+// on the transpose where there are more rows than columns: X is d x L with d <= L.  Three ways, by size and type:
+//   * d <= 64 and both copies of X in LDS: one workgroup for each matrix, all steps on chip, in 32 bits (64 for fp64)
+//   * larger, up to 32 bits: tiled products on v_mfma_f32_16x16x32_f16, numbers held in fp16 parts (below)
+//   * larger, fp64: tiled products in fp64
+//
+// Numbers in fp16 parts.  The singular values stay within 1.9 (checked on the host), so entries of X, A = X X' and B = b A + c A A are
+// bounded and a power of two for each brings them to the top of fp16's range: hi = fp16(x), lo = fp16(x - hi) hold 22 bits and
+// nothing overflows.  fp32 and fp16 data take three products, hi hi + hi lo + lo hi (2^-22 of the terms is lost), at 1/3 of fp16's rate,
+// five times fp32's.  bf16 data keep X in both parts, which is what the term a X and every later step build on, but multiply hi parts
+// only: the products' rounding (2^-12 a factor) then stays below that of the bf16 result, 1.1e-3 to 1.8e-3 against 1.7e-3 of |X|, also
+// where M is of low rank (X in one part grows its rounding by a for each step in the missing directions: 4e-2 there).
 #include "kf_sequence.h"
 
 namespace {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
 
 template <typename T> struct Acc { typedef float type; };
 template <> struct Acc<double> { typedef double type; };
@@ -14,64 +29,499 @@ static __device__ __forceinline__ float to_acc(__hip_bfloat16 x) { return __bflo
 template <typename T> static __device__ __forceinline__ T from_acc(typename Acc<T>::type x) { return kf_from_float<T>(x); }
 template <> __device__ __forceinline__ double from_acc<double>(double x) { return x; }
 
-// |M|_F^2 in 64 bits: one workgroup per matrix, the same order on every run
-template <typename T>
-__global__ __launch_bounds__(256) void orth_norm_kernel(const T* M, long size, double* sum) {
-  __shared__ double red[256];
-  const T* m = M + (long)blockIdx.x * size;
+template <typename X> static __device__ __forceinline__ X block_sum(X s, X* red) {  // red: one for each wave
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) s += __shfl_xor(s, m);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = X(0);
+  for (unsigned i = 0; i < blockDim.x / 64; ++i) s += red[i];
+  return s;
+}
+
+// ----------------------------------------------------------------------------------------------------- on chip
+// Output tiles of RT x RT for each thread.  Where there are fewer tiles of A than threads the sum over L is cut into `slices`.
+template <typename T, int RT, int TH>
+__global__ __launch_bounds__(TH) void orth_chip_kernel(KfOrthArgs a, int slices) {
+  typedef typename Acc<T>::type C;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ double red[TH / 64];
+  const bool tall = a.rows > a.cols;
+  const int d = tall ? a.cols : a.rows, L = tall ? a.rows : a.cols;
+  const int lx = L | 1, la = d | 1;  // odd rows: different banks
+  C* X = (C*)smem;
+  C* Y = X + d * lx;
+  C* A = Y + d * lx;
+  C* B = A + d * la;
+  C* part = B + d * la;  // [slices][d d]
+  const long size = (long)d * L;
+  const T* M = (const T*)a.M + blockIdx.x * size;
+  T* out = (T*)a.X + blockIdx.x * size;
   double s = 0.;
-  for (long i = threadIdx.x; i < size; i += 256) {
+  for (int e = threadIdx.x; e < size; e += TH) {
+    const C x = to_acc(M[e]);
+    const int r = e / a.cols, c = e - r * a.cols;
+    X[tall ? c * lx + r : r * lx + c] = x;
+    s += (double)x * (double)x;
+  }
+  const double f = 1.0 / (sqrt(block_sum(s, red)) + a.eps);
+  for (int e = threadIdx.x; e < size; e += TH) {
+    C& x = X[(e / L) * lx + e % L];
+    x = (C)((double)x * f);
+  }
+  __syncthreads();
+  const int td = (d + RT - 1) / RT, tl = (L + RT - 1) / RT;
+  for (int step = 0; step < a.steps; ++step) {
+    const C ca = (C)a.coef[step][0], cb = (C)a.coef[step][1], cc = (C)a.coef[step][2];
+    // A = X X'
+    for (int w = threadIdx.x; w < td * td * slices; w += TH) {
+      const int t = w / slices, sl = w - t * slices, r0 = t / td * RT, c0 = t % td * RT;
+      C acc[RT][RT] = {};
+      const C *xr[RT], *xc[RT];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        xr[i] = X + (r0 + i < d ? r0 + i : d - 1) * lx;
+        xc[i] = X + (c0 + i < d ? c0 + i : d - 1) * lx;
+      }
+      for (int k = sl; k < L; k += slices) {
+        C u[RT], v[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) u[i] = xr[i][k], v[i] = xc[i][k];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < RT; ++j) acc[i][j] += u[i] * v[j];
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+          if (r0 + i < d && c0 + j < d) {
+            if (slices == 1) A[(r0 + i) * la + c0 + j] = acc[i][j];
+            else part[sl * d * d + (r0 + i) * d + c0 + j] = acc[i][j];
+          }
+    }
+    __syncthreads();
+    if (slices > 1) {
+      for (int e = threadIdx.x; e < d * d; e += TH) {
+        C x = 0;
+        for (int sl = 0; sl < slices; ++sl) x += part[sl * d * d + e];
+        A[(e / d) * la + e % d] = x;
+      }
+      __syncthreads();
+    }
+    // B = b A + c A A (A is symmetric: rows for columns)
+    for (int t = threadIdx.x; t < td * td; t += TH) {
+      const int r0 = t / td * RT, c0 = t % td * RT;
+      C acc[RT][RT] = {};
+      for (int k = 0; k < d; ++k) {
+        C u[RT], v[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          u[i] = A[(r0 + i < d ? r0 + i : d - 1) * la + k];
+          v[i] = A[k * la + (c0 + i < d ? c0 + i : d - 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < RT; ++j) acc[i][j] += u[i] * v[j];
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+          if (r0 + i < d && c0 + j < d) B[(r0 + i) * la + c0 + j] = cb * A[(r0 + i) * la + c0 + j] + cc * acc[i][j];
+    }
+    __syncthreads();
+    // Y = a X + B X
+    for (int t = threadIdx.x; t < td * tl; t += TH) {
+      const int r0 = t / tl * RT, c0 = t % tl * RT;
+      C acc[RT][RT] = {};
+      for (int k = 0; k < d; ++k) {
+        C u[RT], v[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          u[i] = B[(r0 + i < d ? r0 + i : d - 1) * la + k];
+          v[i] = X[k * lx + (c0 + i < L ? c0 + i : L - 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < RT; ++j) acc[i][j] += u[i] * v[j];
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+          if (r0 + i < d && c0 + j < L) Y[(r0 + i) * lx + c0 + j] = ca * X[(r0 + i) * lx + c0 + j] + acc[i][j];
+    }
+    __syncthreads();
+    C* t = X; X = Y; Y = t;
+  }
+  for (int e = threadIdx.x; e < size; e += TH) {
+    const int r = e / a.cols, c = e - r * a.cols;
+    out[e] = from_acc<T>(X[tall ? c * lx + r : r * lx + c]);
+  }
+}
+
+struct ChipPlan { int rt, threads, slices; size_t lds; bool fits; };
+ChipPlan chip_plan(const KfOrthArgs& a) {
+  ChipPlan p;
+  const long d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
+  const size_t e = a.dtype == KF_DTYPE_F64 ? 8 : 4;
+  p.fits = false;
+  if (d > 64 || L > 40000) return p;
+  p.rt = d <= 16 ? 1 : d <= 32 ? 2 : 4;
+  // one wave where a matrix has no work for more (then d <= 16): many of them fit a compute unit
+  p.threads = d * L <= 256 ? 64 : 256;
+  const long tiles = ((d + p.rt - 1) / p.rt) * ((d + p.rt - 1) / p.rt);
+  p.slices = 1;
+  while (2 * p.slices * tiles <= p.threads && 2 * p.slices <= L / 8) p.slices *= 2;
+  p.lds = e * (2 * d * (L | 1) + 2 * d * (d | 1) + (p.slices > 1 ? p.slices * d * d : 0));
+  p.fits = p.lds <= 156 * 1024;
+  return p;
+}
+
+template <typename T, int RT, int TH>
+int launch_chip(kf_handle* h, const KfOrthArgs& a, const ChipPlan& p, hipStream_t stream) {
+  KF_HIP_CHECK(h, hipFuncSetAttribute(reinterpret_cast<const void*>(orth_chip_kernel<T, RT, TH>),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds));
+  hipLaunchKernelGGL((orth_chip_kernel<T, RT, TH>), dim3((unsigned)a.n), dim3(TH), p.lds, stream, a, p.slices);
+  KF_HIP_CHECK(h, hipGetLastError());
+  return KF_OK;
+}
+
+// ------------------------------------------------------------------------------------- |M|_F^2 in 64 bits, by parts
+constexpr int NORM_PARTS = 64;
+template <typename T>
+__global__ __launch_bounds__(256) void orth_norm_kernel(const T* M, long size, double* part) {
+  __shared__ double red[4];
+  const T* m = M + (long)blockIdx.y * size;
+  const long per = (size + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < size ? lo + per : size;
+  double s = 0.;
+  for (long i = lo + threadIdx.x; i < hi; i += 256) {
     const double x = (double)to_acc(m[i]);
     s += x * x;
   }
-  red[threadIdx.x] = s;
-  __syncthreads();
-  for (int w = 128; w; w >>= 1) {
-    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) part[blockIdx.y * NORM_PARTS + blockIdx.x] = s;
+}
+static __device__ __forceinline__ double norm_factor(const double* part, int parts, double eps) {
+  double s = 0.;
+  for (int i = 0; i < parts; ++i) s += part[i];
+  return 1.0 / (sqrt(s) + eps);
+}
+static inline int norm_parts(long size) {
+  const long p = (size + 16383) / 16384;
+  return p < NORM_PARTS ? (int)p : NORM_PARTS;
+}
+
+// ------------------------------------------------------------------------------------------------ fp16 parts
+constexpr float SCALE_X = 16384.f;  // 2^14: |x| <= 1.9 comes to 31130 of fp16's 65504
+constexpr float SCALE_A = 8192.f;   // 2^13: |a| <= 1.9^2 comes to 29573
+
+static __device__ __forceinline__ void parts_of(f4 x, h4* hi, h4* lo) {
+  *hi = __builtin_convertvector(x, h4);
+  *lo = __builtin_convertvector(x - __builtin_convertvector(*hi, f4), h4);
+}
+static __device__ __forceinline__ f4 whole(h4 hi, h4 lo) { return __builtin_convertvector(hi, f4) + __builtin_convertvector(lo, f4); }
+
+// M (rows x cols) times its factor, in parts: dP x LP, zeros behind d and L, transposed where M is tall
+template <typename T>
+__global__ __launch_bounds__(256) void orth_parts_kernel(KfOrthArgs a, const double* part, int parts, int dP, int LP, _Float16* hi, _Float16* lo) {
+  __shared__ float tile[64][65];
+  const bool tall = a.rows > a.cols;
+  const int d = tall ? a.cols : a.rows, L = tall ? a.rows : a.cols;
+  const long z = blockIdx.z, at = z * dP * (long)LP;
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+  const double f = norm_factor(part + z * NORM_PARTS, parts, a.eps) * SCALE_X;
+  const T* M = (const T*)a.M + z * d * (long)L;
+  if (tall) {
+    for (int e = threadIdx.x; e < 4096; e += 256) {
+      const int c = e >> 6, r = e & 63;  // neighbours along M's rows
+      tile[r][c] = r0 + r < d && c0 + c < L ? (float)((double)to_acc(M[(c0 + c) * (long)d + r0 + r]) * f) : 0.f;
+    }
     __syncthreads();
   }
-  if (threadIdx.x == 0) sum[blockIdx.x] = red[0];
+  for (int e = threadIdx.x; e < 1024; e += 256) {
+    const int r = e >> 4, c = 4 * (e & 15);
+    f4 x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      x[j] = tall ? tile[r][c + j] : r0 + r < d && c0 + c + j < L ? (float)((double)to_acc(M[(r0 + r) * (long)L + c0 + c + j]) * f) : 0.f;
+    h4 xh, xl;
+    parts_of(x, &xh, &xl);
+    const long to = at + (long)(r0 + r) * LP + c0 + c;
+    *(h4*)(hi + to) = xh;
+    *(h4*)(lo + to) = xl;
+  }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void orth_scale_kernel(const T* M, long n, int rows, int cols, double eps, const double* sum,
-                                                         typename Acc<T>::type* X) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x, size = (long)rows * cols;
-  if (i >= n * size) return;
+enum { GRAM, POLY, UPDATE };
+
+struct Product {
+  int n, d, L, dP, LP;      // sizes, padded to tiles
+  int tiles_m, tiles_n;     // of one matrix's output
+  long works;
+  const _Float16 *Ph, *Pl;  // left operand, rows over the depth
+  const _Float16 *Qh, *Ql;  // right operand: rows over the depth (GRAM, POLY), or depth x columns (UPDATE)
+  const _Float16 *Dh, *Dl;  // what is added: A (POLY), X (UPDATE)
+  _Float16 *Ch, *Cl;        // output in parts
+  void* out;                // or in T (the last UPDATE), `tall`: transposed
+  int tall;
+  float unscale;            // accumulator -> the output's scale
+  float add;                // factor of what is added
+};
+
+// out = unscale P Q + add D, TILE x TILE of it for each workgroup of 2 x 2 waves.  Depth in steps of 32 through two LDS buffers that
+// global_load_lds fills (16 bytes a lane, no registers); the order of the 16-byte pieces inside a buffer is permuted by row so
+// that the fragment reads meet different banks.  GRAM and POLY are symmetric: tiles on and below the diagonal, stored twice.
+template <typename T, int TILE, int PARTS, int MODE, bool LAST>
+__global__ __launch_bounds__(256, 2) void orth_product_kernel(Product p) {
+  constexpr int WT = TILE / 32, PIECES = TILE * 4, PER = PIECES / 256, GR = TILE / 16;
+  constexpr bool NN = MODE == UPDATE;
+  __shared__ __attribute__((aligned(16))) _Float16 lds[2][2 * PARTS][TILE * 32];  // [buffer][P hi, (P lo,) Q hi(, Q lo)]
+  const long per = (p.works + 7) >> 3, work = (blockIdx.x & 7) * per + (blockIdx.x >> 3);  // neighbours on one die
+  if (work >= p.works) return;
+  const long tiles = p.works / p.n, z = work / tiles;
+  const int x = (int)(work - z * tiles);
+  int tm, tn;
+  if (MODE == UPDATE) {  // bands of 8 tiles, so that what one die works on shares rows and columns
+    const int width = 8 * p.tiles_n, band = x / width, in = x - band * width;
+    const int rows = p.tiles_m - 8 * band < 8 ? p.tiles_m - 8 * band : 8;
+    tm = 8 * band + in % rows;
+    tn = in / rows;
+  } else {
+    tm = (int)((sqrtf(8.f * x + 1.f) - 1.f) * 0.5f);
+    while ((tm + 1) * (tm + 2) / 2 <= x) ++tm;
+    while (tm * (tm + 1) / 2 > x) --tm;
+    tn = x - tm * (tm + 1) / 2;
+  }
+  const int depth = MODE == GRAM ? p.LP : p.dP;
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, i = l & 15, g = l >> 4;
+  const int wm = (w & 1) * (TILE / 2), wn = (w >> 1) * (TILE / 2);
+  const long zP = z * (long)p.dP * (MODE == GRAM ? p.LP : p.dP), zQ = z * (long)p.dP * (MODE == POLY ? p.dP : p.LP);
+
+  // source of each 16-byte piece this lane brings in, at depth 0; along the depth it moves by `step`
+  const _Float16* src[2 * PARTS][PER];
+  const long stepP = 32, stepQ = NN ? 32l * p.LP : 32;
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int s = tid + 256 * u;
+    const int r = s >> 2, c = (s & 3) ^ ((r >> 2) & 3);
+    const long oP = zP + (long)(tm * TILE + r) * depth + 8 * c;
+    long oQ;
+    if (NN) {
+      const int k = s / (TILE / 8), pos = s % (TILE / 8), gr = (pos >> 1) ^ (k & (GR - 1));
+      oQ = zQ + (long)k * p.LP + tn * TILE + 16 * gr + 8 * (pos & 1);
+    } else {
+      oQ = zQ + (long)(tn * TILE + r) * depth + 8 * c;
+    }
+    src[0][u] = p.Ph + oP;
+    if (PARTS == 2) src[1][u] = p.Pl + oP;
+    src[PARTS][u] = p.Qh + oQ;
+    if (PARTS == 2) src[2 * PARTS - 1][u] = p.Ql + oQ;
+  }
+  auto bring = [&](int buf) {
+#pragma unroll
+    for (int k = 0; k < 2 * PARTS; ++k)
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[k][u],
+                                         (__attribute__((address_space(3))) void*)&lds[buf][k][(w * 64 + 256 * u) * 8], 16, 0, 0);
+        src[k][u] += k < PARTS ? stepP : stepQ;
+      }
+  };
+  auto left = [&](const _Float16* t, int r) {  // row r, at the depths the right operand comes in
+    const int sw = (r >> 2) & 3;
+    if (!NN) return *(const h8*)(t + r * 32 + 8 * (g ^ sw));
+    const h4 a = *(const h4*)(t + r * 32 + 8 * ((g >> 1) ^ sw) + 4 * (g & 1));
+    const h4 b = *(const h4*)(t + r * 32 + 8 * ((2 + (g >> 1)) ^ sw) + 4 * (g & 1));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto right = [&](const _Float16* t, int c) {  // columns c .. c + 15
+    if (!NN) {
+      const int r = c + i, sw = (r >> 2) & 3;
+      return *(const h8*)(t + r * 32 + 8 * (g ^ sw));
+    }
+    typedef __attribute__((address_space(3))) s4* lp;
+    const int k = 4 * g + (i >> 2);
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + k * TILE + 16 * ((c >> 4) ^ (k & (GR - 1))) + 4 * (i & 3)));
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + (k + 16) * TILE + 16 * ((c >> 4) ^ (k & (GR - 1))) + 4 * (i & 3)));
+    return __builtin_bit_cast(h8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  f4 acc[WT][WT];  // [m][n]: column (lane % 16) the row of the output, rows its columns
+#pragma unroll
+  for (int m = 0; m < WT; ++m)
+#pragma unroll
+    for (int n = 0; n < WT; ++n) acc[m][n] = f4{0, 0, 0, 0};
+  const int steps = depth / 32;
+  bring(0);
+  for (int s = 0; s < steps; ++s) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // buffer s & 1 is filled, and nobody reads the other one any more
+    if (s + 1 < steps) bring((s + 1) & 1);
+    const _Float16(*b)[TILE * 32] = lds[s & 1];
+    h8 ph[WT], pl[WT];
+#pragma unroll
+    for (int m = 0; m < WT; ++m) {
+      ph[m] = left(b[0], wm + 16 * m + i);
+      if (PARTS == 2) pl[m] = left(b[1], wm + 16 * m + i);
+    }
+#pragma unroll
+    for (int n = 0; n < WT; ++n) {
+      const h8 qh = right(b[PARTS], wn + 16 * n);
+      h8 ql = qh;
+      if (PARTS == 2) ql = right(b[2 * PARTS - 1], wn + 16 * n);
+#pragma unroll
+      for (int m = 0; m < WT; ++m) {
+        if (PARTS == 2) {
+          acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql, ph[m], acc[m][n], 0, 0, 0);
+          acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh, pl[m], acc[m][n], 0, 0, 0);
+        }
+        acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh, ph[m], acc[m][n], 0, 0, 0);
+      }
+    }
+  }
+  const int ld = MODE == UPDATE ? p.LP : p.dP;
+  const long zC = z * (long)p.dP * ld;
+#pragma unroll
+  for (int m = 0; m < WT; ++m)
+#pragma unroll
+    for (int n = 0; n < WT; ++n) {
+      const int row = tm * TILE + wm + 16 * m + i, col = tn * TILE + wn + 16 * n + 4 * g;
+      const long at = zC + (long)row * ld + col;
+      f4 v = acc[m][n] * p.unscale;
+      if (MODE != GRAM) {
+        const h4 dh = *(const h4*)(p.Dh + at);
+        v += p.add * (MODE == POLY && PARTS == 1 ? __builtin_convertvector(dh, f4) : whole(dh, *(const h4*)(p.Dl + at)));
+      }
+      if (LAST) {
+        T* out = (T*)p.out + z * (long)p.d * p.L;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (row < p.d && col + r < p.L) out[p.tall ? (long)(col + r) * p.d + row : (long)row * p.L + col + r] = from_acc<T>(v[r]);
+      } else {
+        h4 vh, vl;
+        parts_of(v, &vh, &vl);
+        *(h4*)(p.Ch + at) = vh;
+        if (MODE == UPDATE || PARTS == 2) *(h4*)(p.Cl + at) = vl;
+        if (MODE != UPDATE && tm != tn) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const long to = zC + (long)(col + r) * ld + row;
+            p.Ch[to] = vh[r];
+            if (PARTS == 2) p.Cl[to] = vl[r];
+          }
+        }
+      }
+    }
+}
+
+struct PartsPlan { int tile, dP, LP, td, tl; size_t x, aa, norm; };
+PartsPlan parts_plan(const kf_handle* h, const KfOrthArgs& a) {
+  PartsPlan p;
+  const int d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
+  const long t = (d + 127) / 128, cu = h->n_cu > 0 ? h->n_cu : 256;
+  p.tile = a.n * t * (t + 1) / 2 >= cu ? 128 : 64;  // the symmetric products' tiles fill the card, or smaller ones
+  p.td = (d + p.tile - 1) / p.tile;
+  p.tl = (L + p.tile - 1) / p.tile;
+  p.dP = p.td * p.tile;
+  p.LP = p.tl * p.tile;
+  p.x = kf_seq_round((size_t)a.n * p.dP * p.LP * 2);
+  p.aa = kf_seq_round((size_t)a.n * p.dP * p.dP * 2);
+  p.norm = kf_seq_round((size_t)a.n * NORM_PARTS * 8);
+  return p;
+}
+
+template <typename T, int TILE, int PARTS>
+int launch_parts(kf_handle* h, const KfOrthArgs& a, const PartsPlan& pl, void* ws, hipStream_t stream) {
+  char* w = (char*)ws;
+  double* norm = (double*)w; w += pl.norm;
+  _Float16 *X[2][2], *A[2], *B[2];
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2; ++j) X[i][j] = (_Float16*)w, w += pl.x;
+  for (int j = 0; j < 2; ++j) A[j] = (_Float16*)w, w += pl.aa;
+  for (int j = 0; j < 2; ++j) B[j] = (_Float16*)w, w += pl.aa;
+  const long size = (long)a.rows * a.cols;
+  const int parts = norm_parts(size);
+  Product p;
+  p.n = (int)a.n;
+  p.tall = a.rows > a.cols;
+  p.d = p.tall ? a.cols : a.rows;
+  p.L = p.tall ? a.rows : a.cols;
+  p.dP = pl.dP; p.LP = pl.LP;
+  p.out = a.X;
+  hipLaunchKernelGGL(orth_norm_kernel<T>, dim3(parts, (unsigned)a.n), dim3(256), 0, stream, (const T*)a.M, size, norm);
+  hipLaunchKernelGGL(orth_parts_kernel<T>, dim3(pl.LP / 64, pl.dP / 64, (unsigned)a.n), dim3(256), 0, stream, a, norm, parts, pl.dP, pl.LP, X[0][0], X[0][1]);
+  for (int s = 0; s < a.steps; ++s) {
+    const double ca = a.coef[s][0], cb = a.coef[s][1], cc = a.coef[s][2];
+    const int from = s & 1, to = from ^ 1;
+    const double top = a.top[s];
+    // |B| <= the largest |b u + c u^2|, u = s^2 <= top^2
+    double bound = fabs(top * top * (cb + cc * top * top));
+    if (cc != 0.0 && -cb / (2 * cc) > 0 && -cb / (2 * cc) < top * top) bound = fmax(bound, fabs(cb * cb / (4 * cc)));
+    int e = 0;
+    frexp(fmax(bound, 1e-6), &e);
+    const double scale_b = ldexp(1.0, 14 - e);  // |B| comes to at most 2^14: room for what A's rounding adds
+    p.Ph = p.Qh = X[from][0]; p.Pl = p.Ql = X[from][1];
+    p.Ch = A[0]; p.Cl = A[1];
+    p.Dh = p.Dl = nullptr;
+    p.tiles_m = p.tiles_n = pl.td;
+    p.works = a.n * pl.td * (pl.td + 1L) / 2;
+    p.unscale = (float)(SCALE_A / ((double)SCALE_X * SCALE_X)); p.add = 0.f;
+    hipLaunchKernelGGL((orth_product_kernel<T, TILE, PARTS, GRAM, false>), dim3((unsigned)(8 * ((p.works + 7) / 8))), dim3(256), 0, stream, p);
+    p.Ph = p.Qh = p.Dh = A[0]; p.Pl = p.Ql = p.Dl = A[1];
+    p.Ch = B[0]; p.Cl = B[1];
+    p.unscale = (float)(cc * scale_b / ((double)SCALE_A * SCALE_A)); p.add = (float)(cb * scale_b / SCALE_A);
+    hipLaunchKernelGGL((orth_product_kernel<T, TILE, PARTS, POLY, false>), dim3((unsigned)(8 * ((p.works + 7) / 8))), dim3(256), 0, stream, p);
+    p.Ph = B[0]; p.Pl = B[1];
+    p.Qh = p.Dh = X[from][0]; p.Ql = p.Dl = X[from][1];
+    p.Ch = X[to][0]; p.Cl = X[to][1];
+    p.tiles_n = pl.tl;
+    p.works = a.n * (long)pl.td * pl.tl;
+    const bool last = s + 1 == a.steps;
+    p.unscale = (float)((last ? 1.0 / SCALE_X : 1.0) / scale_b); p.add = (float)(last ? ca / SCALE_X : ca);
+    const dim3 grid((unsigned)(8 * ((p.works + 7) / 8)));
+    if (last) hipLaunchKernelGGL((orth_product_kernel<T, TILE, PARTS, UPDATE, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((orth_product_kernel<T, TILE, PARTS, UPDATE, false>), grid, dim3(256), 0, stream, p);
+  }
+  KF_HIP_CHECK(h, hipGetLastError());
+  return KF_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ fp64
+__global__ __launch_bounds__(256) void orth_scale64_kernel(KfOrthArgs a, const double* part, int parts, double* X) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x, size = (long)a.rows * a.cols;
+  if (i >= a.n * size) return;
   const long z = i / size, e = i - z * size;
-  const double f = 1.0 / (sqrt(sum[z]) + eps);
-  const long to = rows > cols ? z * size + (e % cols) * rows + e / cols : i;
-  X[to] = (typename Acc<T>::type)((double)to_acc(M[i]) * f);
+  const double f = norm_factor(part + z * NORM_PARTS, parts, a.eps);
+  X[a.rows > a.cols ? z * size + (e % a.cols) * a.rows + e / a.cols : i] = ((const double*)a.M)[i] * f;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void orth_store_kernel(const typename Acc<T>::type* X, long n, int rows, int cols, T* out) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x, size = (long)rows * cols;
-  if (i >= n * size) return;
-  const long z = i / size, e = i - z * size;
-  out[i] = from_acc<T>(X[rows > cols ? z * size + (e % cols) * rows + e / cols : i]);
-}
-
-// C (m x n) = alpha op(A B) + beta D, A (m x k) row-major, B (k x n) row-major or (NT) given as (n x k)
-template <typename C, bool NT>
-__global__ __launch_bounds__(256) void orth_product_kernel(int m, int n, int k, const C* A, const C* B, const C* D, C* out, C alpha, C beta) {
-  __shared__ C sa[16][65], sb[16][65];
+// C (m x n) = alpha op(A B) + beta D, A (m x k) row-major, B (k x n) row-major or (NT) given as (n x k); `tall`: C is stored transposed
+template <bool NT>
+__global__ __launch_bounds__(256) void orth_product64_kernel(int m, int n, int k, const double* A, const double* B, const double* D, double* out,
+                                                             double alpha, double beta, int tall) {
+  __shared__ double sa[16][65], sb[16][65];
   const long z = blockIdx.z;
   A += z * m * (long)k;
   B += z * n * (long)k;
   D += z * m * (long)n;
   out += z * m * (long)n;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  C acc[4][4] = {};
+  double acc[4][4] = {};
   for (int k0 = 0; k0 < k; k0 += 16) {
     for (int i = threadIdx.x; i < 64 * 16; i += 256) {
       const int kk = i & 15, r = i >> 4;
-      sa[kk][r] = r0 + r < m && k0 + kk < k ? A[(long)(r0 + r) * k + k0 + kk] : C(0);
+      sa[kk][r] = r0 + r < m && k0 + kk < k ? A[(long)(r0 + r) * k + k0 + kk] : 0.;
       if (NT) {
-        sb[kk][r] = c0 + r < n && k0 + kk < k ? B[(long)(c0 + r) * k + k0 + kk] : C(0);
+        sb[kk][r] = c0 + r < n && k0 + kk < k ? B[(long)(c0 + r) * k + k0 + kk] : 0.;
       } else {
         const int cc = i & 63, k2 = i >> 6;
-        sb[k2][cc] = c0 + cc < n && k0 + k2 < k ? B[(long)(k0 + k2) * n + c0 + cc] : C(0);
+        sb[k2][cc] = c0 + cc < n && k0 + k2 < k ? B[(long)(k0 + k2) * n + c0 + cc] : 0.;
       }
     }
     __syncthreads();
@@ -86,51 +536,72 @@ __global__ __launch_bounds__(256) void orth_product_kernel(int m, int n, int k, 
   for (int i = 0; i < 4; ++i)
     for (int j = 0; j < 4; ++j) {
       const int r = r0 + ty + 16 * i, c = c0 + tx + 16 * j;
-      if (r < m && c < n) out[(long)r * n + c] = alpha * acc[i][j] + (beta != C(0) ? beta * D[(long)r * n + c] : C(0));
+      if (r < m && c < n) out[tall ? (long)c * m + r : (long)r * n + c] = alpha * acc[i][j] + (beta != 0. ? beta * D[(long)r * n + c] : 0.);
     }
 }
 
-template <typename T>
-int orth_t(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
-  typedef typename Acc<T>::type C;
-  const int d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
-  const size_t big = kf_seq_round((size_t)a.n * d * L * sizeof(C)), small = kf_seq_round((size_t)a.n * d * d * sizeof(C));
+int launch64(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
+  const bool tall = a.rows > a.cols;
+  const int d = tall ? a.cols : a.rows, L = tall ? a.rows : a.cols;
+  const size_t big = kf_seq_round((size_t)a.n * d * L * 8), small = kf_seq_round((size_t)a.n * d * d * 8);
   char* w = (char*)ws;
-  double* sum = (double*)w; w += kf_seq_round((size_t)a.n * 8);
-  C* X = (C*)w; w += big;
-  C* Y = (C*)w; w += big;
-  C* A = (C*)w; w += small;
-  C* B = (C*)w;
-  const long total = a.n * (long)d * L;
-  const unsigned blocks = (unsigned)((total + 255) / 256);
-  hipLaunchKernelGGL(orth_norm_kernel<T>, dim3((unsigned)a.n), dim3(256), 0, stream, (const T*)a.M, (long)d * L, sum);
-  hipLaunchKernelGGL(orth_scale_kernel<T>, dim3(blocks), dim3(256), 0, stream, (const T*)a.M, a.n, a.rows, a.cols, a.eps, sum, X);
+  double* norm = (double*)w; w += kf_seq_round((size_t)a.n * NORM_PARTS * 8);
+  double* X = (double*)w; w += big;
+  double* Y = (double*)w; w += big;
+  double* A = (double*)w; w += small;
+  double* B = (double*)w;
+  const long size = (long)d * L, total = a.n * size;
+  const int parts = norm_parts(size);
+  hipLaunchKernelGGL(orth_norm_kernel<double>, dim3(parts, (unsigned)a.n), dim3(256), 0, stream, (const double*)a.M, size, norm);
+  hipLaunchKernelGGL(orth_scale64_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, a, norm, parts, X);
   const unsigned td = (d + 63) / 64, tl = (L + 63) / 64, z = (unsigned)a.n;
   for (int s = 0; s < a.steps; ++s) {
-    const C ca = (C)a.coef[s][0], cb = (C)a.coef[s][1], cc = (C)a.coef[s][2];
-    hipLaunchKernelGGL((orth_product_kernel<C, true>), dim3(td, td, z), dim3(256), 0, stream, d, d, L, X, X, A, A, C(1), C(0));
-    hipLaunchKernelGGL((orth_product_kernel<C, true>), dim3(td, td, z), dim3(256), 0, stream, d, d, d, A, A, A, B, cc, cb);
-    hipLaunchKernelGGL((orth_product_kernel<C, false>), dim3(tl, td, z), dim3(256), 0, stream, d, L, d, B, X, X, Y, C(1), ca);
-    C* t = X; X = Y; Y = t;
+    const bool last = s + 1 == a.steps;
+    hipLaunchKernelGGL(orth_product64_kernel<true>, dim3(td, td, z), dim3(256), 0, stream, d, d, L, X, X, A, A, 1., 0., 0);
+    hipLaunchKernelGGL(orth_product64_kernel<true>, dim3(td, td, z), dim3(256), 0, stream, d, d, d, A, A, A, B, a.coef[s][2], a.coef[s][1], 0);
+    hipLaunchKernelGGL(orth_product64_kernel<false>, dim3(tl, td, z), dim3(256), 0, stream, d, L, d, B, X, X, last ? (double*)a.X : Y, 1., a.coef[s][0],
+                       last && tall);
+    double* t = X; X = Y; Y = t;
   }
-  hipLaunchKernelGGL(orth_store_kernel<T>, dim3(blocks), dim3(256), 0, stream, X, a.n, a.rows, a.cols, (T*)a.X);
   KF_HIP_CHECK(h, hipGetLastError());
   return KF_OK;
 }
 
+template <typename T>
+int launch_t(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
+  const ChipPlan c = chip_plan(a);
+  if (c.fits) {
+    if (c.threads == 64) return launch_chip<T, 1, 64>(h, a, c, stream);
+    return c.rt == 1 ? launch_chip<T, 1, 256>(h, a, c, stream) : c.rt == 2 ? launch_chip<T, 2, 256>(h, a, c, stream) : launch_chip<T, 4, 256>(h, a, c, stream);
+  }
+  const PartsPlan p = parts_plan(h, a);
+  constexpr int PARTS = std::is_same<T, __hip_bfloat16>::value ? 1 : 2;
+  return p.tile == 128 ? launch_parts<T, 128, PARTS>(h, a, p, ws, stream) : launch_parts<T, 64, PARTS>(h, a, p, ws, stream);
+}
+
 }  // namespace
 
-size_t kf_orthogonalise_ws(const kf_handle*, const KfOrthArgs& a) {
-  const size_t e = a.dtype == KF_DTYPE_F64 ? 8 : 4;
+bool kf_orthogonalise_on_chip(const KfOrthArgs& a) { return chip_plan(a).fits; }
+
+size_t kf_orthogonalise_ws(const kf_handle* h, const KfOrthArgs& a) {
+  if (chip_plan(a).fits) return 0;
   const size_t d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
-  return kf_seq_round((size_t)a.n * 8) + 2 * kf_seq_round((size_t)a.n * d * L * e) + 2 * kf_seq_round((size_t)a.n * d * d * e);
+  if (a.dtype == KF_DTYPE_F64)
+    return kf_seq_round((size_t)a.n * NORM_PARTS * 8) + 2 * kf_seq_round((size_t)a.n * d * L * 8) + 2 * kf_seq_round((size_t)a.n * d * d * 8);
+  const PartsPlan p = parts_plan(h, a);
+  return p.norm + 4 * p.x + 4 * p.aa;
 }
 
 int kf_launch_orthogonalise(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
   switch (a.dtype) {
-    case KF_DTYPE_F64: return orth_t<double>(h, a, ws, stream);
-    case KF_DTYPE_F32: return orth_t<float>(h, a, ws, stream);
-    case KF_DTYPE_BF16: return orth_t<__hip_bfloat16>(h, a, ws, stream);
-    default: return orth_t<__half>(h, a, ws, stream);
+    case KF_DTYPE_F64: {
+      const ChipPlan c = chip_plan(a);
+      if (!c.fits) return launch64(h, a, ws, stream);
+      if (c.threads == 64) return launch_chip<double, 1, 64>(h, a, c, stream);
+      return c.rt == 1 ? launch_chip<double, 1, 256>(h, a, c, stream) : c.rt == 2 ? launch_chip<double, 2, 256>(h, a, c, stream) : launch_chip<double, 4, 256>(h, a, c, stream);
+    }
+    case KF_DTYPE_F32: return launch_t<float>(h, a, ws, stream);
+    case KF_DTYPE_BF16: return launch_t<__hip_bfloat16>(h, a, ws, stream);
+    default: return launch_t<__half>(h, a, ws, stream);
   }
 }

@@ -47,10 +47,12 @@ struct KfOrthArgs {
   long n;
   int rows, cols, dtype, steps;
   double coef[KF_ORTHOGONALISE_STEPS_MAX][3];
+  double top[KF_ORTHOGONALISE_STEPS_MAX];  // no singular value is above this before step s
   double eps;
   const void* M;
   void* X;
 };
+bool kf_orthogonalise_on_chip(const KfOrthArgs& a);
 size_t kf_orthogonalise_ws(const kf_handle* h, const KfOrthArgs& a);
 int kf_launch_orthogonalise(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream);
 
