@@ -71,12 +71,21 @@ __global__ __launch_bounds__(TH) void orth_chip_kernel(KfOrthArgs a, int slices)
     x = (C)((double)x * f);
   }
   __syncthreads();
-  const int td = (d + RT - 1) / RT, tl = (L + RT - 1) / RT;
+  const int td = (d + RT - 1) / RT, tl = (L + RT - 1) / RT, ts = td * (td + 1) / 2;
+  auto below = [](int t, int* r, int* c) {
+    int x = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    x += (x + 1) * (x + 2) / 2 <= t;
+    x -= x * (x + 1) / 2 > t;
+    *r = x * RT;
+    *c = (t - x * (x + 1) / 2) * RT;
+  };
   for (int step = 0; step < a.steps; ++step) {
     const C ca = (C)a.coef[step][0], cb = (C)a.coef[step][1], cc = (C)a.coef[step][2];
-    // A = X X'
-    for (int w = threadIdx.x; w < td * td * slices; w += TH) {
-      const int t = w / slices, sl = w - t * slices, r0 = t / td * RT, c0 = t % td * RT;
+    // A = X X', tiles on and below the diagonal
+    for (int w = threadIdx.x; w < ts * slices; w += TH) {
+      const int t = w / slices, sl = w - t * slices;
+      int r0, c0;
+      below(t, &r0, &c0);
       C acc[RT][RT] = {};
       const C *xr[RT], *xc[RT];
 #pragma unroll
@@ -98,8 +107,8 @@ __global__ __launch_bounds__(TH) void orth_chip_kernel(KfOrthArgs a, int slices)
 #pragma unroll
         for (int j = 0; j < RT; ++j)
           if (r0 + i < d && c0 + j < d) {
-            if (slices == 1) A[(r0 + i) * la + c0 + j] = acc[i][j];
-            else part[sl * d * d + (r0 + i) * d + c0 + j] = acc[i][j];
+            if (slices > 1) part[sl * d * d + (r0 + i) * d + c0 + j] = part[sl * d * d + (c0 + j) * d + r0 + i] = acc[i][j];
+            else A[(r0 + i) * la + c0 + j] = A[(c0 + j) * la + r0 + i] = acc[i][j];
           }
     }
     __syncthreads();
@@ -112,15 +121,16 @@ __global__ __launch_bounds__(TH) void orth_chip_kernel(KfOrthArgs a, int slices)
       __syncthreads();
     }
     // B = b A + c A A (A is symmetric: rows for columns)
-    for (int t = threadIdx.x; t < td * td; t += TH) {
-      const int r0 = t / td * RT, c0 = t % td * RT;
+    for (int t = threadIdx.x; t < ts; t += TH) {
+      int r0, c0;
+      below(t, &r0, &c0);
       C acc[RT][RT] = {};
       for (int k = 0; k < d; ++k) {
         C u[RT], v[RT];
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
           u[i] = A[(r0 + i < d ? r0 + i : d - 1) * la + k];
-          v[i] = A[k * la + (c0 + i < d ? c0 + i : d - 1)];
+          v[i] = A[(c0 + i < d ? c0 + i : d - 1) * la + k];
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i)
@@ -131,7 +141,7 @@ __global__ __launch_bounds__(TH) void orth_chip_kernel(KfOrthArgs a, int slices)
       for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < RT; ++j)
-          if (r0 + i < d && c0 + j < d) B[(r0 + i) * la + c0 + j] = cb * A[(r0 + i) * la + c0 + j] + cc * acc[i][j];
+          if (r0 + i < d && c0 + j < d) B[(r0 + i) * la + c0 + j] = B[(c0 + j) * la + r0 + i] = cb * A[(r0 + i) * la + c0 + j] + cc * acc[i][j];
     }
     __syncthreads();
     // Y = a X + B X
@@ -172,10 +182,10 @@ ChipPlan chip_plan(const KfOrthArgs& a) {
   const size_t e = a.dtype == KF_DTYPE_F64 ? 8 : 4;
   p.fits = false;
   if (d > 64 || L > 40000) return p;
-  p.rt = d <= 16 ? 1 : d <= 32 ? 2 : 4;
+  p.rt = d <= 32 ? 2 : 4;  // (LDS bandwidth bounds these products: tiles of 2 x 2 halve it, and still leave every thread one)
   // one wave where a matrix has no work for more (then d <= 16): many of them fit a compute unit
   p.threads = d * L <= 256 ? 64 : 256;
-  const long tiles = ((d + p.rt - 1) / p.rt) * ((d + p.rt - 1) / p.rt);
+  const long td = (d + p.rt - 1) / p.rt, tiles = td * (td + 1) / 2;
   p.slices = 1;
   while (2 * p.slices * tiles <= p.threads && 2 * p.slices <= L / 8) p.slices *= 2;
   p.lds = e * (2 * d * (L | 1) + 2 * d * (d | 1) + (p.slices > 1 ? p.slices * d * d : 0));
@@ -193,33 +203,50 @@ int launch_chip(kf_handle* h, const KfOrthArgs& a, const ChipPlan& p, hipStream_
 }
 
 // ------------------------------------------------------------------------------------- |M|_F^2 in 64 bits, by parts
-constexpr int NORM_PARTS = 64;
+constexpr int NORM_PARTS = 256;
 template <typename T>
 __global__ __launch_bounds__(256) void orth_norm_kernel(const T* M, long size, double* part) {
+  constexpr int V = 16 / sizeof(T);
+  struct alignas(16) Piece { T v[V]; };
   __shared__ double red[4];
   const T* m = M + (long)blockIdx.y * size;
-  const long per = (size + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < size ? lo + per : size;
   double s = 0.;
-  for (long i = lo + threadIdx.x; i < hi; i += 256) {
+  const long step = gridDim.x * 256l, first = blockIdx.x * 256l + threadIdx.x;
+  const long head = ((uintptr_t)m & 15) ? 0 : size / V;  // whole pieces
+  for (long i = first; i < head; i += step) {
+    const Piece p = reinterpret_cast<const Piece*>(m)[i];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const double x = (double)to_acc(p.v[e]);
+      s += x * x;
+    }
+  }
+  for (long i = head * V + first; i < size; i += step) {
     const double x = (double)to_acc(m[i]);
     s += x * x;
   }
   s = block_sum(s, red);
   if (threadIdx.x == 0) part[blockIdx.y * NORM_PARTS + blockIdx.x] = s;
 }
-static __device__ __forceinline__ double norm_factor(const double* part, int parts, double eps) {
-  double s = 0.;
-  for (int i = 0; i < parts; ++i) s += part[i];
+// by a whole workgroup, the same order everywhere
+static __device__ __forceinline__ double norm_factor(const double* part, int parts, double eps, double* red) {
+  const double s = block_sum((int)threadIdx.x < parts ? part[threadIdx.x] : 0., red);
   return 1.0 / (sqrt(s) + eps);
 }
-static inline int norm_parts(long size) {
-  const long p = (size + 16383) / 16384;
+static inline int norm_parts(long size) {  // about 16 elements a thread
+  const long p = (size + 4095) / 4096;
   return p < NORM_PARTS ? (int)p : NORM_PARTS;
 }
 
 // ------------------------------------------------------------------------------------------------ fp16 parts
 constexpr float SCALE_X = 16384.f;  // 2^14: |x| <= 1.9 comes to 31130 of fp16's 65504
 constexpr float SCALE_A = 8192.f;   // 2^13: |a| <= 1.9^2 comes to 29573
+
+// Where entry (r, c) of a matrix with rows of ld entries has its hi part: alone (STORED 1), or with the lo parts of 32 columns
+// behind the hi parts of the same 32, one 128-byte line (STORED 2).
+template <int STORED> static __device__ __forceinline__ long place(long r, long c, long ld) {
+  return STORED == 1 ? r * ld + c : r * 2 * ld + ((c >> 5) << 6) + (c & 31);
+}
 
 static __device__ __forceinline__ void parts_of(f4 x, h4* hi, h4* lo) {
   *hi = __builtin_convertvector(x, h4);
@@ -228,14 +255,15 @@ static __device__ __forceinline__ void parts_of(f4 x, h4* hi, h4* lo) {
 static __device__ __forceinline__ f4 whole(h4 hi, h4 lo) { return __builtin_convertvector(hi, f4) + __builtin_convertvector(lo, f4); }
 
 // M (rows x cols) times its factor, in parts: dP x LP, zeros behind d and L, transposed where M is tall
-template <typename T>
+template <typename T, int STORED>
 __global__ __launch_bounds__(256) void orth_parts_kernel(KfOrthArgs a, const double* part, int parts, int dP, int LP, _Float16* hi, _Float16* lo) {
   __shared__ float tile[64][65];
   const bool tall = a.rows > a.cols;
   const int d = tall ? a.cols : a.rows, L = tall ? a.rows : a.cols;
-  const long z = blockIdx.z, at = z * dP * (long)LP;
+  const long z = blockIdx.z, at = z * dP * (long)LP * STORED;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  const double f = norm_factor(part + z * NORM_PARTS, parts, a.eps) * SCALE_X;
+  __shared__ double red[4];
+  const double f = norm_factor(part + z * NORM_PARTS, parts, a.eps, red) * SCALE_X;
   const T* M = (const T*)a.M + z * d * (long)L;
   if (tall) {
     for (int e = threadIdx.x; e < 4096; e += 256) {
@@ -252,7 +280,7 @@ __global__ __launch_bounds__(256) void orth_parts_kernel(KfOrthArgs a, const dou
       x[j] = tall ? tile[r][c + j] : r0 + r < d && c0 + c + j < L ? (float)((double)to_acc(M[(r0 + r) * (long)L + c0 + c + j]) * f) : 0.f;
     h4 xh, xl;
     parts_of(x, &xh, &xl);
-    const long to = at + (long)(r0 + r) * LP + c0 + c;
+    const long to = at + place<STORED>(r0 + r, c0 + c, LP);
     *(h4*)(hi + to) = xh;
     *(h4*)(lo + to) = xl;
   }
@@ -261,11 +289,11 @@ __global__ __launch_bounds__(256) void orth_parts_kernel(KfOrthArgs a, const dou
 enum { GRAM, POLY, UPDATE };
 
 struct Product {
-  int n, d, L, dP, LP;      // sizes, padded to tiles
+  int n, d, L, dP, LP;      // sizes; rows and columns are padded to dP and LP, multiples of 128
   int tiles_m, tiles_n;     // of one matrix's output
+  int depth;
   long works;
-  const _Float16 *Ph, *Pl;  // left operand, rows over the depth
-  const _Float16 *Qh, *Ql;  // right operand: rows over the depth (GRAM, POLY), or depth x columns (UPDATE)
+  const _Float16 *P, *Q;    // left operand, rows over the depth; right: rows over the depth (GRAM, POLY), or depth x columns (UPDATE)
   const _Float16 *Dh, *Dl;  // what is added: A (POLY), X (UPDATE)
   _Float16 *Ch, *Cl;        // output in parts
   void* out;                // or in T (the last UPDATE), `tall`: transposed
@@ -274,14 +302,18 @@ struct Product {
   float add;                // factor of what is added
 };
 
-// out = unscale P Q + add D, TILE x TILE of it for each workgroup of 2 x 2 waves.  Depth in steps of 32 through two LDS buffers that
-// global_load_lds fills (16 bytes a lane, no registers); the order of the 16-byte pieces inside a buffer is permuted by row so
-// that the fragment reads meet different banks.  GRAM and POLY are symmetric: tiles on and below the diagonal, stored twice.
+// out = unscale P Q + add D, TILE x TILE of it for each workgroup of 2 x 2 waves.  Depth in steps of BK through a ring of LDS buffers
+// that global_load_lds fills ahead (16 bytes a lane, no registers; each row's part of a step is one 128-byte line); the order of the
+// 16-byte pieces inside a buffer is permuted by row so that the fragment reads meet different banks.  GRAM and POLY are symmetric:
+// tiles on and below the diagonal, stored twice.
+// PARTS 1: hi parts only, stored apart from the lo parts; 2: hi and lo parts, stored together (`place`).
 template <typename T, int TILE, int PARTS, int MODE, bool LAST>
 __global__ __launch_bounds__(256, 2) void orth_product_kernel(Product p) {
-  constexpr int WT = TILE / 32, PIECES = TILE * 4, PER = PIECES / 256, GR = TILE / 16;
+  constexpr int BK = PARTS == 1 ? 64 : 32;
+  constexpr int WT = TILE / 32, PER = TILE * 8 / 256, GR = TILE * PARTS / 16;  // pieces of an operand for each thread; 32-byte groups of a depth's row
   constexpr bool NN = MODE == UPDATE;
-  __shared__ __attribute__((aligned(16))) _Float16 lds[2][2 * PARTS][TILE * 32];  // [buffer][P hi, (P lo,) Q hi(, Q lo)]
+  constexpr int RING = TILE == 128 ? 2 : 3, LOADS = 2 * PER;  // two workgroups (three of the small tiles) fit a compute unit's 160 KB
+  __shared__ __attribute__((aligned(16))) _Float16 lds[RING][2][TILE * 64];
   const long per = (p.works + 7) >> 3, work = (blockIdx.x & 7) * per + (blockIdx.x >> 3);  // neighbours on one die
   if (work >= p.works) return;
   const long tiles = p.works / p.n, z = work / tiles;
@@ -298,57 +330,45 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(Product p) {
     while (tm * (tm + 1) / 2 > x) --tm;
     tn = x - tm * (tm + 1) / 2;
   }
-  const int depth = MODE == GRAM ? p.LP : p.dP;
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, i = l & 15, g = l >> 4;
   const int wm = (w & 1) * (TILE / 2), wn = (w >> 1) * (TILE / 2);
-  const long zP = z * (long)p.dP * (MODE == GRAM ? p.LP : p.dP), zQ = z * (long)p.dP * (MODE == POLY ? p.dP : p.LP);
+  const long ldP = MODE == GRAM ? p.LP : p.dP, ldQ = MODE == POLY ? p.dP : p.LP;
+  const _Float16* P = p.P + z * PARTS * (long)p.dP * ldP;
+  const _Float16* Q = p.Q + z * PARTS * (long)p.dP * ldQ;
 
-  // source of each 16-byte piece this lane brings in, at depth 0; along the depth it moves by `step`
-  const _Float16* src[2 * PARTS][PER];
-  const long stepP = 32, stepQ = NN ? 32l * p.LP : 32;
+  // source of each 16-byte piece this lane brings in; a step further on along the depth it is 64 entries on, or BK rows
+  const _Float16 *srcP[PER], *srcQ[PER];
+  const long stepQ = NN ? (long)BK * PARTS * p.LP : 64;
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
-    const int s = tid + 256 * u;
-    const int r = s >> 2, c = (s & 3) ^ ((r >> 2) & 3);
-    const long oP = zP + (long)(tm * TILE + r) * depth + 8 * c;
-    long oQ;
+    const int s = tid + 256 * u, r = s >> 3, c = (s & 7) ^ (r & 7);
+    srcP[u] = P + (tm * TILE + r) * PARTS * ldP + 8 * c;
     if (NN) {
-      const int k = s / (TILE / 8), pos = s % (TILE / 8), gr = (pos >> 1) ^ (k & (GR - 1));
-      oQ = zQ + (long)k * p.LP + tn * TILE + 16 * gr + 8 * (pos & 1);
+      const int k = s / (2 * GR), pos = s % (2 * GR), gr = (pos >> 1) ^ (k & 7 & (GR - 1));
+      srcQ[u] = Q + k * PARTS * ldQ + tn * TILE * PARTS + 16 * gr + 8 * (pos & 1);
     } else {
-      oQ = zQ + (long)(tn * TILE + r) * depth + 8 * c;
+      srcQ[u] = Q + (tn * TILE + r) * PARTS * ldQ + 8 * c;
     }
-    src[0][u] = p.Ph + oP;
-    if (PARTS == 2) src[1][u] = p.Pl + oP;
-    src[PARTS][u] = p.Qh + oQ;
-    if (PARTS == 2) src[2 * PARTS - 1][u] = p.Ql + oQ;
   }
   auto bring = [&](int buf) {
 #pragma unroll
-    for (int k = 0; k < 2 * PARTS; ++k)
-#pragma unroll
-      for (int u = 0; u < PER; ++u) {
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[k][u],
-                                         (__attribute__((address_space(3))) void*)&lds[buf][k][(w * 64 + 256 * u) * 8], 16, 0, 0);
-        src[k][u] += k < PARTS ? stepP : stepQ;
-      }
-  };
-  auto left = [&](const _Float16* t, int r) {  // row r, at the depths the right operand comes in
-    const int sw = (r >> 2) & 3;
-    if (!NN) return *(const h8*)(t + r * 32 + 8 * (g ^ sw));
-    const h4 a = *(const h4*)(t + r * 32 + 8 * ((g >> 1) ^ sw) + 4 * (g & 1));
-    const h4 b = *(const h4*)(t + r * 32 + 8 * ((2 + (g >> 1)) ^ sw) + 4 * (g & 1));
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-  };
-  auto right = [&](const _Float16* t, int c) {  // columns c .. c + 15
-    if (!NN) {
-      const int r = c + i, sw = (r >> 2) & 3;
-      return *(const h8*)(t + r * 32 + 8 * (g ^ sw));
+    for (int u = 0; u < PER; ++u) {
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)srcP[u],
+                                       (__attribute__((address_space(3))) void*)&lds[buf][0][(w * 64 + 256 * u) * 8], 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)srcQ[u],
+                                       (__attribute__((address_space(3))) void*)&lds[buf][1][(w * 64 + 256 * u) * 8], 16, 0, 0);
+      srcP[u] += 64;
+      srcQ[u] += stepQ;
     }
+  };
+  // row r; `half`: the second 32 depths (PARTS 1), the lo parts (PARTS 2)
+  auto row = [&](const _Float16* t, int r, int half) { return *(const h8*)(t + r * 64 + 8 * ((4 * half + g) ^ (r & 7))); };
+  auto col = [&](const _Float16* t, int c, int half) {  // columns c .. c + 15 of [depth][columns], depths as `row` has them
     typedef __attribute__((address_space(3))) s4* lp;
-    const int k = 4 * g + (i >> 2);
-    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + k * TILE + 16 * ((c >> 4) ^ (k & (GR - 1))) + 4 * (i & 3)));
-    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + (k + 16) * TILE + 16 * ((c >> 4) ^ (k & (GR - 1))) + 4 * (i & 3)));
+    const int k = (PARTS == 1 ? 32 * half : 0) + 8 * g + (i >> 2);  // 4 rows for 16 lanes, and the 4 behind them
+    const int gr = PARTS == 1 ? c >> 4 : ((c >> 5) << 2) + 2 * half + ((c >> 4) & 1);
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + k * TILE * PARTS + 16 * (gr ^ (k & 7 & (GR - 1))) + 4 * (i & 3)));
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + (k + 4) * TILE * PARTS + 16 * (gr ^ ((k + 4) & 7 & (GR - 1))) + 4 * (i & 3)));
     return __builtin_bit_cast(h8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
@@ -357,42 +377,53 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(Product p) {
   for (int m = 0; m < WT; ++m)
 #pragma unroll
     for (int n = 0; n < WT; ++n) acc[m][n] = f4{0, 0, 0, 0};
-  const int steps = depth / 32;
-  bring(0);
+  const int steps = p.depth / BK;
+#pragma unroll
+  for (int s = 0; s < RING - 1; ++s)
+    if (s < steps) bring(s);
+  int buf = 0, next = RING - 1;
   for (int s = 0; s < steps; ++s) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // buffer s & 1 is filled, and nobody reads the other one any more
-    if (s + 1 < steps) bring((s + 1) & 1);
-    const _Float16(*b)[TILE * 32] = lds[s & 1];
-    h8 ph[WT], pl[WT];
+    // all but the newest RING - 2 steps' loads have arrived (at the end fewer are under way, and all are waited for), and this wave's
+    // own reads of the last step have left LDS.  (__syncthreads would wait for every load.)
+    if (RING > 2 && s + RING - 1 <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 2) * LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // this buffer is filled, and nobody reads the one before it any more
+    asm volatile("" ::: "memory");
+    if (s + RING - 1 < steps) bring(next);
+    const _Float16 *tP = lds[buf][0], *tQ = lds[buf][1];
+    buf = buf + 1 == RING ? 0 : buf + 1;
+    next = next + 1 == RING ? 0 : next + 1;
+    h8 ph[WT], pl[WT];  // PARTS 1: the step's two halves; 2: hi and lo parts
 #pragma unroll
     for (int m = 0; m < WT; ++m) {
-      ph[m] = left(b[0], wm + 16 * m + i);
-      if (PARTS == 2) pl[m] = left(b[1], wm + 16 * m + i);
+      const int r = wm + 16 * m + i;
+      ph[m] = row(tP, r, 0);
+      pl[m] = row(tP, r, 1);
     }
 #pragma unroll
     for (int n = 0; n < WT; ++n) {
-      const h8 qh = right(b[PARTS], wn + 16 * n);
-      h8 ql = qh;
-      if (PARTS == 2) ql = right(b[2 * PARTS - 1], wn + 16 * n);
+      const h8 qh = NN ? col(tQ, wn + 16 * n, 0) : row(tQ, wn + 16 * n + i, 0);
+      const h8 ql = NN ? col(tQ, wn + 16 * n, 1) : row(tQ, wn + 16 * n + i, 1);
 #pragma unroll
       for (int m = 0; m < WT; ++m) {
         if (PARTS == 2) {
           acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql, ph[m], acc[m][n], 0, 0, 0);
           acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh, pl[m], acc[m][n], 0, 0, 0);
+        } else {
+          acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql, pl[m], acc[m][n], 0, 0, 0);
         }
         acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh, ph[m], acc[m][n], 0, 0, 0);
       }
     }
   }
   const int ld = MODE == UPDATE ? p.LP : p.dP;
-  const long zC = z * (long)p.dP * ld;
+  const long zC = z * PARTS * (long)p.dP * ld;
 #pragma unroll
   for (int m = 0; m < WT; ++m)
 #pragma unroll
     for (int n = 0; n < WT; ++n) {
       const int row = tm * TILE + wm + 16 * m + i, col = tn * TILE + wn + 16 * n + 4 * g;
-      const long at = zC + (long)row * ld + col;
+      const long at = zC + place<PARTS>(row, col, ld);
       f4 v = acc[m][n] * p.unscale;
       if (MODE != GRAM) {
         const h4 dh = *(const h4*)(p.Dh + at);
@@ -411,7 +442,7 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(Product p) {
         if (MODE != UPDATE && tm != tn) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const long to = zC + (long)(col + r) * ld + row;
+            const long to = zC + place<PARTS>(col + r, row, ld);
             p.Ch[to] = vh[r];
             if (PARTS == 2) p.Cl[to] = vl[r];
           }
@@ -420,31 +451,49 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(Product p) {
     }
 }
 
-struct PartsPlan { int tile, dP, LP, td, tl; size_t x, aa, norm; };
-PartsPlan parts_plan(const kf_handle* h, const KfOrthArgs& a) {
+struct PartsPlan { int dP, LP; size_t x, aa, norm; };
+PartsPlan parts_plan(const KfOrthArgs& a) {
   PartsPlan p;
   const int d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
-  const long t = (d + 127) / 128, cu = h->n_cu > 0 ? h->n_cu : 256;
-  p.tile = a.n * t * (t + 1) / 2 >= cu ? 128 : 64;  // the symmetric products' tiles fill the card, or smaller ones
-  p.td = (d + p.tile - 1) / p.tile;
-  p.tl = (L + p.tile - 1) / p.tile;
-  p.dP = p.td * p.tile;
-  p.LP = p.tl * p.tile;
+  p.dP = (d + 127) / 128 * 128;
+  p.LP = (L + 127) / 128 * 128;
   p.x = kf_seq_round((size_t)a.n * p.dP * p.LP * 2);
   p.aa = kf_seq_round((size_t)a.n * p.dP * p.dP * 2);
   p.norm = kf_seq_round((size_t)a.n * NORM_PARTS * 8);
   return p;
 }
 
-template <typename T, int TILE, int PARTS>
+// one product: tiles of 128 where they fill the card, else of 64
+template <typename T, int PARTS, int MODE, bool LAST>
+void launch_product(const kf_handle* h, Product& p, hipStream_t stream) {
+  const long cu = h->n_cu > 0 ? h->n_cu : 256;
+  const int cols = MODE == UPDATE ? p.L : p.d;
+  auto count = [&](int tile) {
+    p.tiles_m = (p.d + tile - 1) / tile;
+    p.tiles_n = (cols + tile - 1) / tile;
+    p.works = p.n * (MODE == UPDATE ? (long)p.tiles_m * p.tiles_n : p.tiles_m * (p.tiles_m + 1L) / 2);
+  };
+  p.depth = ((MODE == GRAM ? p.L : p.d) + 63) / 64 * 64;
+  count(128);
+  const bool small = p.works < cu;
+  if (small) count(64);
+  const dim3 grid((unsigned)(8 * ((p.works + 7) / 8)));
+  if (small) hipLaunchKernelGGL((orth_product_kernel<T, 64, PARTS, MODE, LAST>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((orth_product_kernel<T, 128, PARTS, MODE, LAST>), grid, dim3(256), 0, stream, p);
+}
+
+template <typename T, int PARTS>
 int launch_parts(kf_handle* h, const KfOrthArgs& a, const PartsPlan& pl, void* ws, hipStream_t stream) {
   char* w = (char*)ws;
   double* norm = (double*)w; w += pl.norm;
-  _Float16 *X[2][2], *A[2], *B[2];
-  for (int i = 0; i < 2; ++i)
-    for (int j = 0; j < 2; ++j) X[i][j] = (_Float16*)w, w += pl.x;
-  for (int j = 0; j < 2; ++j) A[j] = (_Float16*)w, w += pl.aa;
-  for (int j = 0; j < 2; ++j) B[j] = (_Float16*)w, w += pl.aa;
+  _Float16 *X[2][2], *A[2], *B[2];  // hi, lo
+  // (stored together, the lo parts are 32 entries behind the hi parts)
+  auto take = [&](size_t bytes, _Float16** q) {
+    q[0] = (_Float16*)w;
+    q[1] = PARTS == 2 ? q[0] + 32 : (_Float16*)(w + bytes);
+    w += 2 * bytes;
+  };
+  take(pl.x, X[0]); take(pl.x, X[1]); take(pl.aa, A); take(pl.aa, B);
   const long size = (long)a.rows * a.cols;
   const int parts = norm_parts(size);
   Product p;
@@ -455,7 +504,7 @@ int launch_parts(kf_handle* h, const KfOrthArgs& a, const PartsPlan& pl, void* w
   p.dP = pl.dP; p.LP = pl.LP;
   p.out = a.X;
   hipLaunchKernelGGL(orth_norm_kernel<T>, dim3(parts, (unsigned)a.n), dim3(256), 0, stream, (const T*)a.M, size, norm);
-  hipLaunchKernelGGL(orth_parts_kernel<T>, dim3(pl.LP / 64, pl.dP / 64, (unsigned)a.n), dim3(256), 0, stream, a, norm, parts, pl.dP, pl.LP, X[0][0], X[0][1]);
+  hipLaunchKernelGGL((orth_parts_kernel<T, PARTS>), dim3(pl.LP / 64, pl.dP / 64, (unsigned)a.n), dim3(256), 0, stream, a, norm, parts, pl.dP, pl.LP, X[0][0], X[0][1]);
   for (int s = 0; s < a.steps; ++s) {
     const double ca = a.coef[s][0], cb = a.coef[s][1], cc = a.coef[s][2];
     const int from = s & 1, to = from ^ 1;
@@ -466,27 +515,22 @@ int launch_parts(kf_handle* h, const KfOrthArgs& a, const PartsPlan& pl, void* w
     int e = 0;
     frexp(fmax(bound, 1e-6), &e);
     const double scale_b = ldexp(1.0, 14 - e);  // |B| comes to at most 2^14: room for what A's rounding adds
-    p.Ph = p.Qh = X[from][0]; p.Pl = p.Ql = X[from][1];
+    p.P = p.Q = X[from][0];
     p.Ch = A[0]; p.Cl = A[1];
     p.Dh = p.Dl = nullptr;
-    p.tiles_m = p.tiles_n = pl.td;
-    p.works = a.n * pl.td * (pl.td + 1L) / 2;
     p.unscale = (float)(SCALE_A / ((double)SCALE_X * SCALE_X)); p.add = 0.f;
-    hipLaunchKernelGGL((orth_product_kernel<T, TILE, PARTS, GRAM, false>), dim3((unsigned)(8 * ((p.works + 7) / 8))), dim3(256), 0, stream, p);
-    p.Ph = p.Qh = p.Dh = A[0]; p.Pl = p.Ql = p.Dl = A[1];
+    launch_product<T, PARTS, GRAM, false>(h, p, stream);
+    p.P = p.Q = p.Dh = A[0]; p.Dl = A[1];
     p.Ch = B[0]; p.Cl = B[1];
     p.unscale = (float)(cc * scale_b / ((double)SCALE_A * SCALE_A)); p.add = (float)(cb * scale_b / SCALE_A);
-    hipLaunchKernelGGL((orth_product_kernel<T, TILE, PARTS, POLY, false>), dim3((unsigned)(8 * ((p.works + 7) / 8))), dim3(256), 0, stream, p);
-    p.Ph = B[0]; p.Pl = B[1];
-    p.Qh = p.Dh = X[from][0]; p.Ql = p.Dl = X[from][1];
+    launch_product<T, PARTS, POLY, false>(h, p, stream);
+    p.P = B[0];
+    p.Q = p.Dh = X[from][0]; p.Dl = X[from][1];
     p.Ch = X[to][0]; p.Cl = X[to][1];
-    p.tiles_n = pl.tl;
-    p.works = a.n * (long)pl.td * pl.tl;
     const bool last = s + 1 == a.steps;
     p.unscale = (float)((last ? 1.0 / SCALE_X : 1.0) / scale_b); p.add = (float)(last ? ca / SCALE_X : ca);
-    const dim3 grid((unsigned)(8 * ((p.works + 7) / 8)));
-    if (last) hipLaunchKernelGGL((orth_product_kernel<T, TILE, PARTS, UPDATE, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((orth_product_kernel<T, TILE, PARTS, UPDATE, false>), grid, dim3(256), 0, stream, p);
+    if (last) launch_product<T, PARTS, UPDATE, true>(h, p, stream);
+    else launch_product<T, PARTS, UPDATE, false>(h, p, stream);
   }
   KF_HIP_CHECK(h, hipGetLastError());
   return KF_OK;
@@ -494,10 +538,10 @@ int launch_parts(kf_handle* h, const KfOrthArgs& a, const PartsPlan& pl, void* w
 
 // ------------------------------------------------------------------------------------------------ fp64
 __global__ __launch_bounds__(256) void orth_scale64_kernel(KfOrthArgs a, const double* part, int parts, double* X) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x, size = (long)a.rows * a.cols;
-  if (i >= a.n * size) return;
-  const long z = i / size, e = i - z * size;
-  const double f = norm_factor(part + z * NORM_PARTS, parts, a.eps);
+  __shared__ double red[4];
+  const long e = (long)blockIdx.x * 256 + threadIdx.x, size = (long)a.rows * a.cols, z = blockIdx.y, i = z * size + e;
+  const double f = norm_factor(part + z * NORM_PARTS, parts, a.eps, red);
+  if (e >= size) return;
   X[a.rows > a.cols ? z * size + (e % a.cols) * a.rows + e / a.cols : i] = ((const double*)a.M)[i] * f;
 }
 
@@ -550,10 +594,10 @@ int launch64(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
   double* Y = (double*)w; w += big;
   double* A = (double*)w; w += small;
   double* B = (double*)w;
-  const long size = (long)d * L, total = a.n * size;
+  const long size = (long)d * L;
   const int parts = norm_parts(size);
   hipLaunchKernelGGL(orth_norm_kernel<double>, dim3(parts, (unsigned)a.n), dim3(256), 0, stream, (const double*)a.M, size, norm);
-  hipLaunchKernelGGL(orth_scale64_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, a, norm, parts, X);
+  hipLaunchKernelGGL(orth_scale64_kernel, dim3((unsigned)((size + 255) / 256), (unsigned)a.n), dim3(256), 0, stream, a, norm, parts, X);
   const unsigned td = (d + 63) / 64, tl = (L + 63) / 64, z = (unsigned)a.n;
   for (int s = 0; s < a.steps; ++s) {
     const bool last = s + 1 == a.steps;
@@ -571,24 +615,22 @@ template <typename T>
 int launch_t(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
   const ChipPlan c = chip_plan(a);
   if (c.fits) {
-    if (c.threads == 64) return launch_chip<T, 1, 64>(h, a, c, stream);
-    return c.rt == 1 ? launch_chip<T, 1, 256>(h, a, c, stream) : c.rt == 2 ? launch_chip<T, 2, 256>(h, a, c, stream) : launch_chip<T, 4, 256>(h, a, c, stream);
+    if (c.threads == 64) return launch_chip<T, 2, 64>(h, a, c, stream);
+    return c.rt == 2 ? launch_chip<T, 2, 256>(h, a, c, stream) : launch_chip<T, 4, 256>(h, a, c, stream);
   }
-  const PartsPlan p = parts_plan(h, a);
-  constexpr int PARTS = std::is_same<T, __hip_bfloat16>::value ? 1 : 2;
-  return p.tile == 128 ? launch_parts<T, 128, PARTS>(h, a, p, ws, stream) : launch_parts<T, 64, PARTS>(h, a, p, ws, stream);
+  return launch_parts<T, std::is_same<T, __hip_bfloat16>::value ? 1 : 2>(h, a, parts_plan(a), ws, stream);
 }
 
 }  // namespace
 
 bool kf_orthogonalise_on_chip(const KfOrthArgs& a) { return chip_plan(a).fits; }
 
-size_t kf_orthogonalise_ws(const kf_handle* h, const KfOrthArgs& a) {
+size_t kf_orthogonalise_ws(const kf_handle*, const KfOrthArgs& a) {
   if (chip_plan(a).fits) return 0;
   const size_t d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
   if (a.dtype == KF_DTYPE_F64)
     return kf_seq_round((size_t)a.n * NORM_PARTS * 8) + 2 * kf_seq_round((size_t)a.n * d * L * 8) + 2 * kf_seq_round((size_t)a.n * d * d * 8);
-  const PartsPlan p = parts_plan(h, a);
+  const PartsPlan p = parts_plan(a);
   return p.norm + 4 * p.x + 4 * p.aa;
 }
 
@@ -597,8 +639,8 @@ int kf_launch_orthogonalise(kf_handle* h, const KfOrthArgs& a, void* ws, hipStre
     case KF_DTYPE_F64: {
       const ChipPlan c = chip_plan(a);
       if (!c.fits) return launch64(h, a, ws, stream);
-      if (c.threads == 64) return launch_chip<double, 1, 64>(h, a, c, stream);
-      return c.rt == 1 ? launch_chip<double, 1, 256>(h, a, c, stream) : c.rt == 2 ? launch_chip<double, 2, 256>(h, a, c, stream) : launch_chip<double, 4, 256>(h, a, c, stream);
+      if (c.threads == 64) return launch_chip<double, 2, 64>(h, a, c, stream);
+      return c.rt == 2 ? launch_chip<double, 2, 256>(h, a, c, stream) : launch_chip<double, 4, 256>(h, a, c, stream);
     }
     case KF_DTYPE_F32: return launch_t<float>(h, a, ws, stream);
     case KF_DTYPE_BF16: return launch_t<__hip_bfloat16>(h, a, ws, stream);

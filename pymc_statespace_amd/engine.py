@@ -67,6 +67,26 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
+def _addresses(*tensors):
+    return [None if t is None else t.data_ptr() for t in tensors]
+
+
+_SEQ_DTYPES = {torch.float64: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}  # KF_DTYPE_*; 0 is for orthogonalise only
+
+
+def _newton_schulz(coefficients, steps):
+    """(number of steps, double[steps][3]) of ``KalmanEngine.orthogonalise``'s arguments."""
+    most = _lib.KF_ORTHOGONALISE_STEPS_MAX
+    c = np.asarray(coefficients, dtype=np.float64)
+    if c.shape == (3,):
+        if not 1 <= int(steps) <= most:
+            raise ValueError(f"steps must be between 1 and {most}")
+        c = np.broadcast_to(c, (int(steps), 3))
+    if c.ndim != 2 or c.shape[1] != 3 or not 1 <= c.shape[0] <= most:
+        raise ValueError(f"coefficients: (a, b, c), or 1 to {most} of them")
+    return c.shape[0], (C.c_double * (3 * c.shape[0]))(*c.ravel().tolist())
+
+
 class KalmanEngine:
     """One ``kf_handle`` bound to one GPU."""
 
@@ -683,58 +703,63 @@ class KalmanEngine:
 
 
     # ------------------------------------------------------------- sequence layers
-    def _seq(self, x, name, shape, dtype=None):
-        """A sequence operand on this device: last axis contiguous (copied if it is not), any other strides as they are."""
+    def _seq(self, x, name, ndim, shape=None, dtype=None):
+        """A sequence operand on this device: last axis contiguous (copied if it is not), any other strides as they are.  Only its
+        address and strides are used, so a tensor that is in place already is taken as it is.  ``shape``: its first axes."""
         t = x if isinstance(x, torch.Tensor) else torch.as_tensor(np.ascontiguousarray(x))
-        if len(t.shape) != len(shape) or any(want is not None and have != want for have, want in zip(t.shape, shape)):
-            raise ValueError(f"{name}: expected shape {tuple('*' if w is None else w for w in shape)}, got {tuple(t.shape)}")
+        if t.ndim != ndim or (shape is not None and t.shape[:len(shape)] != shape):
+            raise ValueError(f"{name}: expected {ndim} axes{'' if shape is None else f', the first {tuple(shape)}'}, got {tuple(t.shape)}")
         if dtype is not None and t.dtype != dtype:
             raise TypeError(f"{name} is {t.dtype}, q is {dtype}: q, k, v and g_o share one type")
-        t = t.detach().to(self.device)
-        return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+        if t.device != self.device:
+            t = t.detach().to(self.device)
+        return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.detach().contiguous()
 
     def _seq_f32(self, x, name, shape):
         """An fp32 operand (log decays, states), contiguous; other types are converted."""
         if x is None:
             return None
         t = x if isinstance(x, torch.Tensor) else torch.as_tensor(np.ascontiguousarray(x))
-        if tuple(t.shape) != tuple(shape):
+        if t.shape != shape:
             raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+        if t.dtype == torch.float32 and t.device == self.device and t.is_contiguous():
+            return t
         return t.detach().to(self.device, torch.float32).contiguous()
 
     def _seq_i32(self, x, name, B):
         if x is None:
             return None
         t = x if isinstance(x, torch.Tensor) else torch.as_tensor(np.asarray(x))
-        if tuple(t.shape) != (B,) or t.dtype not in (torch.int32, torch.int64):
+        if t.shape != (B,) or t.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{name}: expected {B} whole numbers (int32 or int64), got {tuple(t.shape)} of {t.dtype}")
         if t.dtype == torch.int64:  # what does not fit 32 bits stays out of range
             t = t.clamp(-1, 2**31 - 1)
-        return t.detach().to(self.device, torch.int32).contiguous()
+        return t.to(self.device, torch.int32).contiguous()
 
-    def _attention_args(self, q, k, v, log_decay, scale, step=False):
-        lead = (None,) if step else (None, None)
-        q = self._seq(q, "q", lead + (None, None))
-        if str(q.dtype).replace("torch.", "") not in ("float32", "bfloat16", "float16"):
-            raise TypeError(f"q is {q.dtype}: float32, bfloat16 or float16")
-        lead, (G, K) = tuple(q.shape[:-2]), q.shape[-2:]
-        k = self._seq(k, "k", lead + (G, K), q.dtype)
-        v = self._seq(v, "v", lead + (None, None), q.dtype)
+    def _attention_args(self, q, k, v, log_decay, scale, step=False, g_o=None):
+        ndim = 3 if step else 4
+        q = self._seq(q, "q", ndim)
+        dtype, shape = q.dtype, q.shape
+        code = _SEQ_DTYPES.get(dtype)
+        if not code:
+            raise TypeError(f"q is {dtype}: float32, bfloat16 or float16")
+        lead, G, K = shape[:-2], shape[-2], shape[-1]
+        k = self._seq(k, "k", ndim, shape, dtype)
+        v = self._seq(v, "v", ndim, lead, dtype)
         H, V = v.shape[-2:]
         per_token = getattr(log_decay, "ndim", 1) > 1
-        g = self._seq_f32(log_decay, "log_decay", lead + (H,) if per_token else (H,))
+        g = self._seq_f32(log_decay, "log_decay", (*lead, H) if per_token else (H,))
         if scale is None:
             scale = 1.0 / max(K, 1) ** 0.5
-        d = _lib.KfAttentionDims(lead[0], 1 if step else lead[1], G, H, K, V, _lib.KF_DTYPE[str(q.dtype).replace("torch.", "")],
-                                 1 if per_token else 0, float(scale))
-        for field, t in (("q_stride", q), ("k_stride", k), ("v_stride", v)):
-            self._strides(d, field, t)
-        return d, q, k, v, g
-
-    @staticmethod
-    def _strides(d, field, t):
-        st = t.stride()
-        getattr(d, field)[:] = (st[0], 0, st[1]) if t.ndim == 3 else (st[0], st[1], st[2])
+        if step:
+            strides = [(s[0], 0, s[1]) for s in (q.stride(), k.stride(), v.stride())]
+            return _lib.KfAttentionDims(lead[0], 1, G, H, K, V, code, per_token, scale, *strides), q, k, v, g
+        strides = [s[:3] for s in (q.stride(), k.stride(), v.stride())]
+        d = (*lead, G, H, K, V, code, per_token, scale, *strides)
+        if g_o is None:
+            return _lib.KfAttentionDims(*d), q, k, v, g
+        g_o = self._seq(g_o, "g_o", ndim, v.shape, dtype)
+        return _lib.KfAttentionDims(*d, g_o.stride()[:3]), q, k, v, g, g_o
 
     def _scratch(self, nbytes):
         """Workspace of one call.  From torch's allocator each time: on the current stream, and inside a graph's capture from that
@@ -751,13 +776,13 @@ class KalmanEngine:
         d, q, k, v, g = self._attention_args(q, k, v, log_decay, scale)
         s0 = self._seq_f32(initial_state, "initial_state", (d.B, d.H, d.K, d.V))
         lengths = self._seq_i32(lengths, "lengths", d.B)
-        o = torch.empty(d.B, d.T, d.H, d.V, device=self.device, dtype=q.dtype)
+        o = torch.empty(v.shape, device=self.device, dtype=q.dtype)
         state = torch.empty(d.B, d.H, d.K, d.V, device=self.device, dtype=torch.float32)
         nbytes = C.c_size_t(0)
         self._check(self.lib.kf_linear_attention_workspace(self._h, C.byref(d), 0, C.byref(nbytes)), "kf_linear_attention")
         ws = self._scratch(nbytes)
-        rc = self.lib.kf_linear_attention(self._h, C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(s0), _ptr(lengths), _ptr(o),
-                                          _ptr(state), _ptr(ws), nbytes.value, self._stream())
+        rc = self.lib.kf_linear_attention(self._h, C.byref(d), *_addresses(q, k, v, g, s0, lengths, o, state, ws),
+                                          nbytes.value, self._stream())
         self._check(rc, "kf_linear_attention")
         return o, state
 
@@ -765,9 +790,7 @@ class KalmanEngine:
         """kf_linear_attention_backward: the gradient of <g_o, o> + <g_final_state, state> of ``linear_attention`` on the same
         arguments -> dict(q, k, v, log_decay, initial_state) (initial_state None when none was given); q, k, v in their type,
         the others fp32.  Nothing of the forward call is needed."""
-        d, q, k, v, g = self._attention_args(q, k, v, log_decay, scale)
-        go = self._seq(g_o, "g_o", (d.B, d.T, d.H, d.V), q.dtype)
-        self._strides(d, "g_o_stride", go)
+        d, q, k, v, g, go = self._attention_args(q, k, v, log_decay, scale, g_o=g_o)
         s0 = self._seq_f32(initial_state, "initial_state", (d.B, d.H, d.K, d.V))
         gs = self._seq_f32(g_final_state, "g_final_state", (d.B, d.H, d.K, d.V))
         lengths = self._seq_i32(lengths, "lengths", d.B)
@@ -778,8 +801,7 @@ class KalmanEngine:
         self._check(self.lib.kf_linear_attention_workspace(self._h, C.byref(d), 1, C.byref(nbytes)), "kf_linear_attention_backward")
         ws = self._scratch(nbytes)
         rc = self.lib.kf_linear_attention_backward(
-            self._h, C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(s0), _ptr(lengths), _ptr(go), _ptr(gs), _ptr(out["q"]),
-            _ptr(out["k"]), _ptr(out["v"]), _ptr(out["log_decay"]), _ptr(out["initial_state"]), _ptr(ws), nbytes.value, self._stream())
+            self._h, C.byref(d), *_addresses(q, k, v, g, s0, lengths, go, gs, *out.values(), ws), nbytes.value, self._stream())
         self._check(rc, "kf_linear_attention_backward")
         return out
 
@@ -790,19 +812,19 @@ class KalmanEngine:
         empty row (o zero), one >= N as well, with info 1; rows with the same slot are consecutive tokens of that sequence."""
         d, q, k, v, g = self._attention_args(q, k, v, log_decay, scale, step=True)
         N = state.shape[0] if getattr(state, "ndim", 0) else 0
-        for name, t in (("state", state), ("state_out", state if state_out is None else state_out)):
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != self.device or not t.is_contiguous() or \
-                    tuple(t.shape) != (N, d.H, d.K, d.V):
-                raise ValueError(f"{name} must be a contiguous fp32 tensor (N, {d.H}, {d.K}, {d.V}) on {self.device}: it is used in place")
         out = state if state_out is None else state_out
-        if out.data_ptr() != state.data_ptr() and out.data_ptr() < state.data_ptr() + 4 * state.numel() and \
-                state.data_ptr() < out.data_ptr() + 4 * out.numel():
+        for name, t in (("state", state), ("state_out", out)):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != self.device or not t.is_contiguous() or \
+                    t.shape != (N, d.H, d.K, d.V):
+                raise ValueError(f"{name} must be a contiguous fp32 tensor (N, {d.H}, {d.K}, {d.V}) on {self.device}: it is used in place")
+        here, there = state.data_ptr(), out.data_ptr()
+        if here != there and abs(here - there) < 4 * state.numel():
             raise ValueError("state_out overlaps state without being it")
         slots = self._seq_i32(slots, "slots", d.B)
-        o = torch.empty(d.B, d.H, d.V, device=self.device, dtype=q.dtype)
+        o = torch.empty(v.shape, device=self.device, dtype=q.dtype)
         info = torch.empty(d.B, device=self.device, dtype=torch.int32)
-        rc = self.lib.kf_linear_attention_step(self._h, C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(slots), N, _ptr(state.detach()),
-                                               _ptr(out.detach()), _ptr(o), _ptr(info), self._stream())
+        rc = self.lib.kf_linear_attention_step(self._h, C.byref(d), *_addresses(q, k, v, g, slots), N, here, there, *_addresses(o, info),
+                                               self._stream())
         self._check(rc, "kf_linear_attention_step")
         return o, info
 
@@ -812,28 +834,21 @@ class KalmanEngine:
         (float64, float32, bfloat16, float16).  ``coefficients``: one (a, b, c) used ``steps`` times, or a list of them, one for each
         step.  For instance an update of weights from their gradient, or of a batch of transition matrices from ``value_and_grad``'s."""
         t = M if isinstance(M, torch.Tensor) else torch.as_tensor(np.ascontiguousarray(M))
-        if str(t.dtype).replace("torch.", "") not in _lib.KF_DTYPE:
+        code = _SEQ_DTYPES.get(t.dtype)
+        if code is None:
             raise TypeError(f"M is {t.dtype}: float64, float32, bfloat16 or float16")
         if t.ndim < 2 or t.numel() == 0:
             raise ValueError(f"M must be (..., rows, cols) and not empty, got {tuple(t.shape)}")
-        coef = np.asarray(coefficients, dtype=np.float64)
-        if coef.shape == (3,):
-            if not 1 <= int(steps) <= _lib.KF_ORTHOGONALISE_STEPS_MAX:
-                raise ValueError(f"steps must be between 1 and {_lib.KF_ORTHOGONALISE_STEPS_MAX}")
-            coef = np.repeat(coef[None], int(steps), 0)
-        if coef.ndim != 2 or coef.shape[1] != 3 or not 1 <= coef.shape[0] <= _lib.KF_ORTHOGONALISE_STEPS_MAX:
-            raise ValueError(f"coefficients: (a, b, c), or 1 to {_lib.KF_ORTHOGONALISE_STEPS_MAX} of them")
-        t = t.detach().to(self.device).contiguous()
+        count, coef = _newton_schulz(coefficients, steps)
+        if t.device != self.device or not t.is_contiguous():
+            t = t.detach().to(self.device).contiguous()
         rows, cols = t.shape[-2:]
         n = t.numel() // (rows * cols)
-        X = torch.empty_like(t)
-        code = _lib.KF_DTYPE[str(t.dtype).replace("torch.", "")]
+        X = torch.empty(t.shape, device=self.device, dtype=t.dtype)
         nbytes = C.c_size_t(0)
         self._check(self.lib.kf_orthogonalise_workspace(self._h, n, rows, cols, code, C.byref(nbytes)), "kf_orthogonalise")
         ws = self._scratch(nbytes)
-        coef = np.ascontiguousarray(coef)
-        rc = self.lib.kf_orthogonalise(self._h, n, rows, cols, code, coef.shape[0], coef.ctypes.data_as(C.POINTER(C.c_double)), float(eps),
-                                       _ptr(t), _ptr(X), _ptr(ws), nbytes.value, self._stream())
+        rc = self.lib.kf_orthogonalise(self._h, n, rows, cols, code, count, coef, eps, *_addresses(t, X, ws), nbytes.value, self._stream())
         self._check(rc, "kf_orthogonalise")
         return X
 
