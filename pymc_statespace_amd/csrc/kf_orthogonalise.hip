@@ -1,6 +1,7 @@
 // kf_orthogonalise.hip -- a batch of matrices moved towards their orthogonal factors by Newton-Schulz products:
 //     X = M / (|M|_F + eps);   per step   A = X X',   X <- a X + (b A + c A A) X
-// on the transpose where there are more rows than columns: X is d x L with d <= L.  Three ways, by size and type:
+// on the transpose where there are more rows than columns: X is d x L with d <= L.  Four ways, by size and type:
+//   * d <= 16, L <= 64: one wave for each matrix, all steps in its registers
 //   * d <= 64 and both copies of X in LDS: one workgroup for each matrix, all steps on chip, in 32 bits (64 for fp64)
 //   * larger, up to 32 bits: tiled products on v_mfma_f32_16x16x32_f16, numbers held in fp16 parts (below)
 //   * larger, fp64: tiled products in fp64
@@ -40,11 +41,105 @@ template <typename X> static __device__ __forceinline__ X block_sum(X s, X* red)
   return s;
 }
 
+// ------------------------------------------------------------------------------------- in the registers of one wave
+// d <= 16, L <= 16 NT.  Tiles of 16 x 16 as v_mfma_*_16x16x4 leave them: lane (g, c) holds column c of rows r(s, g), s = 0 .. 3.
+// The same registers are the right operand of a product that runs over those rows, and the left operand's transpose.  X is kept in
+// both orientations, x = X, y = X': A = y'y, A A and B X = (B)'x, X'B = (x)'B then need no other lane's values.
+template <typename C> struct Tile;
+template <> struct Tile<double> {
+  typedef double type __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ int row(int s, int g) { return 4 * s + g; }
+  static __device__ __forceinline__ type mma(type a, type b, type c) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s], b[s], c, 0, 0, 0);
+    return c;
+  }
+};
+template <> struct Tile<float> {
+  typedef f4 type;
+  static __device__ __forceinline__ int row(int s, int g) { return 4 * g + s; }
+  static __device__ __forceinline__ type mma(type a, type b, type c) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <typename T, int NT>
+__global__ __launch_bounds__(256) void orth_wave_kernel(KfOrthArgs a) {
+  typedef typename Acc<T>::type C;
+  typedef Tile<C> Q;
+  typedef typename Q::type V;
+  const long z = blockIdx.x * 4l + (threadIdx.x >> 6);
+  if (z >= a.n) return;
+  const int l = threadIdx.x & 63, g = l >> 4, c = l & 15;
+  const bool tall = a.rows > a.cols;
+  const int d = tall ? a.cols : a.rows, L = tall ? a.rows : a.cols;
+  const int sr = tall ? 1 : a.cols, sc = tall ? a.cols : 1;  // strides of X's rows and columns in M
+  const T* M = (const T*)a.M + z * d * L;
+  V x[NT], y[NT];
+  double sum = 0.;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int r = Q::row(s, g);
+      x[t][s] = r < d && 16 * t + c < L ? to_acc(M[r * sr + (16 * t + c) * sc]) : C(0);
+      y[t][s] = c < d && 16 * t + r < L ? to_acc(M[c * sr + (16 * t + r) * sc]) : C(0);
+      sum += (double)x[t][s] * (double)x[t][s];
+    }
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) sum += __shfl_xor(sum, m);
+  const double f = 1.0 / (sqrt(sum) + a.eps);
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      x[t][s] = (C)((double)x[t][s] * f);
+      y[t][s] = (C)((double)y[t][s] * f);
+    }
+  const V zero = {C(0), C(0), C(0), C(0)};
+  for (int step = 0; step < a.steps; ++step) {
+    const C ca = (C)a.coef[step][0], cb = (C)a.coef[step][1], cc = (C)a.coef[step][2];
+    V A = zero;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) A = Q::mma(y[t], y[t], A);
+    const V B = cb * A + cc * Q::mma(A, A, zero);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const V u = ca * x[t], v = ca * y[t];
+      y[t] = Q::mma(x[t], B, v);
+      x[t] = Q::mma(B, x[t], u);
+    }
+  }
+  T* out = (T*)a.X + z * d * L;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int r = Q::row(s, g);
+      if (r < d && 16 * t + c < L) out[r * sr + (16 * t + c) * sc] = from_acc<T>(x[t][s]);
+    }
+}
+
+template <typename T>
+int launch_wave(kf_handle* h, const KfOrthArgs& a, hipStream_t stream) {
+  const int L = a.rows > a.cols ? a.rows : a.cols;
+  const dim3 grid((unsigned)((a.n + 3) / 4));
+  if (L <= 16) hipLaunchKernelGGL((orth_wave_kernel<T, 1>), grid, dim3(256), 0, stream, a);
+  else if (L <= 32) hipLaunchKernelGGL((orth_wave_kernel<T, 2>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((orth_wave_kernel<T, 4>), grid, dim3(256), 0, stream, a);
+  KF_HIP_CHECK(h, hipGetLastError());
+  return KF_OK;
+}
+static inline bool fits_wave(const KfOrthArgs& a) { return (a.rows <= 16 && a.cols <= 64) || (a.cols <= 16 && a.rows <= 64); }
+
 // ----------------------------------------------------------------------------------------------------- on chip
 // Output tiles of RT x RT for each thread.  Where there are fewer tiles of A than threads the sum over L is cut into `slices`.
-template <typename T, int RT, int TH>
-__global__ __launch_bounds__(TH) void orth_chip_kernel(KfOrthArgs a, int slices) {
+template <typename T, int RT>
+__global__ __launch_bounds__(256) void orth_chip_kernel(KfOrthArgs a, int slices) {
   typedef typename Acc<T>::type C;
+  constexpr int TH = 256;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ double red[TH / 64];
   const bool tall = a.rows > a.cols;
@@ -175,7 +270,7 @@ __global__ __launch_bounds__(TH) void orth_chip_kernel(KfOrthArgs a, int slices)
   }
 }
 
-struct ChipPlan { int rt, threads, slices; size_t lds; bool fits; };
+struct ChipPlan { int rt, slices; size_t lds; bool fits; };
 ChipPlan chip_plan(const KfOrthArgs& a) {
   ChipPlan p;
   const long d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
@@ -183,21 +278,19 @@ ChipPlan chip_plan(const KfOrthArgs& a) {
   p.fits = false;
   if (d > 64 || L > 40000) return p;
   p.rt = d <= 32 ? 2 : 4;  // (LDS bandwidth bounds these products: tiles of 2 x 2 halve it, and still leave every thread one)
-  // one wave where a matrix has no work for more (then d <= 16): many of them fit a compute unit
-  p.threads = d * L <= 256 ? 64 : 256;
   const long td = (d + p.rt - 1) / p.rt, tiles = td * (td + 1) / 2;
   p.slices = 1;
-  while (2 * p.slices * tiles <= p.threads && 2 * p.slices <= L / 8) p.slices *= 2;
+  while (2 * p.slices * tiles <= 256 && 2 * p.slices <= L / 8) p.slices *= 2;
   p.lds = e * (2 * d * (L | 1) + 2 * d * (d | 1) + (p.slices > 1 ? p.slices * d * d : 0));
   p.fits = p.lds <= 156 * 1024;
   return p;
 }
 
-template <typename T, int RT, int TH>
+template <typename T, int RT>
 int launch_chip(kf_handle* h, const KfOrthArgs& a, const ChipPlan& p, hipStream_t stream) {
-  KF_HIP_CHECK(h, hipFuncSetAttribute(reinterpret_cast<const void*>(orth_chip_kernel<T, RT, TH>),
+  KF_HIP_CHECK(h, hipFuncSetAttribute(reinterpret_cast<const void*>(orth_chip_kernel<T, RT>),
                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds));
-  hipLaunchKernelGGL((orth_chip_kernel<T, RT, TH>), dim3((unsigned)a.n), dim3(TH), p.lds, stream, a, p.slices);
+  hipLaunchKernelGGL((orth_chip_kernel<T, RT>), dim3((unsigned)a.n), dim3(256), p.lds, stream, a, p.slices);
   KF_HIP_CHECK(h, hipGetLastError());
   return KF_OK;
 }
@@ -613,20 +706,18 @@ int launch64(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
 
 template <typename T>
 int launch_t(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
+  if (fits_wave(a)) return launch_wave<T>(h, a, stream);
   const ChipPlan c = chip_plan(a);
-  if (c.fits) {
-    if (c.threads == 64) return launch_chip<T, 2, 64>(h, a, c, stream);
-    return c.rt == 2 ? launch_chip<T, 2, 256>(h, a, c, stream) : launch_chip<T, 4, 256>(h, a, c, stream);
-  }
+  if (c.fits) return c.rt == 2 ? launch_chip<T, 2>(h, a, c, stream) : launch_chip<T, 4>(h, a, c, stream);
   return launch_parts<T, std::is_same<T, __hip_bfloat16>::value ? 1 : 2>(h, a, parts_plan(a), ws, stream);
 }
 
 }  // namespace
 
-bool kf_orthogonalise_on_chip(const KfOrthArgs& a) { return chip_plan(a).fits; }
+bool kf_orthogonalise_on_chip(const KfOrthArgs& a) { return fits_wave(a) || chip_plan(a).fits; }
 
 size_t kf_orthogonalise_ws(const kf_handle*, const KfOrthArgs& a) {
-  if (chip_plan(a).fits) return 0;
+  if (kf_orthogonalise_on_chip(a)) return 0;
   const size_t d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
   if (a.dtype == KF_DTYPE_F64)
     return kf_seq_round((size_t)a.n * NORM_PARTS * 8) + 2 * kf_seq_round((size_t)a.n * d * L * 8) + 2 * kf_seq_round((size_t)a.n * d * d * 8);
@@ -637,10 +728,10 @@ size_t kf_orthogonalise_ws(const kf_handle*, const KfOrthArgs& a) {
 int kf_launch_orthogonalise(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
   switch (a.dtype) {
     case KF_DTYPE_F64: {
+      if (fits_wave(a)) return launch_wave<double>(h, a, stream);
       const ChipPlan c = chip_plan(a);
       if (!c.fits) return launch64(h, a, ws, stream);
-      if (c.threads == 64) return launch_chip<double, 2, 64>(h, a, c, stream);
-      return c.rt == 2 ? launch_chip<double, 2, 256>(h, a, c, stream) : launch_chip<double, 4, 256>(h, a, c, stream);
+      return c.rt == 2 ? launch_chip<double, 2>(h, a, c, stream) : launch_chip<double, 4>(h, a, c, stream);
     }
     case KF_DTYPE_F32: return launch_t<float>(h, a, ws, stream);
     case KF_DTYPE_BF16: return launch_t<__hip_bfloat16>(h, a, ws, stream);
