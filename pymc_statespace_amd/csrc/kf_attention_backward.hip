@@ -23,36 +23,36 @@ struct Split {
   long works;
   int segments, seg_chunks;
   long chunks;
-  int vec_q, vec_k, vec_v, vec_g;
   float *adds_s, *adds_r, *factors;  // [B H][segments - 1][D D], [B H][segments] (each segment's whole decay)
   kf_u32x4* starts;                  // S_0 of every chunk: [B H][chunks][D / 32][2][threads]
   float *part_q, *part_k;            // [B][T][H][K], where heads share q and k
   double* part_decay;                // [B H][segments], where decays are fixed
 };
 
-template <int C, typename A, typename T, int D>
+template <int C, typename A, typename T, int D, int MODE>
 struct Stage {  // C rows of a tensor through registers into LDS
+  typedef KfRow<A, T, MODE> Row;
   static constexpr int N = C * D / 8 / (4 * D), LD = D + A::PAD;
-  typename A::frag r[N];
-  __device__ __forceinline__ void load(const T* p, long stride, long t0, long n, int dim, bool vec) {
+  typename Row::Raw r[N];
+  static __device__ __forceinline__ int last_row(long t0, long n) { return (int)(n - t0 < C ? n - t0 : C) - 1; }
+  __device__ __forceinline__ void load(const T* p, long stride, long t0, long n, int dim) {  // t0 < n
+    const int last = last_row(t0, n), row0 = threadIdx.x / (D / 8), col = 8 * (threadIdx.x % (D / 8));
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int x = threadIdx.x + 4 * D * u, row = x / (D / 8), col = 8 * (x % (D / 8));
-      r[u] = KfLoad8<A, T>::load(p + (t0 + row) * stride + col, t0 + row < n ? dim - col : 0, vec);
+      const int row = row0 + 32 * u;
+      r[u] = Row::raw(p + t0 * stride + (row < last ? row : last) * stride, col, dim);
     }
   }
-  __device__ __forceinline__ void put(typename A::elem* s) const {
+  __device__ __forceinline__ void put(typename A::elem* s, long t0, long n, int dim) const {  // the chunk that was loaded
+    const int last = last_row(t0, n), row0 = threadIdx.x / (D / 8), col = 8 * (threadIdx.x % (D / 8));
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int x = threadIdx.x + 4 * D * u;
-      A::put8(s + (x / (D / 8)) * LD + 8 * (x % (D / 8)), r[u]);
-    }
+    for (int u = 0; u < N; ++u) A::put8(s + (row0 + 32 * u) * LD + col, Row::finish(r[u], col, dim, row0 + 32 * u <= last));
   }
 };
 
 // One sweep over a segment's chunks of acc[v][k] <- E acc + sum_t weight_t y_t x_t': S (x = k, y = v, forward in time) or R (x = q,
 // y = do, backward).  STARTS: S, started from the segments before, kept at every chunk's start; else what the segment adds.
-template <typename A, typename T, int D, bool STARTS>
+template <typename A, typename T, int D, int MODE, bool STARTS>
 __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Split sp) {
   constexpr int C = chunk_of<A>(), LD = D + A::PAD, NT = D / 16, TH = 4 * D;
   typedef typename A::elem E;
@@ -80,7 +80,6 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
   const T* x = back ? (const T*)a.q + b * a.qs[0] + grp * a.qs[2] : (const T*)a.k + b * a.ks[0] + grp * a.ks[2];
   const T* y = back ? (const T*)a.g_o + b * a.gs[0] + h * a.gs[2] : (const T*)a.v + b * a.vs[0] + h * a.vs[2];
   const long xs = back ? a.qs[1] : a.ks[1], ys = back ? a.gs[1] : a.vs[1];
-  const bool vx = back ? sp.vec_q : sp.vec_k, vy = back ? sp.vec_g : sp.vec_v;
   const float* ld = a.log_decay + (a.per_token ? b * a.T * a.H + h : (long)h);
   const long c0 = (long)seg * sp.seg_chunks, c1 = c0 + sp.seg_chunks < sp.chunks ? c0 + sp.seg_chunks : sp.chunks;
   const long live = (n + C - 1) / C, last = c1 < live ? c1 : live;  // chunks that hold tokens: c0 .. last - 1
@@ -105,14 +104,14 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
     }
   }
   float through = 1.f;
-  Stage<C, A, T, D> rx, ry;
+  Stage<C, A, T, D, MODE> rx, ry;
   float rg = 0.f;
   const long steps = last > c0 ? last - c0 : 0;
   auto at = [&](long s) { return back ? last - 1 - s : c0 + s; };
   auto decay_of = [&](long c) { return l < C && c * C + l < n ? (a.per_token ? ld[(c * C + l) * a.H] : ld[0]) : 0.f; };
   if (steps) {
-    rx.load(x, xs, at(0) * C, n, a.K, vx);
-    ry.load(y, ys, at(0) * C, n, a.V, vy);
+    rx.load(x, xs, at(0) * C, n, a.K);
+    ry.load(y, ys, at(0) * C, n, a.V);
     if (w == 0) dec[0].fill(decay_of(at(0)), l < C && at(0) * C + l < n);
   }
   for (long s = 0; s < steps; ++s) {
@@ -127,14 +126,14 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
       }
       if (s + 1 == steps && seg == sp.segments - 1) break;  // the state behind the last token is not asked for
     }
-    rx.put(sX);
-    ry.put(sY);
+    rx.put(sX, at(s) * C, n, a.K);
+    ry.put(sY, at(s) * C, n, a.V);
     __syncthreads();
     const bool more = s + 1 < steps;
     const int wd = (int)((s + 1) % NT);  // the wave that computes the next chunk's decays
     if (more) {
-      rx.load(x, xs, at(s + 1) * C, n, a.K, vx);
-      ry.load(y, ys, at(s + 1) * C, n, a.V, vy);
+      rx.load(x, xs, at(s + 1) * C, n, a.K);
+      ry.load(y, ys, at(s + 1) * C, n, a.V);
       if (w == wd) rg = decay_of(at(s + 1));
     }
     const KfChunkDecay<C>& d = dec[s & 1];
@@ -150,7 +149,7 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
         const int tok = 32 * u + 16 * (e >> 2) + 4 * g + (e & 3);
         wt[e] = back ? d.from_start[tok] * a.scale : d.to_end[tok];
       }
-      KfWeighted<A> xw;
+      KfSplit<A> xw;
       xw.set(A::col(sX + 32 * u * LD + 16 * w, LD, i, g), wt);
 #pragma unroll
       for (int t = 0; t < NT; ++t) acc[t] = xw.mma_right(A::col(sY + 32 * u * LD + 16 * t, LD, i, g), acc[t]);
@@ -167,7 +166,7 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
   }
 }
 
-template <typename A, typename T, int D>
+template <typename A, typename T, int D, int MODE>
 __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a, Split sp) {
   constexpr int C = chunk_of<A>(), LD = D + A::PAD, LP = C + A::PAD, NT = D / 16, CT = C / 16, TH = 4 * D;
   typedef typename A::elem E;
@@ -246,14 +245,14 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
   }
   for (int x = tid; x < 2 * C * LP; x += TH) sP[x] = E(0);  // tiles above the diagonal stay zero
 
-  Stage<C, A, T, D> rq, rk, rv, rd;
+  Stage<C, A, T, D, MODE> rq, rk, rv, rd;
   float rg = 0.f;
   kf_u32x4 S0[D / 32][2];
   auto load = [&](long c) {
-    rq.load(q, a.qs[1], c * C, n, a.K, sp.vec_q);
-    rk.load(k, a.ks[1], c * C, n, a.K, sp.vec_k);
-    rv.load(v, a.vs[1], c * C, n, a.V, sp.vec_v);
-    rd.load(go, a.gs[1], c * C, n, a.V, sp.vec_g);
+    rq.load(q, a.qs[1], c * C, n, a.K);
+    rk.load(k, a.ks[1], c * C, n, a.K);
+    rv.load(v, a.vs[1], c * C, n, a.V);
+    rd.load(go, a.gs[1], c * C, n, a.V);
   };
   auto load_start = [&](long c) {
     const kf_u32x4* in = sp.starts + (bh * sp.chunks + c) * (D / 32 * 2 * TH) + tid;
@@ -273,10 +272,10 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
   int turn = 0;
   for (long c = last - 1; c >= c0; --c, turn ^= 1) {
     const long t0 = c * C;
-    rq.put(sQ);
-    rk.put(sK);
-    rv.put(sV);
-    rd.put(sG);
+    rq.put(sQ, t0, n, a.K);
+    rk.put(sK, t0, n, a.K);
+    rv.put(sV, t0, n, a.V);
+    rd.put(sG, t0, n, a.V);
 #pragma unroll
     for (int t = 0; t < NT; ++t) A::put4(sR + (16 * w + i) * LD + 16 * t + 4 * g, R[t]);
     __syncthreads();
@@ -300,11 +299,14 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
       }
       kf_f32x4 p, pb, wj;
       float wi = 0.f;
+      kf_f32x4 fac;
+      if (it == jt) fac = d.pairs(row, 16 * jt + 4 * g) * a.scale;
+      else fac = *reinterpret_cast<const kf_f32x4*>(&d.to_tile_end[16 * jt + 4 * g]) * (d.from_tile[jt][row] * a.scale);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = 16 * jt + 4 * g + r;
         const bool in = j <= row;
-        const float f = a.scale * (it == jt ? d.pair(row, j) : d.from_tile[jt < CT - 1 ? jt : 0][row] * d.to_tile_end[j]);
+        const float f = fac[r];
         p[r] = in ? sa[r] * f : 0.f;
         pb[r] = in ? sb[r] * f : 0.f;
         wj[r] = in ? sa[r] * pb[r] : 0.f;
@@ -391,7 +393,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
       float wt[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) wt[e] = a.scale * d.from_start[32 * u + 16 * (e >> 2) + 4 * g + (e & 3)];
-      KfWeighted<A> qw;
+      KfSplit<A> qw;
       qw.set(cq, wt);
 #pragma unroll
       for (int t = 0; t < NT; ++t) R[t] = qw.mma_right(A::col(sG + 32 * u * LD + 16 * t, LD, i, g), R[t]);
@@ -402,13 +404,13 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
       const int c4 = 16 * w + 4 * g;
       if (tok < a.T) {
         if (tok >= n) dq[t] = dk[t] = dv[t] = kf_f32x4{0, 0, 0, 0};
-        kf_store4((T*)a.g_v + row * a.V + c4, dv[t], a.V - c4, a.V % 4 == 0);
+        kf_store4((T*)a.g_v + row * a.V + c4, dv[t], a.V - c4);
         if (shared_heads) {
-          kf_store4(sp.part_q + row * a.K + c4, dq[t], a.K - c4, a.K % 4 == 0);
-          kf_store4(sp.part_k + row * a.K + c4, dk[t], a.K - c4, a.K % 4 == 0);
+          kf_store4(sp.part_q + row * a.K + c4, dq[t], a.K - c4);
+          kf_store4(sp.part_k + row * a.K + c4, dk[t], a.K - c4);
         } else {
-          kf_store4((T*)a.g_q + row * a.K + c4, dq[t], a.K - c4, a.K % 4 == 0);
-          kf_store4((T*)a.g_k + row * a.K + c4, dk[t], a.K - c4, a.K % 4 == 0);
+          kf_store4((T*)a.g_q + row * a.K + c4, dq[t], a.K - c4);
+          kf_store4((T*)a.g_k + row * a.K + c4, dk[t], a.K - c4);
         }
       }
     }
@@ -485,6 +487,7 @@ __global__ __launch_bounds__(64) void attention_decay_kernel(KfAttnArgs a, const
 
 struct Plan {
   int D;
+  int mode;
   Split sp;
   size_t adds, factors, starts, part, decay;
   size_t bytes() const { return 2 * adds + factors + starts + 2 * part + decay; }
@@ -493,7 +496,8 @@ struct Plan {
 Plan plan(const kf_handle* h, const KfAttnArgs& a) {
   Plan p;
   const int most = a.K > a.V ? a.K : a.V, C = a.dtype == KF_DTYPE_BF16 ? chunk_of<KfBf16>() : chunk_of<KfF32>();
-  p.D = most <= 32 ? 32 : most <= 64 ? 64 : 128;
+  p.mode = kf_rows_mode(a.K, a.V);
+  p.D = p.mode == KF_ROWS_NARROW ? 128 : most <= 32 ? 32 : most <= 64 ? 64 : 128;
   Split& s = p.sp;
   s.chunks = (a.T + C - 1) / C;
   const long rows = a.B * a.H, cu = h->n_cu > 0 ? h->n_cu : 256;
@@ -516,7 +520,7 @@ Plan plan(const kf_handle* h, const KfAttnArgs& a) {
   return p;
 }
 
-template <typename A, typename T, int D>
+template <typename A, typename T, int D, int MODE>
 int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream) {
   constexpr int C = chunk_of<A>(), LD = D + A::PAD, LP = C + A::PAD;
   constexpr size_t lds = sizeof(typename A::elem) * ((4 * C + D) * LD + 2 * C * LP) + 2 * sizeof(KfChunkDecay<C>) +
@@ -526,12 +530,12 @@ int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream)
   if (s.segments > 1) {
     Split two = s;
     two.works = 2 * (s.works / s.segments) * (s.segments - 1);
-    hipLaunchKernelGGL((attention_sweep_kernel<A, T, D, false>), dim3(kf_xcd_grid(two.works)), dim3(4 * D), 0, stream, a, two);
+    hipLaunchKernelGGL((attention_sweep_kernel<A, T, D, MODE, false>), dim3(kf_xcd_grid(two.works)), dim3(4 * D), 0, stream, a, two);
   }
-  hipLaunchKernelGGL((attention_sweep_kernel<A, T, D, true>), dim3(kf_xcd_grid(s.works)), dim3(4 * D), 0, stream, a, s);
-  KF_HIP_CHECK(h, hipFuncSetAttribute(reinterpret_cast<const void*>(attention_gradient_kernel<A, T, D>),
+  hipLaunchKernelGGL((attention_sweep_kernel<A, T, D, MODE, true>), dim3(kf_xcd_grid(s.works)), dim3(4 * D), 0, stream, a, s);
+  KF_HIP_CHECK(h, hipFuncSetAttribute(reinterpret_cast<const void*>(attention_gradient_kernel<A, T, D, MODE>),
                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  hipLaunchKernelGGL((attention_gradient_kernel<A, T, D>), dim3(kf_xcd_grid(s.works)), dim3(4 * D), lds, stream, a, s);
+  hipLaunchKernelGGL((attention_gradient_kernel<A, T, D, MODE>), dim3(kf_xcd_grid(s.works)), dim3(4 * D), lds, stream, a, s);
   if (a.G != a.H) {
     const long total = a.B * a.T * a.G * a.K;
     hipLaunchKernelGGL(attention_group_kernel<T>, dim3((unsigned)((total + 255) / 256), 2), dim3(256), 0, stream, a, s.part_q, s.part_k);
@@ -541,13 +545,20 @@ int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream)
   return KF_OK;
 }
 
+template <typename A, typename T, int MODE>
+int launch_m(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream) {
+  switch (p.D) {
+    case 32: return launch<A, T, 32, MODE>(h, a, p, stream);
+    case 64: return launch<A, T, 64, MODE>(h, a, p, stream);
+    default: return launch<A, T, 128, MODE>(h, a, p, stream);
+  }
+}
+
 template <typename A, typename T>
 int launch_d(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream) {
-  switch (p.D) {
-    case 32: return launch<A, T, 32>(h, a, p, stream);
-    case 64: return launch<A, T, 64>(h, a, p, stream);
-    default: return launch<A, T, 128>(h, a, p, stream);
-  }
+  if (p.mode == KF_ROWS_NARROW) return launch<A, T, 128, KF_ROWS_NARROW>(h, a, p, stream);
+  if (p.mode == KF_ROWS_CUT) return launch_m<A, T, KF_ROWS_CUT>(h, a, p, stream);
+  return launch_m<A, T, KF_ROWS_WHOLE>(h, a, p, stream);
 }
 
 }  // namespace
@@ -557,11 +568,6 @@ size_t kf_attention_backward_workspace(const kf_handle* h, const KfAttnArgs& a) 
 int kf_launch_attention_backward(kf_handle* h, const KfAttnArgs& a, void* ws, hipStream_t stream) {
   Plan p = plan(h, a);
   Split& s = p.sp;
-  const int e = a.dtype == KF_DTYPE_F32 ? 4 : 2;
-  s.vec_q = kf_rows_aligned(a.q, a.qs, 3, a.K, e);
-  s.vec_k = kf_rows_aligned(a.k, a.ks, 3, a.K, e);
-  s.vec_v = kf_rows_aligned(a.v, a.vs, 3, a.V, e);
-  s.vec_g = kf_rows_aligned(a.g_o, a.gs, 3, a.V, e);
   char* w = (char*)ws;
   s.adds_s = (float*)w; w += p.adds;
   s.adds_r = (float*)w; w += p.adds;

@@ -4,6 +4,15 @@
 
 constexpr int KF_CHUNK = 64;
 
+template <int N> static __device__ __forceinline__ double kf_row_shr(double x) {  // from N lanes below in the row of 16, 0 from outside
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(x), 0x110 + N, 0xf, 0xf, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(x), 0x110 + N, 0xf, 0xf, true);
+  return __hiloint2double(hi, lo);
+}
+static __device__ __forceinline__ double kf_readlane(double x, int lane) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), lane), __builtin_amdgcn_readlane(__double2loint(x), lane));
+}
+
 // Decays of one chunk, G_i = sum of the log decays up to and with token i (summed in 64 bits; each exponent is rounded once).
 // No exponent is positive: pairs (i, j) in different 16-token tiles take exp(G_i - G_j) as the product of two factors <= 1 that meet
 // at the end of j's tile, so that only the tiles on the diagonal need an exponential for each pair.
@@ -17,28 +26,41 @@ struct KfChunkDecay {
 
   // by one whole wave, lane l with token l; tokens that are not `live` (lanes from C on are not) neither decay nor write
   __device__ __forceinline__ void fill(float log_decay, bool live) {
-    const int l = threadIdx.x & 63;
+    const int l = threadIdx.x & 63, row = l >> 4;
     double G = live ? (double)kf_clamp_log_decay(log_decay) : 0.0;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const double x = __shfl_up(G, d);
-      if (l >= d) G += x;
-    }
-    const double end = __shfl(G, 63), tile_end = __shfl(G, l | 15);
-    float d[C / 16 - 1];
-#pragma unroll
-    for (int t = 0; t < C / 16 - 1; ++t) d[t] = (float)(G - __shfl(G, 16 * t + 15));
+    // running sums inside each row of 16 lanes, then over the rows
+    G += kf_row_shr<1>(G);
+    G += kf_row_shr<2>(G);
+    G += kf_row_shr<4>(G);
+    G += kf_row_shr<8>(G);
+    double end[4];  // G at the end of each tile
+    end[0] = kf_readlane(G, 15);
+    end[1] = end[0] + kf_readlane(G, 31);
+    end[2] = end[1] + kf_readlane(G, 47);
+    end[3] = end[2] + kf_readlane(G, 63);
+    G += row == 0 ? 0.0 : row == 1 ? end[0] : row == 2 ? end[1] : end[2];
     if (l < C) {
-      from_start[l] = expf((float)G);
-      to_end[l] = expf((float)(end - G));
-      to_tile_end[l] = expf((float)(tile_end - G));
+      from_start[l] = __expf((float)G);
+      to_end[l] = __expf((float)(end[C / 16 - 1] - G));
+      to_tile_end[l] = __expf((float)((row == 0 ? end[0] : row == 1 ? end[1] : row == 2 ? end[2] : end[3]) - G));
 #pragma unroll
-      for (int t = 0; t < C / 16 - 1; ++t) from_tile[t][l] = expf(d[t] > 0.f ? 0.f : d[t]);  // (a NaN stays one)
+      for (int t = 0; t < C / 16 - 1; ++t) {
+        const float d = (float)(G - end[t]);
+        from_tile[t][l] = __expf(d > 0.f ? 0.f : d);  // (a NaN stays one)
+      }
       hi[l] = (float)G;
       lo[l] = (float)(G - (double)hi[l]);
     }
   }
-  __device__ __forceinline__ float pair(int i, int j) const { return __expf((hi[i] - hi[j]) + (lo[i] - lo[j])); }
+  // exp(G_i - G_j) for j .. j + 3 (of the same tile; where j is behind i the value means nothing, and may be infinite)
+  __device__ __forceinline__ kf_f32x4 pairs(int i, int j) const {
+    const float h = hi[i], s = lo[i];
+    const kf_f32x4 hj = *reinterpret_cast<const kf_f32x4*>(&hi[j]), sj = *reinterpret_cast<const kf_f32x4*>(&lo[j]);
+    kf_f32x4 e;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) e[r] = __expf((h - hj[r]) + (s - sj[r]));
+    return e;
+  }
 };
 
 struct KfAttnSplit {
@@ -46,7 +68,6 @@ struct KfAttnSplit {
   int segments;    // of the time axis
   int seg_chunks;  // chunks of each
   int v_tiles;
-  int vec_q, vec_k, vec_v, vec_g;  // rows may be read 16 bytes at a time
 };
 
 // Workgroup -> work, neighbours (the tiles of V and the heads that read the same q and k) on the same one of the 8 dies, whose
@@ -56,11 +77,3 @@ static __device__ __forceinline__ long kf_xcd_work(long works) {
   return (blockIdx.x & 7) * per + (blockIdx.x >> 3);
 }
 static inline unsigned kf_xcd_grid(long works) { return (unsigned)(8 * ((works + 7) >> 3)); }
-
-// A fragment of A stays aligned: base and every stride a multiple of 16 bytes.
-static inline int kf_rows_aligned(const void* p, const long* strides, int n, int dim, int elem) {
-  if (((uintptr_t)p & 15) || dim % 8) return 0;
-  for (int i = 0; i < n; ++i)
-    if ((strides[i] * elem) % 16) return 0;
-  return 1;
-}

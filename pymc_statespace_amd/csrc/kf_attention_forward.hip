@@ -8,15 +8,20 @@
 
 namespace {
 
-// A: arithmetic (KfBf16, KfF32).  T: type of q, k, v, o.  KP, VT: K and this workgroup's columns of V, padded.
+// A: arithmetic (KfBf16, KfF32).  T: type of q, k, v, o.  KP, VT: K and this workgroup's columns of V, padded.  MODE: KF_ROWS_*.
 // OUT false: only what the segment adds to the state.
-template <typename A, typename T, int KP, int VT, bool OUT>
+//
+// What a chunk needs from memory is asked for one chunk ahead, by loads that no branch surrounds (a load that may or may not have been
+// issued makes every later wait one for all of them): at a segment's end they ask for the last chunk again.
+template <typename A, typename T, int KP, int VT, int MODE, bool OUT>
 __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, KfAttnSplit sp, float* adds, float* factors) {
   typedef typename A::elem E;
   typedef typename A::frag F;
+  typedef KfRow<A, T, MODE> Row;
   constexpr int LK = KP + A::PAD, LV = VT + A::PAD, NT = VT / 16, KK = KP / 32;
   constexpr int WK = KP / 16 < 4 ? KP / 16 : 4, WN = 4 / WK;  // the state's tiles: WK waves along K, WN along V
   constexpr int SM = KP / 16 / WK, SN = NT / WN;
+  constexpr int RK = 2048 / KP, RV = 2048 / VT;
   __shared__ __attribute__((aligned(16))) E sK[KF_CHUNK * LK];
   __shared__ __attribute__((aligned(16))) E sV[KF_CHUNK * LV];
   __shared__ __attribute__((aligned(16))) E sS[OUT ? VT * LK : 8];  // the state's transpose as an operand
@@ -32,17 +37,19 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
   const int seg = (int)(rest % segs);
   const long b = rest / segs;
   const long bh = b * a.H + h;
-  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, i = l & 15, g = l >> 4;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i = l & 15, g = l >> 4;
   const int mt0 = (w % WK) * SM, nt0 = (w / WK) * SN;
   const int v0 = vt * VT, nv = a.V - v0;
   const long n = kf_row_length(a.lengths, b, a.T);
   const int grp = h / (a.H / a.G);
   const T* q = (const T*)a.q + b * a.qs[0] + grp * a.qs[2];
   const T* k = (const T*)a.k + b * a.ks[0] + grp * a.ks[2];
-  const T* v = (const T*)a.v + b * a.vs[0] + h * a.vs[2] + v0;
+  const T* v = (const T*)a.v + b * a.vs[0] + h * a.vs[2];
   const float* ld = a.log_decay + (a.per_token ? b * a.T * a.H + h : (long)h);
+  const long ld_step = a.per_token ? a.H : 0;
   const long chunks = (a.T + KF_CHUNK - 1) / KF_CHUNK;
   const long c0 = (long)seg * sp.seg_chunks, c1 = c0 + sp.seg_chunks < chunks ? c0 + sp.seg_chunks : chunks;
+  const long live = (n + KF_CHUNK - 1) / KF_CHUNK, end = c1 < live ? c1 : live;  // chunks with tokens: c0 .. end - 1
 
   kf_f32x4 S[SM][SN];
 #pragma unroll
@@ -71,146 +78,150 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
         for (int t = 0; t < SN; ++t) S[m][t] = S[m][t] * f + u[(m * SN + t) * 256];
     }
   }
-  bool have = OUT && (a.s0 || seg);  // the state may not be zero
   float through = 1.f;
 
-  F rk[KK], rv[VT / 32], rq[KK];
-  float rg = 0.f;
+  typename Row::Raw rk[KK], rv[VT / 32], rq[KK];  // the next chunk's, as loaded
+  float rg = 0.f;                                  // and the log decay of one token of the chunk behind it
+  // this lane's part of a chunk: rows kr + u RK of k, vr + u RV of v, row 16 w + i of q
+  const int kr = tid / (KP / 8), kc = 8 * (tid % (KP / 8)), vr = tid / (VT / 8), vc = 8 * (tid % (VT / 8));
+  auto last_row = [&](long c) { return (int)(n - c * KF_CHUNK < KF_CHUNK ? n - c * KF_CHUNK : KF_CHUNK) - 1; };
+  auto at_row = [](const T* base, long stride, int r, int last) { return base + (r < last ? r : last) * stride; };
   auto load = [&](long c) {
-    const long t0 = c * KF_CHUNK;
+    const int last = last_row(c);
+    const T *pk = k + c * KF_CHUNK * a.ks[1], *pv = v + c * KF_CHUNK * a.vs[1];
 #pragma unroll
-    for (int u = 0; u < KK; ++u) {
-      const int x = tid + 256 * u, row = x / (KP / 8), col = 8 * (x % (KP / 8));
-      rk[u] = KfLoad8<A, T>::load(k + (t0 + row) * a.ks[1] + col, t0 + row < n ? a.K - col : 0, sp.vec_k);
-    }
+    for (int u = 0; u < KK; ++u) rk[u] = Row::raw(at_row(pk, a.ks[1], kr + u * RK, last), kc, a.K);
 #pragma unroll
-    for (int u = 0; u < VT / 32; ++u) {
-      const int x = tid + 256 * u, row = x / (VT / 8), col = 8 * (x % (VT / 8));
-      rv[u] = KfLoad8<A, T>::load(v + (t0 + row) * a.vs[1] + col, t0 + row < n ? nv - col : 0, sp.vec_v);
-    }
-    if (OUT) {
-      const long t = t0 + 16 * w + i;
-#pragma unroll
-      for (int u = 0; u < KK; ++u) rq[u] = KfLoad8<A, T>::load(q + t * a.qs[1] + 32 * u + 8 * g, t < n ? a.K - 32 * u - 8 * g : 0, sp.vec_q);
-    }
+    for (int u = 0; u < VT / 32; ++u) rv[u] = Row::raw(at_row(pv, a.vs[1], vr + u * RV, last), v0 + vc, a.V);
   };
-  auto load_decay = [&](long c) { return c * KF_CHUNK + l < n ? (a.per_token ? ld[(c * KF_CHUNK + l) * a.H] : ld[0]) : 0.f; };
-
-  if (c0 * KF_CHUNK < n) {
-    load(c0);
-    if (w == (int)(c0 & 3)) dec[c0 & 1].fill(load_decay(c0), c0 * KF_CHUNK + l < n);
-  }
-  if (OUT && have) {
+  auto load_q = [&](long c) {
+    const T* pq = at_row(q + c * KF_CHUNK * a.qs[1], a.qs[1], 16 * w + i, last_row(c));
+#pragma unroll
+    for (int u = 0; u < KK; ++u) rq[u] = Row::raw(pq, 32 * u + 8 * g, a.K);
+  };
+  auto log_decay = [&](long c) { return ld[(c * KF_CHUNK + l < n ? c * KF_CHUNK + l : n - 1) * ld_step]; };
+  auto put_state = [&]() {
 #pragma unroll
     for (int m = 0; m < SM; ++m)
 #pragma unroll
       for (int t = 0; t < SN; ++t) A::put4(sS + ((nt0 + t) * 16 + i) * LK + (mt0 + m) * 16 + 4 * g, S[m][t]);
+  };
+
+  if (c0 < end) {
+    const float g0 = log_decay(c0);
+    rg = log_decay(c0 + 1);
+    load(c0);
+    if (OUT) load_q(c0);
+    if (w == 0) dec[c0 & 1].fill(g0, c0 * KF_CHUNK + l < n);
+    if (OUT) put_state();
   }
-  long c = c0;
-  for (; c < c1 && c * KF_CHUNK < n; ++c) {
-    const long t0 = c * KF_CHUNK;
+  for (long c = c0; c < end; ++c) {
+    const long t0 = c * KF_CHUNK, next = c + 1 < end ? c + 1 : c;
+    const int last = last_row(c);  // rows behind it are zero
 #pragma unroll
-    for (int u = 0; u < KK; ++u) {
-      const int x = tid + 256 * u;
-      A::put8(sK + (x / (KP / 8)) * LK + 8 * (x % (KP / 8)), rk[u]);
-    }
+    for (int u = 0; u < KK; ++u) A::put8(sK + (kr + u * RK) * LK + kc, Row::finish(rk[u], kc, a.K, kr + u * RK <= last));
 #pragma unroll
-    for (int u = 0; u < VT / 32; ++u) {
-      const int x = tid + 256 * u;
-      A::put8(sV + (x / (VT / 8)) * LV + 8 * (x % (VT / 8)), rv[u]);
-    }
-    F fq[KK];
-#pragma unroll
-    for (int u = 0; u < KK; ++u) fq[u] = rq[u];
+    for (int u = 0; u < VT / 32; ++u) A::put8(sV + (vr + u * RV) * LV + vc, Row::finish(rv[u], v0 + vc, a.V, vr + u * RV <= last));
     __syncthreads();
-    const bool more = c + 1 < c1 && (c + 1) * KF_CHUNK < n;
-    if (more) {
-      load(c + 1);
-      if (w == (int)((c + 1) & 3)) rg = load_decay(c + 1);
-    }
+    const float g1 = rg;
+    rg = log_decay(c + 2);
+    load(next);
+    if (w == (int)(c & 3)) dec[(c + 1) & 1].fill(g1, (c + 1) * KF_CHUNK + l < n);
     const KfChunkDecay<KF_CHUNK>& D = dec[c & 1];
 
     if (OUT) {
       const int row = 16 * w + i;
-      // scores, transposed: rows j, columns i
-      kf_f32x4 p[4];
+      F fq[KK];
 #pragma unroll
-      for (int jt = 0; jt < 4; ++jt) {
-        p[jt] = kf_f32x4{0, 0, 0, 0};
-        if (jt <= w) {
+      for (int u = 0; u < KK; ++u) fq[u] = Row::finish(rq[u], 32 * u + 8 * g, a.K, row <= last);
+      // scores, transposed: rows j, columns i; as operands, two tiles each.  (w is the same for a whole wave.)
+      F p[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        kf_f32x4 two[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int jt = 2 * x + y;
           kf_f32x4 s = {0, 0, 0, 0};
+          if (jt <= w) {
 #pragma unroll
-          for (int u = 0; u < KK; ++u) s = A::mma(A::row(sK + (16 * jt + i) * LK + 32 * u + 8 * g), fq[u], s);
-          if (jt < w) {
-            const float f = D.from_tile[jt < 3 ? jt : 2][row] * a.scale;
-            const kf_f32x4 e = *reinterpret_cast<const kf_f32x4*>(&D.to_tile_end[16 * jt + 4 * g]);
+            for (int u = 0; u < KK; ++u) s = A::mma(A::row(sK + (16 * jt + i) * LK + 32 * u + 8 * g), fq[u], s);
+            if (jt < w) {
+              s *= D.from_tile[jt < 3 ? jt : 2][row] * a.scale;
+              s *= *reinterpret_cast<const kf_f32x4*>(&D.to_tile_end[16 * jt + 4 * g]);
+            } else {
+              s *= D.pairs(row, 16 * jt + 4 * g) * a.scale;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) p[jt][r] = s[r] * (f * e[r]);
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) p[jt][r] = 4 * g + r <= i ? s[r] * (D.pair(row, 16 * jt + 4 * g + r) * a.scale) : 0.f;
+              for (int r = 0; r < 4; ++r) s[r] = 4 * g + r <= i ? s[r] : 0.f;
+            }
           }
+          two[y] = s;
         }
+        p[x] = A::from(two[0], two[1]);
       }
       const float fs = D.from_start[row] * a.scale;
-      auto from_state = [&](int t) {
+      const long t = t0 + row;
+      T* out = (T*)a.o + ((b * a.T + t) * a.H + h) * (long)a.V + v0;
+      // columns 16 u .. 16 u + 31 of V as two tiles, of which a lane has 8 neighbours: 16 u + 8 g .. + 7
+      auto from_state = [&](int v1) {
         kf_f32x4 o = {0, 0, 0, 0};
-        if (have) {
 #pragma unroll
-          for (int u = 0; u < KK; ++u) o = A::mma(A::row(sS + (16 * t + i) * LK + 32 * u + 8 * g), fq[u], o);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[r] *= fs;
-        }
-        return o;
+        for (int x = 0; x < KK; ++x) o = A::mma(A::row(sS + (v1 + 8 * (i >> 2) + (i & 3)) * LK + 32 * x + 8 * g), fq[x], o);
+        return o * fs;
       };
-      kf_f32x4 o[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) o[t] = from_state(t);
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-        if (2 * x <= w) {
-          const F fp = A::from(p[2 * x], p[2 * x + 1]);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) o[t] = A::mma(A::col(sV + 32 * x * LV + 16 * t, LV, i, g), fp, o[t]);
-        }
-      // A token's infinity or NaN in v would reach the rows before it as 0 x inf.  Where anything is not finite, the products are
-      // taken again without such values, and these added only to the rows from their token on.
+      KfOut8<T> ready[NT / 2];
       float check = 0.f;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int u = 0; u < NT; u += 2) {
+        kf_f32x4 o[2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) check = fmaf(o[t][r], 0.f, check);
-      if (__any(check != 0.f)) {
+        for (int y = 0; y < 2; ++y) {
+          o[y] = from_state(16 * u + 4 * y);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          o[t] = from_state(t);
+          for (int x = 0; x < 2; ++x) o[y] = A::mma(A::col8(sV + 32 * x * LV + 16 * u + 4 * y, LV, i, g), p[x], o[y]);
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            if (2 * x <= w) o[t] = A::mma(A::finite(A::col(sV + 32 * x * LV + 16 * t, LV, i, g)), A::from(p[2 * x], p[2 * x + 1]), o[t]);
+          for (int r = 0; r < 4; ++r) check = fmaf(o[y][r], 0.f, check);
 #pragma unroll
-          for (int jt = 0; jt < 4; ++jt)
-            if (jt <= w)
+          for (int r = 0; r < 4; ++r) o[y][r] = t < n ? o[y][r] : 0.f;
+        }
+        ready[u / 2].set(o[0], o[1]);
+      }
+      const bool strange = __any(check != 0.f);  // something is not finite
+      if (strange) {
+        // A token's infinity or NaN in v would reach the rows before it as 0 x inf: the products once more without such values, and
+        // these added only to the rows from their token on.
 #pragma unroll 1
-              for (int j = 0; j < 16; ++j) {
-                const float pj = __shfl((j & 3) == 0 ? p[jt][0] : (j & 3) == 1 ? p[jt][1] : (j & 3) == 2 ? p[jt][2] : p[jt][3], (j >> 2) * 16 + i);
-                if (16 * jt + j <= row)
+        for (int v1 = 0; v1 < VT; v1 += v1 & 4 ? 28 : 4) {
+          kf_f32x4 o = from_state(v1);
 #pragma unroll
-                  for (int r = 0; r < 4; ++r) {
-                    const float x = A::get(sV + (16 * jt + j) * LV + 16 * t + 4 * g + r);
-                    if (!(fabsf(x) <= 3.4e38f)) o[t][r] += pj * x;
-                  }
-              }
+          for (int x = 0; x < 2; ++x) {
+            o = A::mma(A::finite(A::col8(sV + 32 * x * LV + v1, LV, i, g)), p[x], o);
+#pragma unroll 1
+            for (int j = 0; j < 32; ++j) {  // token 32 x + j: value e = 4 (j / 16) + j % 4 of lane group (j % 16) / 4
+              float pj = 0.f;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) pj = e == 4 * (j >> 4) + (j & 3) ? A::value(p[x], e) : pj;
+              pj = __shfl(pj, ((j & 15) >> 2) * 16 + i);
+              if (32 * x + j <= row)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const float z = A::get(sV + (32 * x + j) * LV + v1 + 8 * g + r);
+                  if (!(fabsf(z) <= 3.4e38f)) o[r] += pj * z;
+                }
+            }
+          }
+          if (t < n) kf_store4(out + v1 + 8 * g, o, nv - v1 - 8 * g);
         }
       }
-      const long t = t0 + row;
-      if (t < a.T) {
-        T* out = (T*)a.o + ((b * a.T + t) * a.H + h) * (long)a.V + v0;
+      // (loads and stores are waited for in the order they were issued in: the next chunk's loads first)
+      load_q(next);
+      if (t < a.T && (!strange || t >= n)) {
 #pragma unroll
-        for (int u = 0; u < NT; ++u) kf_store4(out + 16 * u + 4 * g, t < n ? o[u] : kf_f32x4{0, 0, 0, 0}, nv - 16 * u - 4 * g, a.V % 4 == 0);
+        for (int u = 0; u < NT; u += 2) ready[u / 2].store(out + 16 * u + 8 * g, nv - 16 * u - 8 * g);
       }
     }
 
-    // the state at the chunk's end (nobody needs the last one of a call that does not ask for it)
+    // the state at the chunk's end
     const float fe = D.from_start[KF_CHUNK - 1];
     through *= fe;
 #pragma unroll
@@ -219,34 +230,26 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
       for (int t = 0; t < SN; ++t) S[m][t] *= fe;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      float wt[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) wt[e] = D.to_end[32 * x + 16 * (e >> 2) + 4 * g + (e & 3)];
+      const kf_f32x4 w0 = *reinterpret_cast<const kf_f32x4*>(&D.to_end[32 * x + 4 * g]), w1 = *reinterpret_cast<const kf_f32x4*>(&D.to_end[32 * x + 16 + 4 * g]);
+      const float wt[8] = {w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]};
       F fv[SN];
 #pragma unroll
       for (int t = 0; t < SN; ++t) fv[t] = A::col(sV + 32 * x * LV + 16 * (nt0 + t), LV, i, g);
 #pragma unroll
       for (int m = 0; m < SM; ++m) {
-        KfWeighted<A> kw;
+        KfSplit<A> kw;
         kw.set(A::col(sK + 32 * x * LK + 16 * (mt0 + m), LK, i, g), wt);
 #pragma unroll
         for (int t = 0; t < SN; ++t) S[m][t] = kw.mma(fv[t], S[m][t]);
       }
     }
-    have = true;
-    if (more && w == (int)((c + 1) & 3)) dec[(c + 1) & 1].fill(rg, (c + 1) * KF_CHUNK + l < n);
     __syncthreads();
-    if (OUT && more) {
-#pragma unroll
-      for (int m = 0; m < SM; ++m)
-#pragma unroll
-        for (int t = 0; t < SN; ++t) A::put4(sS + ((nt0 + t) * 16 + i) * LK + (mt0 + m) * 16 + 4 * g, S[m][t]);
-    }
+    if (OUT) put_state();
   }
   if (OUT) {
     // rows behind the sequence's end, in chunks that hold none of it
     const int cols = nv < VT ? nv : VT;
-    for (long x = c * KF_CHUNK + tid / VT; x < c1 * KF_CHUNK && x < a.T; x += 256 / VT)
+    for (long x = (end > c0 ? end : c0) * KF_CHUNK + tid / VT; x < c1 * KF_CHUNK && x < a.T; x += 256 / VT)
       if (tid % VT < cols) ((T*)a.o)[((b * a.T + x) * a.H + h) * (long)a.V + v0 + tid % VT] = kf_from_float<T>(0.f);
     if (a.sT && seg == sp.segments - 1) {
 #pragma unroll
@@ -271,14 +274,17 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
 
 struct Plan {
   int KP, VT;
+  int mode;
   KfAttnSplit sp;
   size_t adds, bytes;
 };
 
 Plan plan(const kf_handle* h, const KfAttnArgs& a) {
   Plan p;
-  p.KP = a.K <= 32 ? 32 : a.K <= 64 ? 64 : 128;
-  p.VT = a.dtype == KF_DTYPE_BF16 && a.V > 32 ? 64 : 32;
+  p.mode = kf_rows_mode(a.K, a.V);
+  const bool narrow = p.mode == KF_ROWS_NARROW;  // one kernel, of the largest K
+  p.KP = narrow ? 128 : a.K <= 32 ? 32 : a.K <= 64 ? 64 : 128;
+  p.VT = a.dtype == KF_DTYPE_BF16 && a.V > 32 && !narrow ? 64 : 32;
   KfAttnSplit& s = p.sp;
   s.v_tiles = (a.V + p.VT - 1) / p.VT;
   const long chunks = (a.T + KF_CHUNK - 1) / KF_CHUNK, rows = a.B * a.H * s.v_tiles;
@@ -296,27 +302,35 @@ Plan plan(const kf_handle* h, const KfAttnArgs& a) {
   return p;
 }
 
-template <typename A, typename T, int KP, int VT>
+template <typename A, typename T, int KP, int VT, int MODE>
 int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, void* ws, hipStream_t stream) {
   float* adds = (float*)ws;
   float* factors = (float*)((char*)ws + p.adds);
   if (p.sp.segments > 1) {
     KfAttnSplit s = p.sp;
     s.works = p.sp.works / p.sp.segments * (p.sp.segments - 1);
-    hipLaunchKernelGGL((attention_chunk_kernel<A, T, KP, VT, false>), dim3(kf_xcd_grid(s.works)), dim3(256), 0, stream, a, s, adds, factors);
+    hipLaunchKernelGGL((attention_chunk_kernel<A, T, KP, VT, MODE, false>), dim3(kf_xcd_grid(s.works)), dim3(256), 0, stream, a, s, adds, factors);
   }
-  hipLaunchKernelGGL((attention_chunk_kernel<A, T, KP, VT, true>), dim3(kf_xcd_grid(p.sp.works)), dim3(256), 0, stream, a, p.sp, adds, factors);
+  hipLaunchKernelGGL((attention_chunk_kernel<A, T, KP, VT, MODE, true>), dim3(kf_xcd_grid(p.sp.works)), dim3(256), 0, stream, a, p.sp, adds, factors);
   KF_HIP_CHECK(h, hipGetLastError());
   return KF_OK;
 }
 
-template <typename A, typename T, int VT>
+template <typename A, typename T, int VT, int MODE>
 int launch_k(kf_handle* h, const KfAttnArgs& a, const Plan& p, void* ws, hipStream_t stream) {
   switch (p.KP) {
-    case 32: return launch<A, T, 32, VT>(h, a, p, ws, stream);
-    case 64: return launch<A, T, 64, VT>(h, a, p, ws, stream);
-    default: return launch<A, T, 128, VT>(h, a, p, ws, stream);
+    case 32: return launch<A, T, 32, VT, MODE>(h, a, p, ws, stream);
+    case 64: return launch<A, T, 64, VT, MODE>(h, a, p, ws, stream);
+    default: return launch<A, T, 128, VT, MODE>(h, a, p, ws, stream);
   }
+}
+
+template <typename A, typename T>
+int launch_t(kf_handle* h, const KfAttnArgs& a, const Plan& p, void* ws, hipStream_t stream) {
+  if (p.mode == KF_ROWS_NARROW) return launch<A, T, 128, 32, KF_ROWS_NARROW>(h, a, p, ws, stream);
+  if constexpr (std::is_same<A, KfBf16>::value)
+    if (p.VT == 64) return p.mode == KF_ROWS_CUT ? launch_k<A, T, 64, KF_ROWS_CUT>(h, a, p, ws, stream) : launch_k<A, T, 64, KF_ROWS_WHOLE>(h, a, p, ws, stream);
+  return p.mode == KF_ROWS_CUT ? launch_k<A, T, 32, KF_ROWS_CUT>(h, a, p, ws, stream) : launch_k<A, T, 32, KF_ROWS_WHOLE>(h, a, p, ws, stream);
 }
 
 }  // namespace
@@ -327,14 +341,10 @@ size_t kf_attention_forward_workspace(const kf_handle* h, const KfAttnArgs& a) {
 }
 
 int kf_launch_attention(kf_handle* h, const KfAttnArgs& a, void* ws, hipStream_t stream) {
-  Plan p = plan(h, a);
-  const int e = a.dtype == KF_DTYPE_F32 ? 4 : 2;
-  p.sp.vec_q = kf_rows_aligned(a.q, a.qs, 3, a.K, e);
-  p.sp.vec_k = kf_rows_aligned(a.k, a.ks, 3, a.K, e);
-  p.sp.vec_v = kf_rows_aligned(a.v, a.vs, 3, a.V, e);
+  const Plan p = plan(h, a);
   switch (a.dtype) {
-    case KF_DTYPE_F32: return launch_k<KfF32, float, 32>(h, a, p, ws, stream);
-    case KF_DTYPE_F16: return launch_k<KfF32, __half, 32>(h, a, p, ws, stream);
-    default: return p.VT == 64 ? launch_k<KfBf16, __hip_bfloat16, 64>(h, a, p, ws, stream) : launch_k<KfBf16, __hip_bfloat16, 32>(h, a, p, ws, stream);
+    case KF_DTYPE_F32: return launch_t<KfF32, float>(h, a, p, ws, stream);
+    case KF_DTYPE_F16: return launch_t<KfF32, __half>(h, a, p, ws, stream);
+    default: return launch_t<KfBf16, __hip_bfloat16>(h, a, p, ws, stream);
   }
 }

@@ -48,6 +48,13 @@ struct KfBf16 {
     const kf_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)a), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(a + 16 * ld));
     return __builtin_bit_cast(frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   }
+  // columns 8 (i / 4) + i % 4 of it: with the ones 4 further on in a second fragment, a lane ends up with 8 neighbours
+  static __device__ __forceinline__ frag col8(const elem* p, int ld, int i, int g) {
+    const elem* a = p + (4 * g + (i >> 2)) * ld + 8 * (i & 3);
+    typedef __attribute__((address_space(3))) kf_s16x4* lds;
+    const kf_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)a), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(a + 16 * ld));
+    return __builtin_bit_cast(frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
   static __device__ __forceinline__ frag from(kf_f32x4 x, kf_f32x4 y) {
     return __builtin_bit_cast(frag, kf_u32x4{kf_pack_bf16(x[0], x[1]), kf_pack_bf16(x[2], x[3]), kf_pack_bf16(y[0], y[1]), kf_pack_bf16(y[2], y[3])});
   }
@@ -97,6 +104,12 @@ struct KfF32 {
     for (int e = 0; e < 8; ++e) f[e] = p[(16 * (e >> 2) + 4 * g + (e & 3)) * ld + i];
     return f;
   }
+  static __device__ __forceinline__ frag col8(const elem* p, int ld, int i, int g) {
+    frag f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = p[(16 * (e >> 2) + 4 * g + (e & 3)) * ld + 8 * (i >> 2) + (i & 3)];
+    return f;
+  }
   static __device__ __forceinline__ frag from(kf_f32x4 x, kf_f32x4 y) { return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7); }
   static __device__ __forceinline__ float value(frag a, int e) { return a[e]; }
   static __device__ __forceinline__ frag finite(frag a) {
@@ -113,54 +126,20 @@ struct KfF32 {
   static __device__ __forceinline__ kf_f32x4 get4(const elem* p) { return *reinterpret_cast<const kf_f32x4*>(p); }
 };
 
-// An operand times a weight for each depth, exact to 24 bits: in fp32 the product itself; in bf16 the fp32 product is cut into three
-// parts of 8 bits each (cut, not rounded: the rest is exact and keeps the sign) and takes three matrix products.
-template <typename A> struct KfWeighted;
-template <> struct KfWeighted<KfF32> {
+// fp32 numbers as one operand (accumulators of two 16 x 16 tiles, or a fragment times a weight for each depth): fp32 as they are;
+// bf16 in two rounded parts, 2 x 8 bits and a sign (at most 2^-18 of each value is lost, 7e-7 on average; one part alone would lose
+// 2^-9, far more than the 32 bits that states and their sums are held in), two products.
+template <typename A> struct KfSplit;
+template <> struct KfSplit<KfF32> {
+  static constexpr int PARTS = 2;  // 16-byte pieces
   kf_f32x8 p;
+  __device__ __forceinline__ void set(kf_f32x4 x, kf_f32x4 y) { p = KfF32::from(x, y); }
   __device__ __forceinline__ void set(kf_f32x8 a, const float (&w)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) p[e] = a[e] * w[e];
   }
   __device__ __forceinline__ kf_f32x4 mma(kf_f32x8 b, kf_f32x4 c) const { return KfF32::mma(p, b, c); }
   __device__ __forceinline__ kf_f32x4 mma_right(kf_f32x8 a, kf_f32x4 c) const { return KfF32::mma(a, p, c); }
-};
-template <> struct KfWeighted<KfBf16> {
-  kf_bf16x8 p0, p1, p2;
-  __device__ __forceinline__ void set(kf_bf16x8 a, const float (&w)[8]) {
-    unsigned x0[8], x1[8], x2[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = KfBf16::value(a, e) * w[e];
-      x0[e] = kf_bits(x);
-      const float r = x - kf_float_of(x0[e] & 0xffff0000u);
-      x1[e] = kf_bits(r);
-      x2[e] = kf_bits(r - kf_float_of(x1[e] & 0xffff0000u));
-    }
-    p0 = pack(x0); p1 = pack(x1); p2 = pack(x2);
-  }
-  static __device__ __forceinline__ kf_bf16x8 pack(const unsigned (&x)[8]) {  // the high halves
-    kf_u32x4 r;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x07060302u);
-    return __builtin_bit_cast(kf_bf16x8, r);
-  }
-  __device__ __forceinline__ kf_f32x4 mma(kf_bf16x8 b, kf_f32x4 c) const {
-    return KfBf16::mma(p0, b, KfBf16::mma(p1, b, KfBf16::mma(p2, b, c)));
-  }
-  __device__ __forceinline__ kf_f32x4 mma_right(kf_bf16x8 a, kf_f32x4 c) const {
-    return KfBf16::mma(a, p0, KfBf16::mma(a, p1, KfBf16::mma(a, p2, c)));
-  }
-};
-
-// Accumulators of two 16 x 16 tiles as one operand: fp32 as they are; bf16 in two rounded parts, 2 x 8 bits and a sign each
-// (2^-18 of each value is lost), two products.
-template <typename A> struct KfSplit;
-template <> struct KfSplit<KfF32> {
-  static constexpr int PARTS = 2;  // 16-byte pieces
-  kf_f32x8 p;
-  __device__ __forceinline__ void set(kf_f32x4 x, kf_f32x4 y) { p = KfF32::from(x, y); }
-  __device__ __forceinline__ kf_f32x4 mma(kf_f32x8 b, kf_f32x4 c) const { return KfF32::mma(p, b, c); }
   __device__ __forceinline__ float value(int e) const { return p[e]; }
   __device__ __forceinline__ kf_u32x4 piece(int k) const {
     return k ? __builtin_bit_cast(kf_u32x4, __builtin_shufflevector(p, p, 4, 5, 6, 7)) : __builtin_bit_cast(kf_u32x4, __builtin_shufflevector(p, p, 0, 1, 2, 3));
@@ -180,55 +159,143 @@ template <> struct KfSplit<KfBf16> {
     }
     lo = KfBf16::from(u, v);
   }
+  __device__ __forceinline__ void set(kf_bf16x8 a, const float (&w)[8]) {
+    kf_f32x4 x, y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = KfBf16::value(a, e) * w[e];
+      y[e] = KfBf16::value(a, 4 + e) * w[4 + e];
+    }
+    set(x, y);
+  }
   __device__ __forceinline__ kf_f32x4 mma(kf_bf16x8 b, kf_f32x4 c) const { return KfBf16::mma(hi, b, KfBf16::mma(lo, b, c)); }
+  __device__ __forceinline__ kf_f32x4 mma_right(kf_bf16x8 a, kf_f32x4 c) const { return KfBf16::mma(a, hi, KfBf16::mma(a, lo, c)); }
   __device__ __forceinline__ float value(int e) const { return KfBf16::value(hi, e) + KfBf16::value(lo, e); }
   __device__ __forceinline__ kf_u32x4 piece(int k) const { return __builtin_bit_cast(kf_u32x4, k ? lo : hi); }
   __device__ __forceinline__ void pieces(kf_u32x4 x, kf_u32x4 y) { hi = __builtin_bit_cast(kf_bf16x8, x); lo = __builtin_bit_cast(kf_bf16x8, y); }
 };
 
-// Eight consecutive elements of a global row as the arithmetic's own (the first `n` of them; n <= 0: none), zeros behind them.
-// vec: the address is 16-byte aligned whenever n >= 8 (decided once for a tensor, on the host).
-template <typename A, typename T> struct KfLoad8;
-template <> struct KfLoad8<KfBf16, __hip_bfloat16> {
-  static __device__ __forceinline__ kf_bf16x8 load(const __hip_bfloat16* p, int n, bool vec) {
-    if (vec && n >= 8) return *reinterpret_cast<const kf_bf16x8*>(p);
-    kf_s16x8 r;
+// 16 bytes at any element's address (global accesses need no alignment beyond the element's)
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) KfAny16 { kf_u32x4 v; };
+
+// Elements col .. col + 7 of a global row of `dim` elements as the arithmetic's own, zeros from dim on and where !ok (`row` is
+// readable all the same), in two steps: `raw` only loads, so that nothing waits for it until `finish` is called.  No branches:
+//   KF_ROWS_WHOLE   dim % 8 == 0
+//   KF_ROWS_CUT     dim >= 8: the last piece is read from where it still ends inside the row, and moved down by the elements too many
+//                   (a number that is the same for all lanes)
+//   KF_ROWS_NARROW  dim < 8 occurs: element by element
+enum { KF_ROWS_WHOLE, KF_ROWS_CUT, KF_ROWS_NARROW };
+static inline int kf_rows_mode(int K, int V) { return K < 8 || V < 8 ? KF_ROWS_NARROW : K % 8 || V % 8 ? KF_ROWS_CUT : KF_ROWS_WHOLE; }
+static __device__ __forceinline__ kf_u32x4 kf_keep(kf_u32x4 x, bool keep) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = e < n ? reinterpret_cast<const short*>(p)[e] : (short)0;
-    return __builtin_bit_cast(kf_bf16x8, r);
+  for (int e = 0; e < 4; ++e) x[e] = keep ? x[e] : 0u;
+  return x;
+}
+// eight 16-bit elements moved down by s (0 .. 7)
+static __device__ __forceinline__ kf_u32x4 kf_down16(kf_u32x4 x, int s) {
+  const kf_u32x4 a = {s & 4 ? x[2] : x[0], s & 4 ? x[3] : x[1], s & 4 ? 0 : x[2], s & 4 ? 0 : x[3]};
+  const kf_u32x4 b = {s & 2 ? a[1] : a[0], s & 2 ? a[2] : a[1], s & 2 ? a[3] : a[2], s & 2 ? 0 : a[3]};
+  const int h = 16 * (s & 1);
+  return kf_u32x4{__builtin_amdgcn_alignbit(b[1], b[0], h), __builtin_amdgcn_alignbit(b[2], b[1], h), __builtin_amdgcn_alignbit(b[3], b[2], h), b[3] >> h};
+}
+template <int MODE> struct KfRow16 {
+  typedef kf_u32x4 Raw;
+  template <typename T> static __device__ __forceinline__ Raw raw(const T* row, int col, int dim) {
+    if constexpr (MODE == KF_ROWS_NARROW) {
+      kf_s16x8 r;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = col + e < dim ? reinterpret_cast<const short*>(row)[col + e] : (short)0;
+      return __builtin_bit_cast(Raw, r);
+    } else {
+      return reinterpret_cast<const KfAny16<T>*>(row + (col < dim - 8 ? col : dim - 8))->v;
+    }
+  }
+  static __device__ __forceinline__ Raw bits(Raw x, int col, int dim, bool ok) {
+    if constexpr (MODE == KF_ROWS_CUT) x = kf_down16(x, col + 8 > dim && col < dim ? col + 8 - dim : 0);
+    return kf_keep(x, ok && col < dim);
   }
 };
-template <> struct KfLoad8<KfF32, float> {
-  static __device__ __forceinline__ kf_f32x8 load(const float* p, int n, bool vec) {
-    if (vec && n >= 8) return KfF32::row(p);
-    kf_f32x8 r;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = e < n ? p[e] : 0.f;
-    return r;
+template <typename A, typename T, int MODE> struct KfRow;
+template <int MODE> struct KfRow<KfBf16, __hip_bfloat16, MODE> : KfRow16<MODE> {
+  static __device__ __forceinline__ kf_bf16x8 finish(kf_u32x4 x, int col, int dim, bool ok) {
+    return __builtin_bit_cast(kf_bf16x8, KfRow16<MODE>::bits(x, col, dim, ok));
   }
 };
-template <> struct KfLoad8<KfF32, __half> {
-  static __device__ __forceinline__ kf_f32x8 load(const __half* p, int n, bool vec) {
+template <int MODE> struct KfRow<KfF32, __half, MODE> : KfRow16<MODE> {
+  static __device__ __forceinline__ kf_f32x8 finish(kf_u32x4 x, int col, int dim, bool ok) {
     typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-    if (vec && n >= 8) return __builtin_convertvector(*reinterpret_cast<const h8*>(p), kf_f32x8);
-    kf_f32x8 r;
+    return __builtin_convertvector(__builtin_bit_cast(h8, KfRow16<MODE>::bits(x, col, dim, ok)), kf_f32x8);
+  }
+};
+template <int MODE> struct KfRow<KfF32, float, MODE> {
+  typedef kf_f32x8 Raw;
+  static __device__ __forceinline__ Raw raw(const float* row, int col, int dim) {
+    Raw r;
+    if constexpr (MODE == KF_ROWS_NARROW) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = e < n ? (float)reinterpret_cast<const _Float16*>(p)[e] : 0.f;
+      for (int e = 0; e < 8; ++e) r[e] = col + e < dim ? row[col + e] : 0.f;
+    } else {
+      const float* p = row + (col < dim - 8 ? col : dim - 8);
+      r = KfF32::from(__builtin_bit_cast(kf_f32x4, reinterpret_cast<const KfAny16<float>*>(p)->v),
+                      __builtin_bit_cast(kf_f32x4, reinterpret_cast<const KfAny16<float>*>(p + 4)->v));
+    }
     return r;
+  }
+  static __device__ __forceinline__ kf_f32x8 finish(Raw x, int col, int dim, bool ok) {
+    if constexpr (MODE == KF_ROWS_CUT) {
+      const int s = col + 8 > dim && col < dim ? col + 8 - dim : 0;
+      kf_f32x8 y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = s & 4 ? (e < 4 ? x[(e + 4) & 7] : 0.f) : x[e];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = s & 2 ? (e < 6 ? y[(e + 2) & 7] : 0.f) : y[e];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = s & 1 ? (e < 7 ? x[(e + 1) & 7] : 0.f) : x[e];
+      x = y;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = ok && col < dim ? x[e] : 0.f;
+    return x;
   }
 };
 
-// Four consecutive outputs, the first n of them; vec: the address is aligned to four elements.
+// Four consecutive outputs, the first n of them.
 template <typename T>
-static __device__ __forceinline__ void kf_store4(T* p, kf_f32x4 x, int n, bool vec) {
-  if (vec && n >= 4) {
-    struct alignas(4 * sizeof(T)) V4 { T v[4]; } r;
+static __device__ __forceinline__ void kf_store4(T* p, kf_f32x4 x, int n) {
+  if (n >= 4) {
+    typedef unsigned W __attribute__((ext_vector_type(sizeof(T))));
+    struct __attribute__((packed, aligned(sizeof(T)))) Any { W v; };
+    struct { T v[4]; } r;
 #pragma unroll
     for (int e = 0; e < 4; ++e) r.v[e] = kf_from_float<T>(x[e]);
-    *reinterpret_cast<V4*>(p) = r;
+    reinterpret_cast<Any*>(p)->v = __builtin_bit_cast(W, r);
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (e < n) p[e] = kf_from_float<T>(x[e]);
   }
 }
+
+// Eight of them, made ready and stored.
+template <typename T> struct alignas(16) KfOut8 {
+  T v[8];
+  __device__ __forceinline__ void set(kf_f32x4 x, kf_f32x4 y) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = kf_from_float<T>(x[e]);
+      v[4 + e] = kf_from_float<T>(y[e]);
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int n) const {
+    if (n >= 8) {
+      struct Half { kf_u32x4 v[sizeof(T) / 2]; };
+      const Half h = __builtin_bit_cast(Half, *this);
+#pragma unroll
+      for (unsigned e = 0; e < sizeof(T) / 2; ++e) reinterpret_cast<KfAny16<T>*>(p + 8 * e / (sizeof(T) / 2))->v = h.v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < n) p[e] = v[e];
+    }
+  }
+};
