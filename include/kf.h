@@ -492,7 +492,7 @@ enum {
 
 /* Sizes, types and layouts of the kf_linear_attention entry points.  q, k: [B][T][G][K], v: [B][T][H][V]; head h reads the queries
  * and keys of group h / (H / G).  Strides are in elements, for the axes batch, token, head (group) in this order; the last axis is
- * contiguous.  A stride of 0 repeats a row.  1 <= K, V <= 128, H a multiple of G, B H < 2^31. */
+ * contiguous.  A stride of 0 repeats a row; tokens are less than 2^24 elements apart.  1 <= K, V <= 128, H a multiple of G, B H < 2^31. */
 typedef struct kf_attention_dims {
   int64_t B, T;
   int32_t G, H, K, V;

@@ -1592,6 +1592,11 @@ static int attention_args(kf_handle* h, const kf_attention_dims* d, const char* 
       KF_SET_ERR(h, "%s: strides must not be negative", which);
       return KF_ERR_ARG;
     }
+  for (int64_t st : {d->q_stride[1], d->k_stride[1], d->v_stride[1]})
+    if (st >= 1 << 24) {  // (offsets inside a chunk of tokens are 32 bits wide)
+      KF_SET_ERR(h, "%s: a stride of %ld elements between tokens (below 2^24)", which, (long)st);
+      return KF_ERR_UNSUPPORTED;
+    }
   memset(a, 0, sizeof(*a));
   a->B = d->B; a->T = d->T; a->G = d->G; a->H = d->H; a->K = d->K; a->V = d->V;
   a->dtype = d->dtype; a->per_token = d->decay_per_token != 0; a->scale = (float)d->scale;
@@ -1656,6 +1661,10 @@ extern "C" int kf_linear_attention_backward(kf_handle* h, const kf_attention_dim
   if (dims->g_o_stride[0] < 0 || dims->g_o_stride[1] < 0 || dims->g_o_stride[2] < 0) {
     KF_SET_ERR(h, "kf_linear_attention_backward: strides must not be negative");
     return KF_ERR_ARG;
+  }
+  if (dims->g_o_stride[1] >= 1 << 24) {
+    KF_SET_ERR(h, "kf_linear_attention_backward: a stride of %ld elements between tokens (below 2^24)", (long)dims->g_o_stride[1]);
+    return KF_ERR_UNSUPPORTED;
   }
   rc = workspace_ok(h, "kf_linear_attention_backward", kf_attention_backward_workspace(h, a), workspace, workspace_bytes);
   if (rc) return rc;

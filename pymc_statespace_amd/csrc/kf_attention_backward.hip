@@ -17,7 +17,7 @@
 namespace {
 
 // K and V are padded to one size D; a workgroup has D / 16 waves, wave w has columns 16 w .. of K (in dv: of V).
-template <typename A> constexpr int chunk_of() { return A::PAD == 8 ? 64 : 32; }  // fp32 tiles are twice as wide: half as many tokens
+template <typename A> constexpr int chunk_of() { return sizeof(typename A::elem) == 2 ? 64 : 32; }  // fp32 tiles are twice as wide: half as many tokens
 
 struct Split {
   long works;
@@ -32,21 +32,23 @@ struct Split {
 template <int C, typename A, typename T, int D, int MODE>
 struct Stage {  // C rows of a tensor through registers into LDS
   typedef KfRow<A, T, MODE> Row;
-  static constexpr int N = C * D / 8 / (4 * D), LD = D + A::PAD;
+  typedef KfTile<A, D> Tile;
+  static constexpr int N = C * D / 8 / (4 * D);
   typename Row::Raw r[N];
   static __device__ __forceinline__ int last_row(long t0, long n) { return (int)(n - t0 < C ? n - t0 : C) - 1; }
   __device__ __forceinline__ void load(const T* p, long stride, long t0, long n, int dim) {  // t0 < n
     const int last = last_row(t0, n), row0 = threadIdx.x / (D / 8), col = 8 * (threadIdx.x % (D / 8));
+    const T* base = p + t0 * stride;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       const int row = row0 + 32 * u;
-      r[u] = Row::raw(p + t0 * stride + (row < last ? row : last) * stride, col, dim);
+      r[u] = Row::raw(base, (unsigned)__umul24((unsigned)(row < last ? row : last), (unsigned)stride), col, dim);
     }
   }
   __device__ __forceinline__ void put(typename A::elem* s, long t0, long n, int dim) const {  // the chunk that was loaded
     const int last = last_row(t0, n), row0 = threadIdx.x / (D / 8), col = 8 * (threadIdx.x % (D / 8));
 #pragma unroll
-    for (int u = 0; u < N; ++u) A::put8(s + (row0 + 32 * u) * LD + col, Row::finish(r[u], col, dim, row0 + 32 * u <= last));
+    for (int u = 0; u < N; ++u) Tile::put8(s, row0 + 32 * u, col, Row::finish(r[u], col, dim, row0 + 32 * u <= last));
   }
 };
 
@@ -54,10 +56,11 @@ struct Stage {  // C rows of a tensor through registers into LDS
 // y = do, backward).  STARTS: S, started from the segments before, kept at every chunk's start; else what the segment adds.
 template <typename A, typename T, int D, int MODE, bool STARTS>
 __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Split sp) {
-  constexpr int C = chunk_of<A>(), LD = D + A::PAD, NT = D / 16, TH = 4 * D;
+  constexpr int C = chunk_of<A>(), NT = D / 16, TH = 4 * D;
   typedef typename A::elem E;
-  __shared__ __attribute__((aligned(16))) E sX[C * LD];
-  __shared__ __attribute__((aligned(16))) E sY[C * LD];
+  typedef KfTile<A, D> TD;
+  __shared__ __attribute__((aligned(16))) E sX[C * D];
+  __shared__ __attribute__((aligned(16))) E sY[C * D];
   __shared__ KfChunkDecay<C> dec[2];
   const long work = kf_xcd_work(sp.works);
   if (work >= sp.works) return;
@@ -74,7 +77,7 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
   const long b = rest / segs;
   const int seg = back ? s0 + 1 : s0;  // (nothing is behind the last segment, nothing before the first)
   const long bh = b * a.H + h;
-  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, i = l & 15, g = l >> 4;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i = l & 15, g = l >> 4;
   const long n = kf_row_length(a.lengths, b, a.T);
   const int grp = h / (a.H / a.G);
   const T* x = back ? (const T*)a.q + b * a.qs[0] + grp * a.qs[2] : (const T*)a.k + b * a.ks[0] + grp * a.ks[2];
@@ -108,10 +111,12 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
   float rg = 0.f;
   const long steps = last > c0 ? last - c0 : 0;
   auto at = [&](long s) { return back ? last - 1 - s : c0 + s; };
-  auto decay_of = [&](long c) { return l < C && c * C + l < n ? (a.per_token ? ld[(c * C + l) * a.H] : ld[0]) : 0.f; };
+  const long ld_step = a.per_token ? a.H : 0;
+  auto decay_of = [&](long c) { return ld[(c * C + l < 0 ? 0 : c * C + l < n ? c * C + l : n - 1) * ld_step]; };  // (in bounds for any c)
   if (steps) {
     rx.load(x, xs, at(0) * C, n, a.K);
     ry.load(y, ys, at(0) * C, n, a.V);
+    rg = decay_of(at(1));
     if (w == 0) dec[0].fill(decay_of(at(0)), l < C && at(0) * C + l < n);
   }
   for (long s = 0; s < steps; ++s) {
@@ -129,13 +134,13 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
     rx.put(sX, at(s) * C, n, a.K);
     ry.put(sY, at(s) * C, n, a.V);
     __syncthreads();
-    const bool more = s + 1 < steps;
-    const int wd = (int)((s + 1) % NT);  // the wave that computes the next chunk's decays
-    if (more) {
-      rx.load(x, xs, at(s + 1) * C, n, a.K);
-      ry.load(y, ys, at(s + 1) * C, n, a.V);
-      if (w == wd) rg = decay_of(at(s + 1));
-    }
+    // (loads that no branch surrounds, so that each wait is for its own: behind the last chunk the same one again)
+    const long next = s + 1 < steps ? s + 1 : s;
+    const float g1 = rg;
+    rg = decay_of(at(s + 2));
+    rx.load(x, xs, at(next) * C, n, a.K);
+    ry.load(y, ys, at(next) * C, n, a.V);
+    if (w == (int)(s % NT)) dec[(s + 1) & 1].fill(g1, l < C && at(s + 1) >= 0 && at(s + 1) * C + l < n);
     const KfChunkDecay<C>& d = dec[s & 1];
     const float fe = d.from_start[C - 1];
     through *= fe;
@@ -150,11 +155,10 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
         wt[e] = back ? d.from_start[tok] * a.scale : d.to_end[tok];
       }
       KfSplit<A> xw;
-      xw.set(A::col(sX + 32 * u * LD + 16 * w, LD, i, g), wt);
+      xw.set(TD::col(sX, 32 * u, 16 * w, i, g), wt);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t] = xw.mma_right(A::col(sY + 32 * u * LD + 16 * t, LD, i, g), acc[t]);
+      for (int t = 0; t < NT; ++t) acc[t] = xw.mma_right(TD::col(sY, 32 * u, 16 * t, i, g), acc[t]);
     }
-    if (more && w == wd) dec[(s + 1) & 1].fill(rg, l < C && at(s + 1) * C + l < n);
     __syncthreads();
   }
   if (!STARTS) {
@@ -168,18 +172,20 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
 
 template <typename A, typename T, int D, int MODE>
 __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a, Split sp) {
-  constexpr int C = chunk_of<A>(), LD = D + A::PAD, LP = C + A::PAD, NT = D / 16, CT = C / 16, TH = 4 * D;
+  constexpr int C = chunk_of<A>(), NT = D / 16, CT = C / 16, TH = 4 * D;
+  typedef KfTile<A, D> TD;  // rows of q, k, v, do, R
+  typedef KfTile<A, C> TC;  // rows of scores
   typedef typename A::elem E;
   typedef typename A::frag F;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   E* sQ = (E*)smem;
-  E* sK = sQ + C * LD;
-  E* sV = sK + C * LD;
-  E* sG = sV + C * LD;
-  E* sR = sG + C * LD;   // R as an operand, [k][v]
-  E* sP = sR + D * LD;   // s D A, [i][j]
-  E* sB = sP + C * LP;   // s D B
-  KfChunkDecay<C>* dec = (KfChunkDecay<C>*)(sB + C * LP);
+  E* sK = sQ + C * D;
+  E* sV = sK + C * D;
+  E* sG = sV + C * D;
+  E* sR = sG + C * D;   // R as an operand, [k][v]
+  E* sP = sR + D * D;   // s D A, [i][j]
+  E* sB = sP + C * C;   // s D B
+  KfChunkDecay<C>* dec = (KfChunkDecay<C>*)(sB + C * C);
   float* rs = (float*)(dec + 2);  // [CT][C]: sums of W over the columns of one tile
   float* cs = rs + CT * C;        // [CT][C]: over the rows
   float* xs = cs + CT * C;        // [NT][C]: q . dq|state, this wave's columns of K
@@ -194,7 +200,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
   const int seg = (int)(rest % sp.segments);
   const long b = rest / sp.segments;
   const long bh = b * a.H + h;
-  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, i = l & 15, g = l >> 4;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i = l & 15, g = l >> 4;
   const long n = kf_row_length(a.lengths, b, a.T);
   const int grp = h / (a.H / a.G);
   const T* q = (const T*)a.q + b * a.qs[0] + grp * a.qs[2];
@@ -243,7 +249,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
       if (a.per_token && c == 0) a.g_decay[row] = 0.f;
     }
   }
-  for (int x = tid; x < 2 * C * LP; x += TH) sP[x] = E(0);  // tiles above the diagonal stay zero
+  for (int x = tid; x < 2 * C * C; x += TH) sP[x] = E(0);  // tiles above the diagonal stay zero
 
   Stage<C, A, T, D, MODE> rq, rk, rv, rd;
   float rg = 0.f;
@@ -262,10 +268,12 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
       S0[u][1] = in[(2 * u + 1) * TH];
     }
   };
-  auto decay_of = [&](long c) { return l < C && c * C + l < n ? (a.per_token ? ld[(c * C + l) * a.H] : ld[0]) : 0.f; };
+  const long ld_step = a.per_token ? a.H : 0;
+  auto decay_of = [&](long c) { return ld[(c * C + l < 0 ? 0 : c * C + l < n ? c * C + l : n - 1) * ld_step]; };  // (in bounds for any c)
   if (last > c0) {
     load(last - 1);
     load_start(last - 1);
+    rg = decay_of(last - 2);
     if (w == 0) dec[0].fill(decay_of(last - 1), l < C && (last - 1) * C + l < n);
   }
   double decay_sum = 0.;
@@ -277,13 +285,14 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
     rv.put(sV, t0, n, a.V);
     rd.put(sG, t0, n, a.V);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) A::put4(sR + (16 * w + i) * LD + 16 * t + 4 * g, R[t]);
+    for (int t = 0; t < NT; ++t) TD::put4(sR, 16 * w + i, 16 * t + 4 * g, R[t]);
     __syncthreads();
-    const bool more = c > c0;
-    if (more) {
-      load(c - 1);
-      if (w == 0) rg = decay_of(c - 1);
-    }
+    // (loads that no branch surrounds, so that each wait is for its own: before the first chunk the same one again)
+    const long next = c > c0 ? c - 1 : c;
+    const float g1 = rg;
+    rg = decay_of(c - 2);
+    load(next);
+    if (w == NT - 1) dec[turn ^ 1].fill(g1, l < C && c > 0 && t0 - C + l < n);
     const KfChunkDecay<C>& d = dec[turn];
 
     // scores: tile (it, jt) of A and B, rows j, columns i
@@ -294,8 +303,8 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
       kf_f32x4 sa = {0, 0, 0, 0}, sb = {0, 0, 0, 0};
 #pragma unroll
       for (int u = 0; u < D / 32; ++u) {
-        sa = A::mma(A::row(sK + (16 * jt + i) * LD + 32 * u + 8 * g), A::row(sQ + row * LD + 32 * u + 8 * g), sa);
-        sb = A::mma(A::row(sV + (16 * jt + i) * LD + 32 * u + 8 * g), A::row(sG + row * LD + 32 * u + 8 * g), sb);
+        sa = A::mma(TD::row(sK, 16 * jt + i, 32 * u, g), TD::row(sQ, row, 32 * u, g), sa);
+        sb = A::mma(TD::row(sV, 16 * jt + i, 32 * u, g), TD::row(sG, row, 32 * u, g), sb);
       }
       kf_f32x4 p, pb, wj;
       float wi = 0.f;
@@ -312,8 +321,8 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
         wj[r] = in ? sa[r] * pb[r] : 0.f;
         wi += wj[r];
       }
-      A::put4(sP + row * LP + 16 * jt + 4 * g, p);
-      A::put4(sB + row * LP + 16 * jt + 4 * g, pb);
+      TC::put4(sP, row, 16 * jt + 4 * g, p);
+      TC::put4(sB, row, 16 * jt + 4 * g, pb);
       wi += __shfl_xor(wi, 16);
       wi += __shfl_xor(wi, 32);
       if (g == 0) rs[jt * C + row] = wi;
@@ -337,15 +346,15 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
       fr.set(R[2 * u], R[2 * u + 1]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) cross += fs.value(e) * R[2 * u + (e >> 2)][e & 3];
-      const F fc = A::col(sR + 32 * u * LD + 16 * w, LD, i, g);  // rows v of this wave, depth k
+      const F fc = TD::col(sR, 32 * u, 16 * w, i, g);  // rows v of this wave, depth k
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
-        dq[t] = fs.mma(A::row_t(sG + (16 * t + i) * LD + 32 * u + 4 * g), dq[t]);
-        dk[t] = fr.mma(A::row_t(sV + (16 * t + i) * LD + 32 * u + 4 * g), dk[t]);
-        dv[t] = A::mma(fc, A::row_t(sK + (16 * t + i) * LD + 32 * u + 4 * g), dv[t]);
+        dq[t] = fs.mma(TD::row_t(sG, 16 * t + i, 32 * u, g), dq[t]);
+        dk[t] = fr.mma(TD::row_t(sV, 16 * t + i, 32 * u, g), dk[t]);
+        dv[t] = A::mma(fc, TD::row_t(sK, 16 * t + i, 32 * u, g), dv[t]);
       }
     }
-    if (more) load_start(c - 1);
+    load_start(next);
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) cross += __shfl_xor(cross, m);
     if (l == 0) cr[w] = cross;
@@ -356,7 +365,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
       dq[t] *= fi;
       dk[t] *= fj;
       dv[t] *= fj;
-      const kf_f32x4 qv = A::get4(sQ + tok * LD + 16 * w + 4 * g), kv = A::get4(sK + tok * LD + 16 * w + 4 * g);
+      const kf_f32x4 qv = TD::get4(sQ, tok, 16 * w + 4 * g), kv = TD::get4(sK, tok, 16 * w + 4 * g);
       float x = 0.f, y = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -380,14 +389,14 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
     for (int t = 0; t < NT; ++t) R[t] *= fe;
 #pragma unroll
     for (int u = 0; u < C / 32; ++u) {
-      const F ck = A::col(sK + 32 * u * LD + 16 * w, LD, i, g), cq = A::col(sQ + 32 * u * LD + 16 * w, LD, i, g),
-              cg = A::col(sG + 32 * u * LD + 16 * w, LD, i, g);
+      const F ck = TD::col(sK, 32 * u, 16 * w, i, g), cq = TD::col(sQ, 32 * u, 16 * w, i, g),
+              cg = TD::col(sG, 32 * u, 16 * w, i, g);
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
-        if (2 * u <= t) dq[t] = A::mma(ck, A::row_t(sB + (16 * t + i) * LP + 32 * u + 4 * g), dq[t]);
+        if (2 * u <= t) dq[t] = A::mma(ck, TC::row_t(sB, 16 * t + i, 32 * u, g), dq[t]);
         if (2 * u + 1 >= t) {
-          dk[t] = A::mma(cq, A::col(sB + 32 * u * LP + 16 * t, LP, i, g), dk[t]);
-          dv[t] = A::mma(cg, A::col(sP + 32 * u * LP + 16 * t, LP, i, g), dv[t]);
+          dk[t] = A::mma(cq, TC::col(sB, 32 * u, 16 * t, i, g), dk[t]);
+          dv[t] = A::mma(cg, TC::col(sP, 32 * u, 16 * t, i, g), dv[t]);
         }
       }
       float wt[8];
@@ -396,7 +405,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
       KfSplit<A> qw;
       qw.set(cq, wt);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) R[t] = qw.mma_right(A::col(sG + 32 * u * LD + 16 * t, LD, i, g), R[t]);
+      for (int t = 0; t < NT; ++t) R[t] = qw.mma_right(TD::col(sG, 32 * u, 16 * t, i, g), R[t]);
     }
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
@@ -441,7 +450,6 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
       } else {
         decay_sum += valid ? dg : 0.;
       }
-      if (more) dec[turn ^ 1].fill(rg, l < C && t0 - C + l < n);
     }
     __syncthreads();
   }
@@ -522,8 +530,8 @@ Plan plan(const kf_handle* h, const KfAttnArgs& a) {
 
 template <typename A, typename T, int D, int MODE>
 int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream) {
-  constexpr int C = chunk_of<A>(), LD = D + A::PAD, LP = C + A::PAD;
-  constexpr size_t lds = sizeof(typename A::elem) * ((4 * C + D) * LD + 2 * C * LP) + 2 * sizeof(KfChunkDecay<C>) +
+  constexpr int C = chunk_of<A>();
+  constexpr size_t lds = sizeof(typename A::elem) * ((4 * C + D) * D + 2 * C * C) + 2 * sizeof(KfChunkDecay<C>) +
                          sizeof(float) * (2 * (C / 16) * C + 2 * (D / 16) * C + D / 16);
   static_assert(lds <= 160 * 1024, "LDS of one workgroup");
   const Split& s = p.sp;

@@ -18,13 +18,15 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
   typedef typename A::elem E;
   typedef typename A::frag F;
   typedef KfRow<A, T, MODE> Row;
-  constexpr int LK = KP + A::PAD, LV = VT + A::PAD, NT = VT / 16, KK = KP / 32;
+  typedef KfTile<A, KP> TK;  // k, and the state's transpose
+  typedef KfTile<A, VT> TV;  // v, columns paired (kf_paired): so are the state's columns all through this kernel
+  constexpr int NT = VT / 16, KK = KP / 32;
   constexpr int WK = KP / 16 < 4 ? KP / 16 : 4, WN = 4 / WK;  // the state's tiles: WK waves along K, WN along V
   constexpr int SM = KP / 16 / WK, SN = NT / WN;
   constexpr int RK = 2048 / KP, RV = 2048 / VT;
-  __shared__ __attribute__((aligned(16))) E sK[KF_CHUNK * LK];
-  __shared__ __attribute__((aligned(16))) E sV[KF_CHUNK * LV];
-  __shared__ __attribute__((aligned(16))) E sS[OUT ? VT * LK : 8];  // the state's transpose as an operand
+  __shared__ __attribute__((aligned(16))) E sK[KF_CHUNK * KP];
+  __shared__ __attribute__((aligned(16))) E sV[KF_CHUNK * VT];
+  __shared__ __attribute__((aligned(16))) E sS[OUT ? VT * KP : 8];  // the state's transpose as an operand
   __shared__ __attribute__((aligned(16))) KfChunkDecay<KF_CHUNK> dec[2];
 
   const long work = kf_xcd_work(sp.works);
@@ -37,7 +39,16 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
   const int seg = (int)(rest % segs);
   const long b = rest / segs;
   const long bh = b * a.H + h;
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i = l & 15, g = l >> 4;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i0 = l & 15, g0 = l >> 4;
+  int i = i0, g = g0;
+  // (fp32 operands take twice the registers: there the LDS addresses are computed anew in each part of the loop -- held across it they
+  // spilled, 39 against 37 us for 5 x 1000 tokens; bf16 has room for them, 46 against 47 us for 4 x 2048)
+  auto fresh = [&]() {
+    if constexpr (std::is_same<A, KfF32>::value) {
+      i = kf_fresh(i0);
+      g = kf_fresh(g0);
+    }
+  };
   const int mt0 = (w % WK) * SM, nt0 = (w / WK) * SN;
   const int v0 = vt * VT, nv = a.V - v0;
   const long n = kf_row_length(a.lengths, b, a.T);
@@ -57,7 +68,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
 #pragma unroll
     for (int t = 0; t < SN; ++t) {
       S[m][t] = kf_f32x4{0, 0, 0, 0};
-      const int c = (nt0 + t) * 16 + i;
+      const int c = kf_paired((nt0 + t) * 16 + i);
       if (OUT && a.s0 && c < nv) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -85,43 +96,54 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
   // this lane's part of a chunk: rows kr + u RK of k, vr + u RV of v, row 16 w + i of q
   const int kr = tid / (KP / 8), kc = 8 * (tid % (KP / 8)), vr = tid / (VT / 8), vc = 8 * (tid % (VT / 8));
   auto last_row = [&](long c) { return (int)(n - c * KF_CHUNK < KF_CHUNK ? n - c * KF_CHUNK : KF_CHUNK) - 1; };
-  auto at_row = [](const T* base, long stride, int r, int last) { return base + (r < last ? r : last) * stride; };
+  const unsigned kst = (unsigned)a.ks[1], vst = (unsigned)a.vs[1], qst = (unsigned)a.qs[1];
+  auto off = [](int r, int last, unsigned stride) { return (unsigned)__umul24((unsigned)(r < last ? r : last), stride); };
   auto load = [&](long c) {
     const int last = last_row(c);
     const T *pk = k + c * KF_CHUNK * a.ks[1], *pv = v + c * KF_CHUNK * a.vs[1];
 #pragma unroll
-    for (int u = 0; u < KK; ++u) rk[u] = Row::raw(at_row(pk, a.ks[1], kr + u * RK, last), kc, a.K);
+    for (int u = 0; u < KK; ++u) rk[u] = Row::raw(pk, off(kr + u * RK, last, kst), kc, a.K);
 #pragma unroll
-    for (int u = 0; u < VT / 32; ++u) rv[u] = Row::raw(at_row(pv, a.vs[1], vr + u * RV, last), v0 + vc, a.V);
+    for (int u = 0; u < VT / 32; ++u) rv[u] = Row::raw(pv, off(vr + u * RV, last, vst), v0 + vc, a.V);
   };
   auto load_q = [&](long c) {
-    const T* pq = at_row(q + c * KF_CHUNK * a.qs[1], a.qs[1], 16 * w + i, last_row(c));
+    const T* pq = q + c * KF_CHUNK * a.qs[1];
+    const unsigned r = off(16 * w + i, last_row(c), qst);
 #pragma unroll
-    for (int u = 0; u < KK; ++u) rq[u] = Row::raw(pq, 32 * u + 8 * g, a.K);
+    for (int u = 0; u < KK; ++u) rq[u] = Row::raw(pq, r, 32 * u + 8 * g, a.K);
+  };
+  // full chunks without padded columns need no zeros
+  const bool whole = MODE == KF_ROWS_WHOLE && a.K == KP && nv >= VT;
+  auto put = [&](int last, auto plain) {
+    constexpr bool P = decltype(plain)::value;
+#pragma unroll
+    for (int u = 0; u < KK; ++u) TK::put8(sK, kr + u * RK, kc, Row::template finish<P>(rk[u], kc, a.K, kr + u * RK <= last));
+#pragma unroll
+    for (int u = 0; u < VT / 32; ++u) TV::put8_paired(sV, vr + u * RV, vc, Row::template finish<P>(rv[u], v0 + vc, a.V, vr + u * RV <= last));
   };
   auto log_decay = [&](long c) { return ld[(c * KF_CHUNK + l < n ? c * KF_CHUNK + l : n - 1) * ld_step]; };
   auto put_state = [&]() {
 #pragma unroll
     for (int m = 0; m < SM; ++m)
 #pragma unroll
-      for (int t = 0; t < SN; ++t) A::put4(sS + ((nt0 + t) * 16 + i) * LK + (mt0 + m) * 16 + 4 * g, S[m][t]);
+      for (int t = 0; t < SN; ++t) TK::put4(sS, (nt0 + t) * 16 + i, (mt0 + m) * 16 + 4 * g, S[m][t]);
   };
 
   if (c0 < end) {
-    const float g0 = log_decay(c0);
+    const float first = log_decay(c0);
     rg = log_decay(c0 + 1);
     load(c0);
     if (OUT) load_q(c0);
-    if (w == 0) dec[c0 & 1].fill(g0, c0 * KF_CHUNK + l < n);
+    if (w == 0) dec[c0 & 1].fill(first, c0 * KF_CHUNK + l < n);
     if (OUT) put_state();
   }
   for (long c = c0; c < end; ++c) {
     const long t0 = c * KF_CHUNK, next = c + 1 < end ? c + 1 : c;
+    fresh();
     const int last = last_row(c);  // rows behind it are zero
-#pragma unroll
-    for (int u = 0; u < KK; ++u) A::put8(sK + (kr + u * RK) * LK + kc, Row::finish(rk[u], kc, a.K, kr + u * RK <= last));
-#pragma unroll
-    for (int u = 0; u < VT / 32; ++u) A::put8(sV + (vr + u * RV) * LV + vc, Row::finish(rv[u], v0 + vc, a.V, vr + u * RV <= last));
+    const bool plain = whole && last == KF_CHUNK - 1;
+    if (plain) put(last, std::true_type{});
+    else put(last, std::false_type{});
     __syncthreads();
     const float g1 = rg;
     rg = log_decay(c + 2);
@@ -132,8 +154,13 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
     if (OUT) {
       const int row = 16 * w + i;
       F fq[KK];
+      if (plain) {
 #pragma unroll
-      for (int u = 0; u < KK; ++u) fq[u] = Row::finish(rq[u], 32 * u + 8 * g, a.K, row <= last);
+        for (int u = 0; u < KK; ++u) fq[u] = Row::template finish<true>(rq[u], 0, 0, true);
+      } else {
+#pragma unroll
+        for (int u = 0; u < KK; ++u) fq[u] = Row::finish(rq[u], 32 * u + 8 * g, a.K, row <= last);
+      }
       // scores, transposed: rows j, columns i; as operands, two tiles each.  (w is the same for a whole wave.)
       F p[2];
 #pragma unroll
@@ -145,7 +172,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
           kf_f32x4 s = {0, 0, 0, 0};
           if (jt <= w) {
 #pragma unroll
-            for (int u = 0; u < KK; ++u) s = A::mma(A::row(sK + (16 * jt + i) * LK + 32 * u + 8 * g), fq[u], s);
+            for (int u = 0; u < KK; ++u) s = A::mma(TK::row(sK, 16 * jt + i, 32 * u, g), fq[u], s);
             if (jt < w) {
               s *= D.from_tile[jt < 3 ? jt : 2][row] * a.scale;
               s *= *reinterpret_cast<const kf_f32x4*>(&D.to_tile_end[16 * jt + 4 * g]);
@@ -166,9 +193,10 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
       auto from_state = [&](int v1) {
         kf_f32x4 o = {0, 0, 0, 0};
 #pragma unroll
-        for (int x = 0; x < KK; ++x) o = A::mma(A::row(sS + (v1 + 8 * (i >> 2) + (i & 3)) * LK + 32 * x + 8 * g), fq[x], o);
+        for (int x = 0; x < KK; ++x) o = A::mma(TK::row(sS, v1 + i, 32 * x, g), fq[x], o);
         return o * fs;
       };
+      fresh();
       KfOut8<T> ready[NT / 2];
       float check = 0.f;
 #pragma unroll
@@ -176,13 +204,18 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
         kf_f32x4 o[2];
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          o[y] = from_state(16 * u + 4 * y);
+          o[y] = from_state(16 * (u + y));
 #pragma unroll
-          for (int x = 0; x < 2; ++x) o[y] = A::mma(A::col8(sV + 32 * x * LV + 16 * u + 4 * y, LV, i, g), p[x], o[y]);
+          for (int x = 0; x < 2; ++x) o[y] = A::mma(TV::col(sV, 32 * x, 16 * (u + y), i, g), p[x], o[y]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) check = fmaf(o[y][r], 0.f, check);
+        }
+        if (!plain) {  // (a row behind the end has a query of zeros; the state may be infinite all the same)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[y][r] = t < n ? o[y][r] : 0.f;
+          for (int r = 0; r < 4; ++r) {
+            o[0][r] = t < n ? o[0][r] : 0.f;
+            o[1][r] = t < n ? o[1][r] : 0.f;
+          }
         }
         ready[u / 2].set(o[0], o[1]);
       }
@@ -191,11 +224,11 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
         // A token's infinity or NaN in v would reach the rows before it as 0 x inf: the products once more without such values, and
         // these added only to the rows from their token on.
 #pragma unroll 1
-        for (int v1 = 0; v1 < VT; v1 += v1 & 4 ? 28 : 4) {
+        for (int v1 = 0; v1 < VT; v1 += 16) {
           kf_f32x4 o = from_state(v1);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            o = A::mma(A::finite(A::col8(sV + 32 * x * LV + v1, LV, i, g)), p[x], o);
+            o = A::mma(A::finite(TV::col(sV, 32 * x, v1, i, g)), p[x], o);
 #pragma unroll 1
             for (int j = 0; j < 32; ++j) {  // token 32 x + j: value e = 4 (j / 16) + j % 4 of lane group (j % 16) / 4
               float pj = 0.f;
@@ -205,12 +238,13 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
               if (32 * x + j <= row)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                  const float z = A::get(sV + (32 * x + j) * LV + v1 + 8 * g + r);
+                  const float z = A::get(sV + TV::at(32 * x + j, v1 + 4 * g + r));
                   if (!(fabsf(z) <= 3.4e38f)) o[r] += pj * z;
                 }
             }
           }
-          if (t < n) kf_store4(out + v1 + 8 * g, o, nv - v1 - 8 * g);
+          const int cv = kf_paired(v1 + 4 * g);
+          if (t < n) kf_store4(out + cv, o, nv - cv);
         }
       }
       // (loads and stores are waited for in the order they were issued in: the next chunk's loads first)
@@ -222,6 +256,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
     }
 
     // the state at the chunk's end
+    fresh();
     const float fe = D.from_start[KF_CHUNK - 1];
     through *= fe;
 #pragma unroll
@@ -234,11 +269,11 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
       const float wt[8] = {w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]};
       F fv[SN];
 #pragma unroll
-      for (int t = 0; t < SN; ++t) fv[t] = A::col(sV + 32 * x * LV + 16 * (nt0 + t), LV, i, g);
+      for (int t = 0; t < SN; ++t) fv[t] = TV::col(sV, 32 * x, 16 * (nt0 + t), i, g);
 #pragma unroll
       for (int m = 0; m < SM; ++m) {
         KfSplit<A> kw;
-        kw.set(A::col(sK + 32 * x * LK + 16 * (mt0 + m), LK, i, g), wt);
+        kw.set(TK::col(sK, 32 * x, 16 * (mt0 + m), i, g), wt);
 #pragma unroll
         for (int t = 0; t < SN; ++t) S[m][t] = kw.mma(fv[t], S[m][t]);
       }
@@ -258,7 +293,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
         for (int t = 0; t < SN; ++t)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int kk = (mt0 + m) * 16 + 4 * g + r, cc = (nt0 + t) * 16 + i;
+            const int kk = (mt0 + m) * 16 + 4 * g + r, cc = kf_paired((nt0 + t) * 16 + i);
             if (kk < a.K && cc < nv) a.sT[(bh * a.K + kk) * a.V + v0 + cc] = S[m][t][r];
           }
     }

@@ -18,6 +18,14 @@ typedef float kf_f32x4 __attribute__((ext_vector_type(4)));
 typedef float kf_f32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned kf_u32x4 __attribute__((ext_vector_type(4)));
 
+// x, but computed anew here as far as the compiler can tell: keeps addresses built from it out of registers held across a loop
+static __device__ __forceinline__ int kf_fresh(int x) {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("" : "+v"(x));
+#endif
+  return x;
+}
+
 static __device__ __forceinline__ unsigned kf_bits(float x) { return __builtin_bit_cast(unsigned, x); }
 static __device__ __forceinline__ float kf_float_of(unsigned x) { return __builtin_bit_cast(float, x); }
 // two floats rounded to nearest even, packed (v_cvt_pk_bf16_f32)
@@ -31,30 +39,7 @@ static __device__ __forceinline__ unsigned kf_pack_bf16(float lo, float hi) {
 struct KfBf16 {
   typedef unsigned short elem;
   typedef kf_bf16x8 frag;
-  static constexpr int PAD = 8;  // elements after a row in LDS: 16 bytes, so that 16 rows start in different banks
   static __device__ __forceinline__ kf_f32x4 mma(frag a, frag b, kf_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-  static __device__ __forceinline__ frag zero() { return __builtin_bit_cast(frag, kf_u32x4{0, 0, 0, 0}); }
-  // row i of a [i][depth] tile, p at its first depth of this lane
-  static __device__ __forceinline__ frag row(const elem* p) { return *reinterpret_cast<const frag*>(p); }
-  // the same row at depth T, p at 4 g
-  static __device__ __forceinline__ frag row_t(const elem* p) {
-    const kf_s16x4 x = *reinterpret_cast<const kf_s16x4*>(p), y = *reinterpret_cast<const kf_s16x4*>(p + 16);
-    return __builtin_bit_cast(frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-  }
-  // column i of a [depth][i] tile, p at its corner
-  static __device__ __forceinline__ frag col(const elem* p, int ld, int i, int g) {
-    const elem* a = p + (4 * g + (i >> 2)) * ld + 4 * (i & 3);
-    typedef __attribute__((address_space(3))) kf_s16x4* lds;
-    const kf_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)a), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(a + 16 * ld));
-    return __builtin_bit_cast(frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-  }
-  // columns 8 (i / 4) + i % 4 of it: with the ones 4 further on in a second fragment, a lane ends up with 8 neighbours
-  static __device__ __forceinline__ frag col8(const elem* p, int ld, int i, int g) {
-    const elem* a = p + (4 * g + (i >> 2)) * ld + 8 * (i & 3);
-    typedef __attribute__((address_space(3))) kf_s16x4* lds;
-    const kf_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)a), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(a + 16 * ld));
-    return __builtin_bit_cast(frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-  }
   static __device__ __forceinline__ frag from(kf_f32x4 x, kf_f32x4 y) {
     return __builtin_bit_cast(frag, kf_u32x4{kf_pack_bf16(x[0], x[1]), kf_pack_bf16(x[2], x[3]), kf_pack_bf16(y[0], y[1]), kf_pack_bf16(y[2], y[3])});
   }
@@ -68,47 +53,16 @@ struct KfBf16 {
     for (int e = 0; e < 8; ++e) x[e] = (x[e] & 0x7f80) == 0x7f80 ? (short)0 : x[e];
     return __builtin_bit_cast(frag, x);
   }
-  // four consecutive elements
-  static __device__ __forceinline__ void put4(elem* p, kf_f32x4 x) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(kf_pack_bf16(x[0], x[1]), kf_pack_bf16(x[2], x[3]));
-  }
-  static __device__ __forceinline__ void put8(elem* p, frag x) { *reinterpret_cast<frag*>(p) = x; }
   static __device__ __forceinline__ float get(const elem* p) { return kf_float_of((unsigned)*p << 16); }
-  static __device__ __forceinline__ kf_f32x4 get4(const elem* p) {
-    const uint2 x = *reinterpret_cast<const uint2*>(p);
-    return kf_f32x4{kf_float_of(x.x << 16), kf_float_of(x.x & 0xffff0000u), kf_float_of(x.y << 16), kf_float_of(x.y & 0xffff0000u)};
-  }
 };
 
 struct KfF32 {
   typedef float elem;
   typedef kf_f32x8 frag;
-  static constexpr int PAD = 4;
   static __device__ __forceinline__ kf_f32x4 mma(frag a, frag b, kf_f32x4 c) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
     return c;
-  }
-  static __device__ __forceinline__ frag zero() { return frag{0, 0, 0, 0, 0, 0, 0, 0}; }
-  static __device__ __forceinline__ frag row(const elem* p) {
-    const kf_f32x4 x = *reinterpret_cast<const kf_f32x4*>(p), y = *reinterpret_cast<const kf_f32x4*>(p + 4);
-    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-  }
-  static __device__ __forceinline__ frag row_t(const elem* p) {
-    const kf_f32x4 x = *reinterpret_cast<const kf_f32x4*>(p), y = *reinterpret_cast<const kf_f32x4*>(p + 16);
-    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-  }
-  static __device__ __forceinline__ frag col(const elem* p, int ld, int i, int g) {
-    frag f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = p[(16 * (e >> 2) + 4 * g + (e & 3)) * ld + i];
-    return f;
-  }
-  static __device__ __forceinline__ frag col8(const elem* p, int ld, int i, int g) {
-    frag f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = p[(16 * (e >> 2) + 4 * g + (e & 3)) * ld + 8 * (i >> 2) + (i & 3)];
-    return f;
   }
   static __device__ __forceinline__ frag from(kf_f32x4 x, kf_f32x4 y) { return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7); }
   static __device__ __forceinline__ float value(frag a, int e) { return a[e]; }
@@ -117,14 +71,81 @@ struct KfF32 {
     for (int e = 0; e < 8; ++e) a[e] = (kf_bits(a[e]) & 0x7f800000u) == 0x7f800000u ? 0.f : a[e];
     return a;
   }
-  static __device__ __forceinline__ void put4(elem* p, kf_f32x4 x) { *reinterpret_cast<kf_f32x4*>(p) = x; }
-  static __device__ __forceinline__ void put8(elem* p, frag x) {
-    put4(p, __builtin_shufflevector(x, x, 0, 1, 2, 3));
-    put4(p + 4, __builtin_shufflevector(x, x, 4, 5, 6, 7));
-  }
   static __device__ __forceinline__ float get(const elem* p) { return *p; }
-  static __device__ __forceinline__ kf_f32x4 get4(const elem* p) { return *reinterpret_cast<const kf_f32x4*>(p); }
 };
+
+// Rows of COLS elements in LDS.  The 16-byte pieces of a row are permuted (by exclusive or) so that each of the reads below meets
+// different banks: 8 rows' pieces at the same depth, and 32 bytes of 4 neighbouring rows, fill the 128 bytes of a cycle.
+template <typename A, int COLS> struct KfTile;
+template <int COLS, int PIECE> struct KfTileAt {
+  static __device__ __forceinline__ int at(int r, int c) {
+    constexpr int PIECES = COLS / PIECE;
+    static_assert(PIECES >= 4, "a row of 64 bytes at least");
+    const int x = PIECES >= 8 ? ((r & 3) << 1) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1);
+    return r * COLS + (((c / PIECE) ^ x) * PIECE) + c % PIECE;
+  }
+};
+template <int COLS> struct KfTile<KfBf16, COLS> : KfTileAt<COLS, 8> {
+  typedef KfBf16::elem E;
+  typedef KfBf16::frag F;
+  using KfTileAt<COLS, 8>::at;
+  // operand: row r, depths c .. c + 31 in order C (c a multiple of 32)
+  static __device__ __forceinline__ F row(const E* p, int r, int c, int g) { return *reinterpret_cast<const F*>(p + at(r, c + 8 * g)); }
+  // the same in order T
+  static __device__ __forceinline__ F row_t(const E* p, int r, int c, int g) {
+    const kf_s16x4 x = *reinterpret_cast<const kf_s16x4*>(p + at(r, c + 4 * g)), y = *reinterpret_cast<const kf_s16x4*>(p + at(r, c + 16 + 4 * g));
+    return __builtin_bit_cast(F, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  // operand: column c + i, depths r .. r + 31 of the rows in order T
+  static __device__ __forceinline__ F col(const E* p, int r, int c, int i, int g) {
+    typedef __attribute__((address_space(3))) kf_s16x4* lds;
+    const int rr = r + 4 * g + (i >> 2), cc = c + 4 * (i & 3);
+    const kf_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(p + at(rr, cc))), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(p + at(rr + 16, cc)));
+    return __builtin_bit_cast(F, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  static __device__ __forceinline__ void put8(E* p, int r, int c, F x) { *reinterpret_cast<F*>(p + at(r, c)) = x; }
+  // with the columns of each 32 so ordered that a lane's four values of two neighbouring 16-wide tiles are 8 neighbours: column
+  // 8 a + 4 y + b at 16 y + 4 a + b
+  static __device__ __forceinline__ void put8_paired(E* p, int r, int c, F x) {
+    const kf_u32x4 w = __builtin_bit_cast(kf_u32x4, x);
+    const int to = (c & ~31) + (c & 31) / 2;
+    *reinterpret_cast<uint2*>(p + at(r, to)) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(p + at(r, to + 16)) = make_uint2(w[2], w[3]);
+  }
+  static __device__ __forceinline__ void put4(E* p, int r, int c, kf_f32x4 x) {
+    *reinterpret_cast<uint2*>(p + at(r, c)) = make_uint2(kf_pack_bf16(x[0], x[1]), kf_pack_bf16(x[2], x[3]));
+  }
+  static __device__ __forceinline__ kf_f32x4 get4(const E* p, int r, int c) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p + at(r, c));
+    return kf_f32x4{kf_float_of(x.x << 16), kf_float_of(x.x & 0xffff0000u), kf_float_of(x.y << 16), kf_float_of(x.y & 0xffff0000u)};
+  }
+};
+template <int COLS> struct KfTile<KfF32, COLS> : KfTileAt<COLS, 4> {
+  typedef KfF32::elem E;
+  typedef KfF32::frag F;
+  using KfTileAt<COLS, 4>::at;
+  static __device__ __forceinline__ kf_f32x4 get4(const E* p, int r, int c) { return *reinterpret_cast<const kf_f32x4*>(p + at(r, c)); }
+  static __device__ __forceinline__ F row(const E* p, int r, int c, int g) { return KfF32::from(get4(p, r, c + 8 * g), get4(p, r, c + 8 * g + 4)); }
+  static __device__ __forceinline__ F row_t(const E* p, int r, int c, int g) { return KfF32::from(get4(p, r, c + 4 * g), get4(p, r, c + 16 + 4 * g)); }
+  static __device__ __forceinline__ F col(const E* p, int r, int c, int i, int g) {
+    F f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = p[at(r + 16 * (e >> 2) + 4 * g + (e & 3), c + i)];
+    return f;
+  }
+  static __device__ __forceinline__ void put4(E* p, int r, int c, kf_f32x4 x) { *reinterpret_cast<kf_f32x4*>(p + at(r, c)) = x; }
+  static __device__ __forceinline__ void put8(E* p, int r, int c, F x) {
+    put4(p, r, c, __builtin_shufflevector(x, x, 0, 1, 2, 3));
+    put4(p, r, c + 4, __builtin_shufflevector(x, x, 4, 5, 6, 7));
+  }
+  static __device__ __forceinline__ void put8_paired(E* p, int r, int c, F x) {
+    const int to = (c & ~31) + (c & 31) / 2;
+    put4(p, r, to, __builtin_shufflevector(x, x, 0, 1, 2, 3));
+    put4(p, r, to + 16, __builtin_shufflevector(x, x, 4, 5, 6, 7));
+  }
+};
+// the column that stands at place c of such rows
+static __device__ __forceinline__ int kf_paired(int c) { return (c & ~31) + 8 * ((c >> 2) & 3) + 4 * ((c >> 4) & 1) + (c & 3); }
 
 // fp32 numbers as one operand (accumulators of two 16 x 16 tiles, or a fragment times a weight for each depth): fp32 as they are;
 // bf16 in two rounded parts, 2 x 8 bits and a sign (at most 2^-18 of each value is lost, 7e-7 on average; one part alone would lose
@@ -179,7 +200,8 @@ template <> struct KfSplit<KfBf16> {
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) KfAny16 { kf_u32x4 v; };
 
 // Elements col .. col + 7 of a global row of `dim` elements as the arithmetic's own, zeros from dim on and where !ok (`row` is
-// readable all the same), in two steps: `raw` only loads, so that nothing waits for it until `finish` is called.  No branches:
+// readable all the same), in two steps: `raw` only loads, so that nothing waits for it until `finish` is called (PLAIN: it is known that
+// nothing is to be zero).  No branches:
 //   KF_ROWS_WHOLE   dim % 8 == 0
 //   KF_ROWS_CUT     dim >= 8: the last piece is read from where it still ends inside the row, and moved down by the elements too many
 //                   (a number that is the same for all lanes)
@@ -200,48 +222,52 @@ static __device__ __forceinline__ kf_u32x4 kf_down16(kf_u32x4 x, int s) {
 }
 template <int MODE> struct KfRow16 {
   typedef kf_u32x4 Raw;
-  template <typename T> static __device__ __forceinline__ Raw raw(const T* row, int col, int dim) {
+  // the row at `row` elements behind `base` (the same for all lanes)
+  template <typename T> static __device__ __forceinline__ Raw raw(const T* base, unsigned row, int col, int dim) {
     if constexpr (MODE == KF_ROWS_NARROW) {
       kf_s16x8 r;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = col + e < dim ? reinterpret_cast<const short*>(row)[col + e] : (short)0;
+      for (int e = 0; e < 8; ++e) r[e] = col + e < dim ? reinterpret_cast<const short*>(base)[row + col + e] : (short)0;
       return __builtin_bit_cast(Raw, r);
     } else {
-      return reinterpret_cast<const KfAny16<T>*>(row + (col < dim - 8 ? col : dim - 8))->v;
+      const unsigned off = (row + (unsigned)(col < dim - 8 ? col : dim - 8)) * (unsigned)sizeof(T);
+      return reinterpret_cast<const KfAny16<T>*>(reinterpret_cast<const char*>(base) + off)->v;
     }
   }
-  static __device__ __forceinline__ Raw bits(Raw x, int col, int dim, bool ok) {
+  template <bool PLAIN = false> static __device__ __forceinline__ Raw bits(Raw x, int col, int dim, bool ok) {
+    if constexpr (PLAIN) return x;
     if constexpr (MODE == KF_ROWS_CUT) x = kf_down16(x, col + 8 > dim && col < dim ? col + 8 - dim : 0);
     return kf_keep(x, ok && col < dim);
   }
 };
 template <typename A, typename T, int MODE> struct KfRow;
 template <int MODE> struct KfRow<KfBf16, __hip_bfloat16, MODE> : KfRow16<MODE> {
-  static __device__ __forceinline__ kf_bf16x8 finish(kf_u32x4 x, int col, int dim, bool ok) {
-    return __builtin_bit_cast(kf_bf16x8, KfRow16<MODE>::bits(x, col, dim, ok));
+  template <bool PLAIN = false> static __device__ __forceinline__ kf_bf16x8 finish(kf_u32x4 x, int col, int dim, bool ok) {
+    return __builtin_bit_cast(kf_bf16x8, KfRow16<MODE>::template bits<PLAIN>(x, col, dim, ok));
   }
 };
 template <int MODE> struct KfRow<KfF32, __half, MODE> : KfRow16<MODE> {
-  static __device__ __forceinline__ kf_f32x8 finish(kf_u32x4 x, int col, int dim, bool ok) {
+  template <bool PLAIN = false> static __device__ __forceinline__ kf_f32x8 finish(kf_u32x4 x, int col, int dim, bool ok) {
     typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-    return __builtin_convertvector(__builtin_bit_cast(h8, KfRow16<MODE>::bits(x, col, dim, ok)), kf_f32x8);
+    return __builtin_convertvector(__builtin_bit_cast(h8, KfRow16<MODE>::template bits<PLAIN>(x, col, dim, ok)), kf_f32x8);
   }
 };
 template <int MODE> struct KfRow<KfF32, float, MODE> {
   typedef kf_f32x8 Raw;
-  static __device__ __forceinline__ Raw raw(const float* row, int col, int dim) {
+  static __device__ __forceinline__ Raw raw(const float* base, unsigned row, int col, int dim) {
     Raw r;
     if constexpr (MODE == KF_ROWS_NARROW) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = col + e < dim ? row[col + e] : 0.f;
+      for (int e = 0; e < 8; ++e) r[e] = col + e < dim ? base[row + col + e] : 0.f;
     } else {
-      const float* p = row + (col < dim - 8 ? col : dim - 8);
+      const char* p = reinterpret_cast<const char*>(base) + (row + (unsigned)(col < dim - 8 ? col : dim - 8)) * 4u;
       r = KfF32::from(__builtin_bit_cast(kf_f32x4, reinterpret_cast<const KfAny16<float>*>(p)->v),
-                      __builtin_bit_cast(kf_f32x4, reinterpret_cast<const KfAny16<float>*>(p + 4)->v));
+                      __builtin_bit_cast(kf_f32x4, reinterpret_cast<const KfAny16<float>*>(p + 16)->v));
     }
     return r;
   }
-  static __device__ __forceinline__ kf_f32x8 finish(Raw x, int col, int dim, bool ok) {
+  template <bool PLAIN = false> static __device__ __forceinline__ kf_f32x8 finish(Raw x, int col, int dim, bool ok) {
+    if constexpr (PLAIN) return x;
     if constexpr (MODE == KF_ROWS_CUT) {
       const int s = col + 8 > dim && col < dim ? col + 8 - dim : 0;
       kf_f32x8 y;

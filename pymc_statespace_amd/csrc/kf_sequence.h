@@ -10,7 +10,7 @@ struct KfAttnArgs {
   int G, H, K, V;
   int dtype, per_token;
   float scale;
-  const void *q, *k, *v, *g_o;           // last axis contiguous, strides below (elements): batch, token, head
+  const void *q, *k, *v, *g_o;           // last axis contiguous, strides below (elements): batch, token (below 2^24), head
   long qs[3], ks[3], vs[3], gs[3];
   const float* log_decay;                // [B][T][H] (per_token) or [H]
   const float* s0;                       // [B][H][K][V] or NULL

@@ -713,7 +713,7 @@ class KalmanEngine:
             raise TypeError(f"{name} is {t.dtype}, q is {dtype}: q, k, v and g_o share one type")
         if t.device != self.device:
             t = t.detach().to(self.device)
-        return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.detach().contiguous()
+        return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and (ndim == 3 or t.stride(1) < 1 << 24) else t.detach().contiguous()
 
     def _seq_f32(self, x, name, shape):
         """An fp32 operand (log decays, states), contiguous; other types are converted."""

@@ -90,13 +90,14 @@ def _dims(**kw):
     (dict(B=0), -1), (dict(T=0), -1), (dict(G=0), -1), (dict(H=0), -1), (dict(K=0), -1), (dict(V=-3), -1), (dict(H=3, G=2), -1),
     (dict(K=129), -4), (dict(V=200), -4), (dict(dtype=0), -4), (dict(dtype=7), -4), (dict(scale=float("nan")), -1),
     (dict(scale=float("inf")), -1), (dict(scale=1e39), -1), (dict(B=2**31), -4), (dict(T=2**31), -4), (dict(B=2**30, H=4), -4),
-    (dict(q_stride=(0, -1, 0)), -1), (dict(k_stride=(-8, 8, 8)), -1), (dict(v_stride=(8, 8, -8)), -1)])
+    (dict(q_stride=(0, -1, 0)), -1), (dict(k_stride=(-8, 8, 8)), -1), (dict(v_stride=(8, 8, -8)), -1),
+    (dict(k_stride=(0, 1 << 24, 0)), -4)])
 def test_sizes_that_are_refused(lib, handle, bad, rc):
     d, n, one = _dims(**bad), C.c_size_t(), C.c_void_p(16)
     assert lib.kf_linear_attention_workspace(handle, C.byref(d), 0, C.byref(n)) == rc
     assert lib.kf_linear_attention(handle, C.byref(d), *[one] * 8, one, 1 << 30, None) == rc
     assert lib.kf_linear_attention_backward(handle, C.byref(d), *[one] * 13, one, 1 << 30, None) == rc
-    if not {"T", "q_stride"} & set(bad):
+    if not {"T", "q_stride"} & set(bad) and bad.get("k_stride") != (0, 1 << 24, 0):
         assert lib.kf_linear_attention_step(handle, C.byref(d), *[one] * 5, 4, *[one] * 4, None) == rc
     assert lib.kf_last_error(handle)
 
