@@ -200,7 +200,13 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
   const int seg = (int)(rest % sp.segments);
   const long b = rest / sp.segments;
   const long bh = b * a.H + h;
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i = l & 15, g = l >> 4;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i0 = l & 15, g0 = l >> 4;
+  int i = i0, g = g0;
+  // LDS addresses are computed anew in each part of the loop: held across it they would not fit the registers
+  auto fresh = [&]() {
+    i = kf_fresh(i0);
+    g = kf_fresh(g0);
+  };
   const long n = kf_row_length(a.lengths, b, a.T);
   const int grp = h / (a.H / a.G);
   const T* q = (const T*)a.q + b * a.qs[0] + grp * a.qs[2];
@@ -280,6 +286,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
   int turn = 0;
   for (long c = last - 1; c >= c0; --c, turn ^= 1) {
     const long t0 = c * C;
+    fresh();
     rq.put(sQ, t0, n, a.K);
     rk.put(sK, t0, n, a.K);
     rv.put(sV, t0, n, a.V);
@@ -296,6 +303,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
     const KfChunkDecay<C>& d = dec[turn];
 
     // scores: tile (it, jt) of A and B, rows j, columns i
+    fresh();
     for (int x = w; x < CT * (CT + 1) / 2; x += NT) {
       int it = 0;
       while ((it + 1) * (it + 2) / 2 <= x) ++it;
@@ -335,6 +343,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
     }
 
     // through the states; rows k (dv: rows v), columns tokens
+    fresh();
     kf_f32x4 dq[CT], dk[CT], dv[CT];
 #pragma unroll
     for (int t = 0; t < CT; ++t) dq[t] = dk[t] = dv[t] = kf_f32x4{0, 0, 0, 0};
@@ -358,6 +367,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) cross += __shfl_xor(cross, m);
     if (l == 0) cr[w] = cross;
+    fresh();
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
       const int tok = 16 * t + i;
@@ -384,6 +394,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
     __syncthreads();
 
     // inside the chunk, and R at its start
+    fresh();
     const float fe = d.from_start[C - 1];
 #pragma unroll
     for (int t = 0; t < NT; ++t) R[t] *= fe;
@@ -407,6 +418,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
 #pragma unroll
       for (int t = 0; t < NT; ++t) R[t] = qw.mma_right(TD::col(sG, 32 * u, 16 * t, i, g), R[t]);
     }
+    fresh();
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
       const long tok = t0 + 16 * t + i, row = (b * a.T + tok) * a.H + h;
