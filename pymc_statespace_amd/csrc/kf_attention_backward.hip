@@ -78,6 +78,7 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
   const int seg = back ? s0 + 1 : s0;  // (nothing is behind the last segment, nothing before the first)
   const long bh = b * a.H + h;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i = l & 15, g = l >> 4;
+  const KfLanes lt = TD::lanes(i, g);
   const long n = kf_row_length(a.lengths, b, a.T);
   const int grp = h / (a.H / a.G);
   const T* x = back ? (const T*)a.q + b * a.qs[0] + grp * a.qs[2] : (const T*)a.k + b * a.ks[0] + grp * a.ks[2];
@@ -155,9 +156,9 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
         wt[e] = back ? d.from_start[tok] * a.scale : d.to_end[tok];
       }
       KfSplit<A> xw;
-      xw.set(TD::col(sX, 32 * u, 16 * w, i, g), wt);
+      xw.set(TD::col(sX, lt, 32 * u, 16 * w), wt);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t] = xw.mma_right(TD::col(sY, 32 * u, 16 * t, i, g), acc[t]);
+      for (int t = 0; t < NT; ++t) acc[t] = xw.mma_right(TD::col(sY, lt, 32 * u, 16 * t), acc[t]);
     }
     __syncthreads();
   }
@@ -200,12 +201,13 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
   const int seg = (int)(rest % sp.segments);
   const long b = rest / sp.segments;
   const long bh = b * a.H + h;
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i0 = l & 15, g0 = l >> 4;
-  int i = i0, g = g0;
-  // LDS addresses are computed anew in each part of the loop: held across it they would not fit the registers
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i = l & 15, g = l >> 4;
+  const KfLanes lt0 = TD::lanes(i, g), lc0 = TC::lanes(i, g);
+  KfLanes lt = lt0, lc = lc0;
+  // each part of the loop builds its LDS addresses from these six anew: held across it they would not fit the registers
   auto fresh = [&]() {
-    i = kf_fresh(i0);
-    g = kf_fresh(g0);
+    lt = kf_fresh(lt0);
+    lc = kf_fresh(lc0);
   };
   const long n = kf_row_length(a.lengths, b, a.T);
   const int grp = h / (a.H / a.G);
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
     rv.put(sV, t0, n, a.V);
     rd.put(sG, t0, n, a.V);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) TD::put4(sR, 16 * w + i, 16 * t + 4 * g, R[t]);
+    for (int t = 0; t < NT; ++t) TD::put4(sR, lt, 16 * w, 16 * t, R[t]);
     __syncthreads();
     // (loads that no branch surrounds, so that each wait is for its own: before the first chunk the same one again)
     const long next = c > c0 ? c - 1 : c;
@@ -307,21 +309,21 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
     for (int x = w; x < CT * (CT + 1) / 2; x += NT) {
       int it = 0;
       while ((it + 1) * (it + 2) / 2 <= x) ++it;
-      const int jt = x - it * (it + 1) / 2, row = 16 * it + i;
+      const int jt = x - it * (it + 1) / 2, i1 = kf_fresh(i), gs = kf_fresh(g), row = 16 * it + i1;
       kf_f32x4 sa = {0, 0, 0, 0}, sb = {0, 0, 0, 0};
 #pragma unroll
       for (int u = 0; u < D / 32; ++u) {
-        sa = A::mma(TD::row(sK, 16 * jt + i, 32 * u, g), TD::row(sQ, row, 32 * u, g), sa);
-        sb = A::mma(TD::row(sV, 16 * jt + i, 32 * u, g), TD::row(sG, row, 32 * u, g), sb);
+        sa = A::mma(TD::row(sK, lt, 16 * jt, 32 * u), TD::row(sQ, lt, 16 * it, 32 * u), sa);
+        sb = A::mma(TD::row(sV, lt, 16 * jt, 32 * u), TD::row(sG, lt, 16 * it, 32 * u), sb);
       }
       kf_f32x4 p, pb, wj;
       float wi = 0.f;
       kf_f32x4 fac;
-      if (it == jt) fac = d.pairs(row, 16 * jt + 4 * g) * a.scale;
-      else fac = *reinterpret_cast<const kf_f32x4*>(&d.to_tile_end[16 * jt + 4 * g]) * (d.from_tile[jt][row] * a.scale);
+      if (it == jt) fac = d.pairs(row, 16 * jt + 4 * gs) * a.scale;
+      else fac = *reinterpret_cast<const kf_f32x4*>(&d.to_tile_end[16 * jt + 4 * gs]) * (d.from_tile[jt][row] * a.scale);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int j = 16 * jt + 4 * g + r;
+        const int j = 16 * jt + 4 * gs + r;
         const bool in = j <= row;
         const float f = fac[r];
         p[r] = in ? sa[r] * f : 0.f;
@@ -329,16 +331,15 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
         wj[r] = in ? sa[r] * pb[r] : 0.f;
         wi += wj[r];
       }
-      TC::put4(sP, row, 16 * jt + 4 * g, p);
-      TC::put4(sB, row, 16 * jt + 4 * g, pb);
+      TC::put4(sP, lc, 16 * it, 16 * jt, p);
+      TC::put4(sB, lc, 16 * it, 16 * jt, pb);
       wi += __shfl_xor(wi, 16);
       wi += __shfl_xor(wi, 32);
-      if (g == 0) rs[jt * C + row] = wi;
+      if (gs == 0) rs[jt * C + row] = wi;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-#pragma unroll
-        for (int m = 1; m < 16; m *= 2) wj[r] += __shfl_xor(wj[r], m);
-        if (i == 0) cs[it * C + 16 * jt + 4 * g + r] = wj[r];
+        wj[r] = kf_row_sum(wj[r]);
+        if (i1 == 0) cs[it * C + 16 * jt + 4 * gs + r] = wj[r];
       }
     }
 
@@ -350,32 +351,35 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
     float cross = 0.f;
 #pragma unroll
     for (int u = 0; u < D / 32; ++u) {
+      __builtin_amdgcn_sched_barrier(0);  // (one depth at a time: all of them at once would not fit the registers)
       KfSplit<A> fs, fr;
       fs.pieces(S0[u][0], S0[u][1]);
       fr.set(R[2 * u], R[2 * u + 1]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) cross += fs.value(e) * R[2 * u + (e >> 2)][e & 3];
-      const F fc = TD::col(sR, 32 * u, 16 * w, i, g);  // rows v of this wave, depth k
+      const F fc = TD::col(sR, lt, 32 * u, 16 * w);  // rows v of this wave, depth k
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
-        dq[t] = fs.mma(TD::row_t(sG, 16 * t + i, 32 * u, g), dq[t]);
-        dk[t] = fr.mma(TD::row_t(sV, 16 * t + i, 32 * u, g), dk[t]);
-        dv[t] = A::mma(fc, TD::row_t(sK, 16 * t + i, 32 * u, g), dv[t]);
+        if (t && t % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+        dq[t] = fs.mma(TD::row_t(sG, lt, 16 * t, 32 * u), dq[t]);
+        dk[t] = fr.mma(TD::row_t(sV, lt, 16 * t, 32 * u), dk[t]);
+        dv[t] = A::mma(fc, TD::row_t(sK, lt, 16 * t, 32 * u), dv[t]);
       }
     }
     load_start(next);
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) cross += __shfl_xor(cross, m);
+    cross = kf_row_sum(cross);
+    cross += __shfl_xor(cross, 16);
+    cross += __shfl_xor(cross, 32);
     if (l == 0) cr[w] = cross;
-    fresh();
+    const int i1 = kf_fresh(i);
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
-      const int tok = 16 * t + i;
+      const int tok = 16 * t + i1;
       const float fi = a.scale * d.from_start[tok], fj = d.to_end[tok];
       dq[t] *= fi;
       dk[t] *= fj;
       dv[t] *= fj;
-      const kf_f32x4 qv = TD::get4(sQ, tok, 16 * w + 4 * g), kv = TD::get4(sK, tok, 16 * w + 4 * g);
+      const kf_f32x4 qv = TD::get4(sQ, lt, 16 * t, 16 * w), kv = TD::get4(sK, lt, 16 * t, 16 * w);
       float x = 0.f, y = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -400,29 +404,34 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
     for (int t = 0; t < NT; ++t) R[t] *= fe;
 #pragma unroll
     for (int u = 0; u < C / 32; ++u) {
-      const F ck = TD::col(sK, 32 * u, 16 * w, i, g), cq = TD::col(sQ, 32 * u, 16 * w, i, g),
-              cg = TD::col(sG, 32 * u, 16 * w, i, g);
+      __builtin_amdgcn_sched_barrier(0);
+      const F ck = TD::col(sK, lt, 32 * u, 16 * w), cq = TD::col(sQ, lt, 32 * u, 16 * w),
+              cg = TD::col(sG, lt, 32 * u, 16 * w);
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
-        if (2 * u <= t) dq[t] = A::mma(ck, TC::row_t(sB, 16 * t + i, 32 * u, g), dq[t]);
+        if (2 * u <= t) dq[t] = A::mma(ck, TC::row_t(sB, lc, 16 * t, 32 * u), dq[t]);
         if (2 * u + 1 >= t) {
-          dk[t] = A::mma(cq, TC::col(sB, 32 * u, 16 * t, i, g), dk[t]);
-          dv[t] = A::mma(cg, TC::col(sP, 32 * u, 16 * t, i, g), dv[t]);
+          dk[t] = A::mma(cq, TC::col(sB, lc, 32 * u, 16 * t), dk[t]);
+          dv[t] = A::mma(cg, TC::col(sP, lc, 32 * u, 16 * t), dv[t]);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
       float wt[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) wt[e] = a.scale * d.from_start[32 * u + 16 * (e >> 2) + 4 * g + (e & 3)];
       KfSplit<A> qw;
       qw.set(cq, wt);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) R[t] = qw.mma_right(TD::col(sG, 32 * u, 16 * t, i, g), R[t]);
+      for (int t = 0; t < NT; ++t) {
+        if (t && t % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+        R[t] = qw.mma_right(TD::col(sG, lt, 32 * u, 16 * t), R[t]);
+      }
     }
-    fresh();
+    const int c4 = 16 * w + 4 * kf_fresh(g);
+    long row = (b * a.T + t0 + kf_fresh(i)) * a.H + h;
 #pragma unroll
-    for (int t = 0; t < CT; ++t) {
-      const long tok = t0 + 16 * t + i, row = (b * a.T + tok) * a.H + h;
-      const int c4 = 16 * w + 4 * g;
+    for (int t = 0; t < CT; ++t, row += 16 * a.H) {
+      const long tok = t0 + 16 * t + i;
       if (tok < a.T) {
         if (tok >= n) dq[t] = dk[t] = dv[t] = kf_f32x4{0, 0, 0, 0};
         kf_store4((T*)a.g_v + row * a.V + c4, dv[t], a.V - c4);

@@ -39,16 +39,8 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
   const int seg = (int)(rest % segs);
   const long b = rest / segs;
   const long bh = b * a.H + h;
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i0 = l & 15, g0 = l >> 4;
-  int i = i0, g = g0;
-  // (fp32 operands take twice the registers: there the LDS addresses are computed anew in each part of the loop -- held across it they
-  // spilled, 39 against 37 us for 5 x 1000 tokens; bf16 has room for them, 46 against 47 us for 4 x 2048)
-  auto fresh = [&]() {
-    if constexpr (std::is_same<A, KfF32>::value) {
-      i = kf_fresh(i0);
-      g = kf_fresh(g0);
-    }
-  };
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i = l & 15, g = l >> 4;
+  const KfLanes lk = TK::lanes(i, g), lv = TV::lanes(i, g);
   const int mt0 = (w % WK) * SM, nt0 = (w / WK) * SN;
   const int v0 = vt * VT, nv = a.V - v0;
   const long n = kf_row_length(a.lengths, b, a.T);
@@ -126,7 +118,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
 #pragma unroll
     for (int m = 0; m < SM; ++m)
 #pragma unroll
-      for (int t = 0; t < SN; ++t) TK::put4(sS, (nt0 + t) * 16 + i, (mt0 + m) * 16 + 4 * g, S[m][t]);
+      for (int t = 0; t < SN; ++t) TK::put4(sS, lk, (nt0 + t) * 16, (mt0 + m) * 16, S[m][t]);
   };
 
   if (c0 < end) {
@@ -139,7 +131,6 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
   }
   for (long c = c0; c < end; ++c) {
     const long t0 = c * KF_CHUNK, next = c + 1 < end ? c + 1 : c;
-    fresh();
     const int last = last_row(c);  // rows behind it are zero
     const bool plain = whole && last == KF_CHUNK - 1;
     if (plain) put(last, std::true_type{});
@@ -172,7 +163,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
           kf_f32x4 s = {0, 0, 0, 0};
           if (jt <= w) {
 #pragma unroll
-            for (int u = 0; u < KK; ++u) s = A::mma(TK::row(sK, 16 * jt + i, 32 * u, g), fq[u], s);
+            for (int u = 0; u < KK; ++u) s = A::mma(TK::row(sK, lk, 16 * jt, 32 * u), fq[u], s);
             if (jt < w) {
               s *= D.from_tile[jt < 3 ? jt : 2][row] * a.scale;
               s *= *reinterpret_cast<const kf_f32x4*>(&D.to_tile_end[16 * jt + 4 * g]);
@@ -193,10 +184,9 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
       auto from_state = [&](int v1) {
         kf_f32x4 o = {0, 0, 0, 0};
 #pragma unroll
-        for (int x = 0; x < KK; ++x) o = A::mma(TK::row(sS, v1 + i, 32 * x, g), fq[x], o);
+        for (int x = 0; x < KK; ++x) o = A::mma(TK::row(sS, lk, v1, 32 * x), fq[x], o);
         return o * fs;
       };
-      fresh();
       KfOut8<T> ready[NT / 2];
       float check = 0.f;
 #pragma unroll
@@ -206,7 +196,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
         for (int y = 0; y < 2; ++y) {
           o[y] = from_state(16 * (u + y));
 #pragma unroll
-          for (int x = 0; x < 2; ++x) o[y] = A::mma(TV::col(sV, 32 * x, 16 * (u + y), i, g), p[x], o[y]);
+          for (int x = 0; x < 2; ++x) o[y] = A::mma(TV::col(sV, lv, 32 * x, 16 * (u + y)), p[x], o[y]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) check = fmaf(o[y][r], 0.f, check);
         }
@@ -228,7 +218,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
           kf_f32x4 o = from_state(v1);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            o = A::mma(A::finite(TV::col(sV, 32 * x, v1, i, g)), p[x], o);
+            o = A::mma(A::finite(TV::col(sV, lv, 32 * x, v1)), p[x], o);
 #pragma unroll 1
             for (int j = 0; j < 32; ++j) {  // token 32 x + j: value e = 4 (j / 16) + j % 4 of lane group (j % 16) / 4
               float pj = 0.f;
@@ -256,7 +246,6 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
     }
 
     // the state at the chunk's end
-    fresh();
     const float fe = D.from_start[KF_CHUNK - 1];
     through *= fe;
 #pragma unroll
@@ -269,11 +258,11 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
       const float wt[8] = {w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]};
       F fv[SN];
 #pragma unroll
-      for (int t = 0; t < SN; ++t) fv[t] = TV::col(sV, 32 * x, 16 * (nt0 + t), i, g);
+      for (int t = 0; t < SN; ++t) fv[t] = TV::col(sV, lv, 32 * x, 16 * (nt0 + t));
 #pragma unroll
       for (int m = 0; m < SM; ++m) {
         KfSplit<A> kw;
-        kw.set(TK::col(sK, 32 * x, 16 * (mt0 + m), i, g), wt);
+        kw.set(TK::col(sK, lk, 32 * x, 16 * (mt0 + m)), wt);
 #pragma unroll
         for (int t = 0; t < SN; ++t) S[m][t] = kw.mma(fv[t], S[m][t]);
       }

@@ -26,6 +26,17 @@ static __device__ __forceinline__ int kf_fresh(int x) {
   return x;
 }
 
+// sums over the 16 lanes of a row, in all of them
+template <int CTRL> static __device__ __forceinline__ float kf_dpp(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+static __device__ __forceinline__ float kf_row_sum(float x) {
+  x += kf_dpp<0x128>(x);  // row_ror 8, 4, 2, 1
+  x += kf_dpp<0x124>(x);
+  x += kf_dpp<0x122>(x);
+  return x + kf_dpp<0x121>(x);
+}
+
 static __device__ __forceinline__ unsigned kf_bits(float x) { return __builtin_bit_cast(unsigned, x); }
 static __device__ __forceinline__ float kf_float_of(unsigned x) { return __builtin_bit_cast(float, x); }
 // two floats rounded to nearest even, packed (v_cvt_pk_bf16_f32)
@@ -76,72 +87,96 @@ struct KfF32 {
 
 // Rows of COLS elements in LDS.  The 16-byte pieces of a row are permuted (by exclusive or) so that each of the reads below meets
 // different banks: 8 rows' pieces at the same depth, and 32 bytes of 4 neighbouring rows, fill the 128 bytes of a cycle.
-template <typename A, int COLS> struct KfTile;
-template <int COLS, int PIECE> struct KfTileAt {
-  static __device__ __forceinline__ int at(int r, int c) {
-    constexpr int PIECES = COLS / PIECE;
-    static_assert(PIECES >= 4, "a row of 64 bytes at least");
+//
+// A lane's part of an address is computed once (KfLanes, in bytes); row, column and depth of the tile come in as constants: whole 8
+// pieces and rows as an offset, the pieces inside 8 by exclusive or.
+struct KfLanes { int row, row_t, col; };
+static __device__ __forceinline__ KfLanes kf_fresh(const KfLanes& x) { return {kf_fresh(x.row), kf_fresh(x.row_t), kf_fresh(x.col)}; }
+template <typename A, int COLS> struct KfTile {
+  typedef typename A::elem E;
+  typedef typename A::frag F;
+  static constexpr int SZ = sizeof(E), PIECE = 16 / SZ, PIECES = COLS / PIECE;
+  static_assert(PIECES >= 4, "a row of 64 bytes at least");
+  static __device__ __forceinline__ int at(int r, int c) {  // element
     const int x = PIECES >= 8 ? ((r & 3) << 1) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1);
     return r * COLS + (((c / PIECE) ^ x) * PIECE) + c % PIECE;
   }
-};
-template <int COLS> struct KfTile<KfBf16, COLS> : KfTileAt<COLS, 8> {
-  typedef KfBf16::elem E;
-  typedef KfBf16::frag F;
-  using KfTileAt<COLS, 8>::at;
-  // operand: row r, depths c .. c + 31 in order C (c a multiple of 32)
-  static __device__ __forceinline__ F row(const E* p, int r, int c, int g) { return *reinterpret_cast<const F*>(p + at(r, c + 8 * g)); }
+  static __device__ __forceinline__ KfLanes lanes(int i, int g) {
+    return {at(i, 8 * g) * SZ, at(i, 4 * g) * SZ, (SZ == 2 ? at(4 * g + (i >> 2), 4 * (i & 3)) : at(4 * g, i)) * SZ};
+  }
+  // byte address of a lane's part at row r (a multiple of 8) and column c (a multiple of what the lanes' parts span)
+  static __device__ __forceinline__ int mix(int lane, int r, int c) {
+    const int p = c / PIECE;
+    return (lane ^ ((p & 7) * 16)) + (p >> 3) * 128 + r * (COLS * SZ);
+  }
+  template <typename X> static __device__ __forceinline__ X read(const E* p, int byte) { return *reinterpret_cast<const X*>(reinterpret_cast<const char*>(p) + byte); }
+  template <typename X> static __device__ __forceinline__ void write(E* p, int byte, X x) { *reinterpret_cast<X*>(reinterpret_cast<char*>(p) + byte) = x; }
+
+  // operand: row r + i, depths c .. c + 31 in order C (c a multiple of 32)
+  static __device__ __forceinline__ F row(const E* p, const KfLanes& L, int r, int c) {
+    const int b = mix(L.row, r, c);
+    if constexpr (SZ == 2) return read<F>(p, b);
+    else return A::from(read<kf_f32x4>(p, b), read<kf_f32x4>(p, b ^ 16));
+  }
   // the same in order T
-  static __device__ __forceinline__ F row_t(const E* p, int r, int c, int g) {
-    const kf_s16x4 x = *reinterpret_cast<const kf_s16x4*>(p + at(r, c + 4 * g)), y = *reinterpret_cast<const kf_s16x4*>(p + at(r, c + 16 + 4 * g));
-    return __builtin_bit_cast(F, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  static __device__ __forceinline__ F row_t(const E* p, const KfLanes& L, int r, int c) {
+    if constexpr (SZ == 2) {
+      const kf_s16x4 x = read<kf_s16x4>(p, mix(L.row_t, r, c)), y = read<kf_s16x4>(p, mix(L.row_t, r, c + 16));
+      return __builtin_bit_cast(F, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      return A::from(read<kf_f32x4>(p, mix(L.row_t, r, c)), read<kf_f32x4>(p, mix(L.row_t, r, c + 16)));
+    }
   }
   // operand: column c + i, depths r .. r + 31 of the rows in order T
-  static __device__ __forceinline__ F col(const E* p, int r, int c, int i, int g) {
-    typedef __attribute__((address_space(3))) kf_s16x4* lds;
-    const int rr = r + 4 * g + (i >> 2), cc = c + 4 * (i & 3);
-    const kf_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(p + at(rr, cc))), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(p + at(rr + 16, cc)));
-    return __builtin_bit_cast(F, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  static __device__ __forceinline__ F col(const E* p, const KfLanes& L, int r, int c) {
+    if constexpr (SZ == 2) {
+      typedef __attribute__((address_space(3))) kf_s16x4* lds;
+      const char* q = reinterpret_cast<const char*>(p);
+      const kf_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(q + mix(L.col, r, c))),
+                     y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(q + mix(L.col, r + 16, c)));
+      return __builtin_bit_cast(F, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      F f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = read<float>(p, (mix(L.col, r, c) ^ (32 * (e & 3))) + (16 * (e >> 2) + (e & 3)) * COLS * SZ);
+      return f;
+    }
   }
-  static __device__ __forceinline__ void put8(E* p, int r, int c, F x) { *reinterpret_cast<F*>(p + at(r, c)) = x; }
+  // four accumulators of row r + i at columns c + 4 g .. + 3 (c a multiple of 16)
+  static __device__ __forceinline__ void put4(E* p, const KfLanes& L, int r, int c, kf_f32x4 x) {
+    if constexpr (SZ == 2) write(p, mix(L.row_t, r, c), make_uint2(kf_pack_bf16(x[0], x[1]), kf_pack_bf16(x[2], x[3])));
+    else write(p, mix(L.row_t, r, c), x);
+  }
+  static __device__ __forceinline__ kf_f32x4 get4(const E* p, const KfLanes& L, int r, int c) {
+    if constexpr (SZ == 2) {
+      const uint2 x = read<uint2>(p, mix(L.row_t, r, c));
+      return kf_f32x4{kf_float_of(x.x << 16), kf_float_of(x.x & 0xffff0000u), kf_float_of(x.y << 16), kf_float_of(x.y & 0xffff0000u)};
+    } else {
+      return read<kf_f32x4>(p, mix(L.row_t, r, c));
+    }
+  }
+  // eight elements of any row r at column c (a multiple of 8)
+  static __device__ __forceinline__ void put8(E* p, int r, int c, F x) {
+    const int b = at(r, c) * SZ;
+    if constexpr (SZ == 2) {
+      write(p, b, x);
+    } else {
+      write(p, b, __builtin_shufflevector(x, x, 0, 1, 2, 3));
+      write(p, b ^ 16, __builtin_shufflevector(x, x, 4, 5, 6, 7));
+    }
+  }
   // with the columns of each 32 so ordered that a lane's four values of two neighbouring 16-wide tiles are 8 neighbours: column
   // 8 a + 4 y + b at 16 y + 4 a + b
   static __device__ __forceinline__ void put8_paired(E* p, int r, int c, F x) {
-    const kf_u32x4 w = __builtin_bit_cast(kf_u32x4, x);
     const int to = (c & ~31) + (c & 31) / 2;
-    *reinterpret_cast<uint2*>(p + at(r, to)) = make_uint2(w[0], w[1]);
-    *reinterpret_cast<uint2*>(p + at(r, to + 16)) = make_uint2(w[2], w[3]);
-  }
-  static __device__ __forceinline__ void put4(E* p, int r, int c, kf_f32x4 x) {
-    *reinterpret_cast<uint2*>(p + at(r, c)) = make_uint2(kf_pack_bf16(x[0], x[1]), kf_pack_bf16(x[2], x[3]));
-  }
-  static __device__ __forceinline__ kf_f32x4 get4(const E* p, int r, int c) {
-    const uint2 x = *reinterpret_cast<const uint2*>(p + at(r, c));
-    return kf_f32x4{kf_float_of(x.x << 16), kf_float_of(x.x & 0xffff0000u), kf_float_of(x.y << 16), kf_float_of(x.y & 0xffff0000u)};
-  }
-};
-template <int COLS> struct KfTile<KfF32, COLS> : KfTileAt<COLS, 4> {
-  typedef KfF32::elem E;
-  typedef KfF32::frag F;
-  using KfTileAt<COLS, 4>::at;
-  static __device__ __forceinline__ kf_f32x4 get4(const E* p, int r, int c) { return *reinterpret_cast<const kf_f32x4*>(p + at(r, c)); }
-  static __device__ __forceinline__ F row(const E* p, int r, int c, int g) { return KfF32::from(get4(p, r, c + 8 * g), get4(p, r, c + 8 * g + 4)); }
-  static __device__ __forceinline__ F row_t(const E* p, int r, int c, int g) { return KfF32::from(get4(p, r, c + 4 * g), get4(p, r, c + 16 + 4 * g)); }
-  static __device__ __forceinline__ F col(const E* p, int r, int c, int i, int g) {
-    F f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = p[at(r + 16 * (e >> 2) + 4 * g + (e & 3), c + i)];
-    return f;
-  }
-  static __device__ __forceinline__ void put4(E* p, int r, int c, kf_f32x4 x) { *reinterpret_cast<kf_f32x4*>(p + at(r, c)) = x; }
-  static __device__ __forceinline__ void put8(E* p, int r, int c, F x) {
-    put4(p, r, c, __builtin_shufflevector(x, x, 0, 1, 2, 3));
-    put4(p, r, c + 4, __builtin_shufflevector(x, x, 4, 5, 6, 7));
-  }
-  static __device__ __forceinline__ void put8_paired(E* p, int r, int c, F x) {
-    const int to = (c & ~31) + (c & 31) / 2;
-    put4(p, r, to, __builtin_shufflevector(x, x, 0, 1, 2, 3));
-    put4(p, r, to + 16, __builtin_shufflevector(x, x, 4, 5, 6, 7));
+    if constexpr (SZ == 2) {
+      const kf_u32x4 w = __builtin_bit_cast(kf_u32x4, x);
+      write(p, at(r, to) * SZ, make_uint2(w[0], w[1]));
+      write(p, at(r, to + 16) * SZ, make_uint2(w[2], w[3]));
+    } else {
+      write(p, at(r, to) * SZ, __builtin_shufflevector(x, x, 0, 1, 2, 3));
+      write(p, at(r, to + 16) * SZ, __builtin_shufflevector(x, x, 4, 5, 6, 7));
+    }
   }
 };
 // the column that stands at place c of such rows
