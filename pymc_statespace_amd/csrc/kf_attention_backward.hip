@@ -24,6 +24,7 @@ struct Split {
   int segments, seg_chunks;
   long chunks;
   float *adds_s, *adds_r, *factors;  // [B H][segments - 1][D D], [B H][segments] (each segment's whole decay)
+  float *products_s, *products_r;    // [B H][segments - 1]: see kf_attention_scan_kernel
   kf_u32x4* starts;                  // S_0 of every chunk: [B H][chunks][D / 32][2][threads]
   float *part_q, *part_k;            // [B][T][H][K], where heads share q and k
   double* part_decay;                // [B H][segments], where decays are fixed
@@ -100,8 +101,9 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
     }
   }
   if (STARTS) {
-    for (int s = 0; s < seg; ++s) {
-      const float f = sp.factors[bh * sp.segments + s];
+    const bool summed = sp.segments > KF_FUSED_SEGMENTS;
+    for (int s = summed && seg ? seg - 1 : 0; s < seg; ++s) {
+      const float f = summed ? sp.products_s[bh * (sp.segments - 1) + s] : sp.factors[bh * sp.segments + s];
       const kf_f32x4* u = reinterpret_cast<const kf_f32x4*>(sp.adds_s) + (bh * (sp.segments - 1) + s) * (D * D / 4) + tid;
 #pragma unroll
       for (int t = 0; t < NT; ++t) acc[t] = acc[t] * f + u[t * TH];
@@ -231,8 +233,9 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
         if (16 * t + 4 * g + r < a.V) R[t][r] = a.g_sT[(bh * a.K + kk) * a.V + 16 * t + 4 * g + r];
     }
   }
-  for (int s = sp.segments - 1; s > seg; --s) {
-    const float f = sp.factors[bh * sp.segments + s];
+  const bool summed = sp.segments > KF_FUSED_SEGMENTS;
+  for (int s = summed && seg + 1 < sp.segments ? seg + 1 : sp.segments - 1; s > seg; --s) {
+    const float f = summed ? sp.products_r[bh * (sp.segments - 1) + s - 1] : sp.factors[bh * sp.segments + s];
     const kf_f32x4* u = reinterpret_cast<const kf_f32x4*>(sp.adds_r) + (bh * (sp.segments - 1) + s - 1) * (D * D / 4) + tid;
 #pragma unroll
     for (int t = 0; t < NT; ++t) R[t] = R[t] * f + u[t * TH];
@@ -518,8 +521,8 @@ struct Plan {
   int D;
   int mode;
   Split sp;
-  size_t adds, factors, starts, part, decay;
-  size_t bytes() const { return 2 * adds + factors + starts + 2 * part + decay; }
+  size_t adds, factors, products, starts, part, decay;
+  size_t bytes() const { return 2 * adds + factors + 2 * products + starts + 2 * part + decay; }
 };
 
 Plan plan(const kf_handle* h, const KfAttnArgs& a) {
@@ -530,12 +533,11 @@ Plan plan(const kf_handle* h, const KfAttnArgs& a) {
   Split& s = p.sp;
   s.chunks = (a.T + C - 1) / C;
   const long rows = a.B * a.H, cu = h->n_cu > 0 ? h->n_cu : 256;
-  // as many workgroups as the card holds at once (by LDS: one on each compute unit for D = 128, more for smaller ones); no segment
-  // under 4 chunks
+  // as many workgroups as the card holds at once (by LDS: one on each compute unit for D = 128, more for smaller ones), where there are
+  // chunks for them (18 heads of 333 tokens in fp32: with at least 4 chunks in a segment 150 us, 2: 93, 1: 65)
   const long room = cu * (p.D == 128 ? 1 : p.D == 64 ? 2 : 4);
   long segs = (room + rows - 1) / rows;
-  segs = segs > 32 ? 32 : segs;
-  segs = segs > s.chunks / 4 ? s.chunks / 4 : segs;
+  segs = segs > s.chunks ? s.chunks : segs;
   segs = segs < 1 ? 1 : segs;
   s.seg_chunks = (int)((s.chunks + segs - 1) / segs);
   s.segments = (int)((s.chunks + s.seg_chunks - 1) / s.seg_chunks);
@@ -543,6 +545,7 @@ Plan plan(const kf_handle* h, const KfAttnArgs& a) {
   const size_t state = (size_t)p.D * p.D * 4;
   p.adds = kf_seq_round(rows * (s.segments - 1) * state);
   p.factors = kf_seq_round((size_t)rows * s.segments * 4);
+  p.products = kf_seq_round((size_t)rows * (s.segments - 1) * 4);
   p.starts = kf_seq_round((size_t)rows * s.chunks * state);
   p.part = a.G != a.H ? kf_seq_round((size_t)a.B * a.T * a.H * a.K * 4) : 0;
   p.decay = a.per_token ? 0 : kf_seq_round((size_t)rows * s.segments * 8);
@@ -560,6 +563,8 @@ int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream)
     Split two = s;
     two.works = 2 * (s.works / s.segments) * (s.segments - 1);
     hipLaunchKernelGGL((attention_sweep_kernel<A, T, D, MODE, false>), dim3(kf_xcd_grid(two.works)), dim3(4 * D), 0, stream, a, two);
+    if (s.segments > KF_FUSED_SEGMENTS)
+      kf_attention_scan(s.adds_s, s.adds_r, s.factors, s.products_s, s.products_r, a.B * a.H, s.segments - 1, (long)D * D, s.segments, stream);
   }
   hipLaunchKernelGGL((attention_sweep_kernel<A, T, D, MODE, true>), dim3(kf_xcd_grid(s.works)), dim3(4 * D), 0, stream, a, s);
   KF_HIP_CHECK(h, hipFuncSetAttribute(reinterpret_cast<const void*>(attention_gradient_kernel<A, T, D, MODE>),
@@ -601,6 +606,8 @@ int kf_launch_attention_backward(kf_handle* h, const KfAttnArgs& a, void* ws, hi
   s.adds_s = (float*)w; w += p.adds;
   s.adds_r = (float*)w; w += p.adds;
   s.factors = (float*)w; w += p.factors;
+  s.products_s = (float*)w; w += p.products;
+  s.products_r = (float*)w; w += p.products;
   s.starts = (kf_u32x4*)w; w += p.starts;
   s.part_q = (float*)w; w += p.part;
   s.part_k = (float*)w; w += p.part;

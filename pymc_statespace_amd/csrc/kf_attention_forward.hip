@@ -14,7 +14,7 @@ namespace {
 // What a chunk needs from memory is asked for one chunk ahead, by loads that no branch surrounds (a load that may or may not have been
 // issued makes every later wait one for all of them): at a segment's end they ask for the last chunk again.
 template <typename A, typename T, int KP, int VT, int MODE, bool OUT>
-__global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, KfAttnSplit sp, float* adds, float* factors) {
+__global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, KfAttnSplit sp, float* adds, float* factors, const float* products) {
   typedef typename A::elem E;
   typedef typename A::frag F;
   typedef KfRow<A, T, MODE> Row;
@@ -72,8 +72,10 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
   // what the segments before this one add, each decayed through those behind it
   const long cell = (bh * (sp.segments - 1)) * sp.v_tiles;
   if (OUT) {
-    for (int s = 0; s < seg; ++s) {
-      const float f = factors[bh * (sp.segments - 1) + s];
+    // (many segments: already summed up, with the products of the decays)
+    const bool summed = sp.segments > KF_FUSED_SEGMENTS;
+    for (int s = summed && seg ? seg - 1 : 0; s < seg; ++s) {
+      const float f = (summed ? products : factors)[bh * (sp.segments - 1) + s];
       const kf_f32x4* u = reinterpret_cast<const kf_f32x4*>(adds) + (cell + (long)s * sp.v_tiles + vt) * (KP * VT / 4) + tid;
 #pragma unroll
       for (int m = 0; m < SM; ++m)
@@ -300,7 +302,7 @@ struct Plan {
   int KP, VT;
   int mode;
   KfAttnSplit sp;
-  size_t adds, bytes;
+  size_t adds, factors, bytes;
 };
 
 Plan plan(const kf_handle* h, const KfAttnArgs& a) {
@@ -313,16 +315,17 @@ Plan plan(const kf_handle* h, const KfAttnArgs& a) {
   s.v_tiles = (a.V + p.VT - 1) / p.VT;
   const long chunks = (a.T + KF_CHUNK - 1) / KF_CHUNK, rows = a.B * a.H * s.v_tiles;
   const long cu = h->n_cu > 0 ? h->n_cu : 256;
-  // two workgroups for each compute unit; no segment under 4 chunks, of which a segment costs the card about one more to combine
+  // two workgroups for each compute unit, where there are chunks for them (5 x 1000 tokens in fp32, 60 tiles of heads: with at least 4
+  // chunks in a segment 53 us, 2: 46 us)
   long segs = (2 * cu + rows - 1) / rows;
-  segs = segs > 32 ? 32 : segs;
-  segs = segs > chunks / 4 ? chunks / 4 : segs;
+  segs = segs > chunks / 2 ? chunks / 2 : segs;
   segs = segs < 1 ? 1 : segs;
   s.seg_chunks = (int)((chunks + segs - 1) / segs);
   s.segments = (int)((chunks + s.seg_chunks - 1) / s.seg_chunks);
   s.works = rows * s.segments;
   p.adds = kf_seq_round((size_t)rows * (s.segments - 1) * p.KP * p.VT * 4);
-  p.bytes = p.adds + kf_seq_round((size_t)a.B * a.H * (s.segments - 1) * 4);
+  p.factors = kf_seq_round((size_t)a.B * a.H * (s.segments - 1) * 4);
+  p.bytes = p.adds + 2 * p.factors;
   return p;
 }
 
@@ -330,12 +333,15 @@ template <typename A, typename T, int KP, int VT, int MODE>
 int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, void* ws, hipStream_t stream) {
   float* adds = (float*)ws;
   float* factors = (float*)((char*)ws + p.adds);
+  float* products = (float*)((char*)factors + p.factors);
   if (p.sp.segments > 1) {
     KfAttnSplit s = p.sp;
     s.works = p.sp.works / p.sp.segments * (p.sp.segments - 1);
-    hipLaunchKernelGGL((attention_chunk_kernel<A, T, KP, VT, MODE, false>), dim3(kf_xcd_grid(s.works)), dim3(256), 0, stream, a, s, adds, factors);
+    hipLaunchKernelGGL((attention_chunk_kernel<A, T, KP, VT, MODE, false>), dim3(kf_xcd_grid(s.works)), dim3(256), 0, stream, a, s, adds, factors, products);
+    if (s.segments > KF_FUSED_SEGMENTS)
+      kf_attention_scan(adds, nullptr, factors, products, nullptr, a.B * a.H, s.segments - 1, (long)s.v_tiles * KP * VT, s.segments - 1, stream);
   }
-  hipLaunchKernelGGL((attention_chunk_kernel<A, T, KP, VT, MODE, true>), dim3(kf_xcd_grid(p.sp.works)), dim3(256), 0, stream, a, p.sp, adds, factors);
+  hipLaunchKernelGGL((attention_chunk_kernel<A, T, KP, VT, MODE, true>), dim3(kf_xcd_grid(p.sp.works)), dim3(256), 0, stream, a, p.sp, adds, factors, products);
   KF_HIP_CHECK(h, hipGetLastError());
   return KF_OK;
 }
