@@ -10,7 +10,7 @@
 // a running sum of q.dq - k.dk over the whole sequence, loses what those sums share).  Then R <- E R + sum_i s e^{G_i} q_i do_i'.
 //
 // Launches: (1) where the time axis is cut into segments, what each segment adds to S and to R; (2) S at every chunk's start, kept
-// in the layout of the operand it becomes; (3) the chunks of each segment from its last to its first, R in registers; (4) sums over
+// as the accumulators that hold it; (3) the chunks of each segment from its last to its first, R in registers; (4) sums over
 // the heads that share queries and keys, and over tokens for fixed decays.
 #include "kf_attention_chunk.h"
 
@@ -25,7 +25,7 @@ struct Split {
   long chunks;
   float *adds_s, *adds_r, *factors;  // [B H][segments - 1][D D], [B H][segments] (each segment's whole decay)
   float *products_s, *products_r;    // [B H][segments - 1]: see kf_attention_scan_kernel
-  kf_u32x4* starts;                  // S_0 of every chunk: [B H][chunks][D / 32][2][threads]
+  kf_f32x4* starts;                  // S_0 of every chunk: [B H][chunks][D / 16][threads]
   float *part_q, *part_k;            // [B][T][H][K], where heads share q and k
   double* part_decay;                // [B H][segments], where decays are fixed
 };
@@ -124,13 +124,11 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
   }
   for (long s = 0; s < steps; ++s) {
     if (STARTS) {
-      kf_u32x4* out = sp.starts + (bh * sp.chunks + at(s)) * (D / 32 * 2 * TH) + tid;
+      kf_f32x4* out = sp.starts + (bh * sp.chunks + at(s)) * (D / 32 * 2 * TH) + tid;
 #pragma unroll
       for (int u = 0; u < D / 32; ++u) {
-        KfSplit<A> f;
-        f.set(acc[2 * u], acc[2 * u + 1]);
-        out[(2 * u) * TH] = f.piece(0);
-        out[(2 * u + 1) * TH] = f.piece(1);
+        out[(2 * u) * TH] = acc[2 * u];
+        out[(2 * u + 1) * TH] = acc[2 * u + 1];
       }
       if (s + 1 == steps && seg == sp.segments - 1) break;  // the state behind the last token is not asked for
     }
@@ -174,7 +172,7 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
 }
 
 template <typename A, typename T, int D, int MODE>
-__global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a, Split sp) {
+__global__ __launch_bounds__(4 * D, 2) void attention_gradient_kernel(KfAttnArgs a, Split sp) {
   constexpr int C = chunk_of<A>(), NT = D / 16, CT = C / 16, TH = 4 * D;
   typedef KfTile<A, D> TD;  // rows of q, k, v, do, R
   typedef KfTile<A, C> TC;  // rows of scores
@@ -264,7 +262,7 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
 
   Stage<C, A, T, D, MODE> rq, rk, rv, rd;
   float rg = 0.f;
-  kf_u32x4 S0[D / 32][2];
+  kf_f32x4 S0[NT];
   auto load = [&](long c) {
     rq.load(q, a.qs[1], c * C, n, a.K);
     rk.load(k, a.ks[1], c * C, n, a.K);
@@ -272,12 +270,9 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
     rd.load(go, a.gs[1], c * C, n, a.V);
   };
   auto load_start = [&](long c) {
-    const kf_u32x4* in = sp.starts + (bh * sp.chunks + c) * (D / 32 * 2 * TH) + tid;
+    const kf_f32x4* in = sp.starts + (bh * sp.chunks + c) * (D / 32 * 2 * TH) + tid;
 #pragma unroll
-    for (int u = 0; u < D / 32; ++u) {
-      S0[u][0] = in[(2 * u) * TH];
-      S0[u][1] = in[(2 * u + 1) * TH];
-    }
+    for (int u = 0; u < NT; ++u) S0[u] = in[u * TH];
   };
   const long ld_step = a.per_token ? a.H : 0;
   auto decay_of = [&](long c) { return ld[(c * C + l < 0 ? 0 : c * C + l < n ? c * C + l : n - 1) * ld_step]; };  // (in bounds for any c)
@@ -356,10 +351,10 @@ __global__ __launch_bounds__(4 * D) void attention_gradient_kernel(KfAttnArgs a,
     for (int u = 0; u < D / 32; ++u) {
       __builtin_amdgcn_sched_barrier(0);  // (one depth at a time: all of them at once would not fit the registers)
       KfSplit<A> fs, fr;
-      fs.pieces(S0[u][0], S0[u][1]);
+      fs.set(S0[2 * u], S0[2 * u + 1]);
       fr.set(R[2 * u], R[2 * u + 1]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) cross += fs.value(e) * R[2 * u + (e >> 2)][e & 3];
+      for (int e = 0; e < 8; ++e) cross += S0[2 * u + (e >> 2)][e & 3] * R[2 * u + (e >> 2)][e & 3];
       const F fc = TD::col(sR, lt, 32 * u, 16 * w);  // rows v of this wave, depth k
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
@@ -608,7 +603,7 @@ int kf_launch_attention_backward(kf_handle* h, const KfAttnArgs& a, void* ws, hi
   s.factors = (float*)w; w += p.factors;
   s.products_s = (float*)w; w += p.products;
   s.products_r = (float*)w; w += p.products;
-  s.starts = (kf_u32x4*)w; w += p.starts;
+  s.starts = (kf_f32x4*)w; w += p.starts;
   s.part_q = (float*)w; w += p.part;
   s.part_k = (float*)w; w += p.part;
   s.part_decay = (double*)w;

@@ -182,12 +182,11 @@ template <typename A, int COLS> struct KfTile {
 // the column that stands at place c of such rows
 static __device__ __forceinline__ int kf_paired(int c) { return (c & ~31) + 8 * ((c >> 2) & 3) + 4 * ((c >> 4) & 1) + (c & 3); }
 
-// fp32 numbers as one operand (accumulators of two 16 x 16 tiles, or a fragment times a weight for each depth): fp32 as they are;
-// bf16 in two rounded parts, 2 x 8 bits and a sign (at most 2^-18 of each value is lost, 7e-7 on average; one part alone would lose
-// 2^-9, far more than the 32 bits that states and their sums are held in), two products.
+// fp32 numbers as one operand (accumulators of two 16 x 16 tiles, or a fragment times a weight for each depth), exactly: fp32 as they
+// are; bf16 cut into three parts of 8 bits each (cut, not rounded: what is left is exact and keeps the sign), three products.  Two parts
+// would leave 2^-18 of each value out and states and their gradients 2.4e-6 off where fp32 sums leave 1.5e-7.
 template <typename A> struct KfSplit;
 template <> struct KfSplit<KfF32> {
-  static constexpr int PARTS = 2;  // 16-byte pieces
   kf_f32x8 p;
   __device__ __forceinline__ void set(kf_f32x4 x, kf_f32x4 y) { p = KfF32::from(x, y); }
   __device__ __forceinline__ void set(kf_f32x8 a, const float (&w)[8]) {
@@ -196,39 +195,38 @@ template <> struct KfSplit<KfF32> {
   }
   __device__ __forceinline__ kf_f32x4 mma(kf_f32x8 b, kf_f32x4 c) const { return KfF32::mma(p, b, c); }
   __device__ __forceinline__ kf_f32x4 mma_right(kf_f32x8 a, kf_f32x4 c) const { return KfF32::mma(a, p, c); }
-  __device__ __forceinline__ float value(int e) const { return p[e]; }
-  __device__ __forceinline__ kf_u32x4 piece(int k) const {
-    return k ? __builtin_bit_cast(kf_u32x4, __builtin_shufflevector(p, p, 4, 5, 6, 7)) : __builtin_bit_cast(kf_u32x4, __builtin_shufflevector(p, p, 0, 1, 2, 3));
-  }
-  __device__ __forceinline__ void pieces(kf_u32x4 x, kf_u32x4 y) { p = KfF32::from(__builtin_bit_cast(kf_f32x4, x), __builtin_bit_cast(kf_f32x4, y)); }
 };
 template <> struct KfSplit<KfBf16> {
-  static constexpr int PARTS = 2;
-  kf_bf16x8 hi, lo;
-  __device__ __forceinline__ void set(kf_f32x4 x, kf_f32x4 y) {
-    hi = KfBf16::from(x, y);
-    kf_f32x4 u, v;
+  kf_bf16x8 p0, p1, p2;
+  static __device__ __forceinline__ kf_bf16x8 high(const float (&x)[8]) {  // the high halves
+    kf_u32x4 r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      u[e] = x[e] - KfBf16::value(hi, e);
-      v[e] = y[e] - KfBf16::value(hi, 4 + e);
-    }
-    lo = KfBf16::from(u, v);
+    for (int e = 0; e < 4; ++e) r[e] = __builtin_amdgcn_perm(kf_bits(x[2 * e + 1]), kf_bits(x[2 * e]), 0x07060302u);
+    return __builtin_bit_cast(kf_bf16x8, r);
+  }
+  static __device__ __forceinline__ void rest(float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] -= kf_float_of(kf_bits(x[e]) & 0xffff0000u);
+  }
+  __device__ __forceinline__ void cut(float (&x)[8]) {
+    p0 = high(x);
+    rest(x);
+    p1 = high(x);
+    rest(x);
+    p2 = high(x);
+  }
+  __device__ __forceinline__ void set(kf_f32x4 x, kf_f32x4 y) {
+    float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    cut(v);
   }
   __device__ __forceinline__ void set(kf_bf16x8 a, const float (&w)[8]) {
-    kf_f32x4 x, y;
+    float v[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[e] = KfBf16::value(a, e) * w[e];
-      y[e] = KfBf16::value(a, 4 + e) * w[4 + e];
-    }
-    set(x, y);
+    for (int e = 0; e < 8; ++e) v[e] = KfBf16::value(a, e) * w[e];
+    cut(v);
   }
-  __device__ __forceinline__ kf_f32x4 mma(kf_bf16x8 b, kf_f32x4 c) const { return KfBf16::mma(hi, b, KfBf16::mma(lo, b, c)); }
-  __device__ __forceinline__ kf_f32x4 mma_right(kf_bf16x8 a, kf_f32x4 c) const { return KfBf16::mma(a, hi, KfBf16::mma(a, lo, c)); }
-  __device__ __forceinline__ float value(int e) const { return KfBf16::value(hi, e) + KfBf16::value(lo, e); }
-  __device__ __forceinline__ kf_u32x4 piece(int k) const { return __builtin_bit_cast(kf_u32x4, k ? lo : hi); }
-  __device__ __forceinline__ void pieces(kf_u32x4 x, kf_u32x4 y) { hi = __builtin_bit_cast(kf_bf16x8, x); lo = __builtin_bit_cast(kf_bf16x8, y); }
+  __device__ __forceinline__ kf_f32x4 mma(kf_bf16x8 b, kf_f32x4 c) const { return KfBf16::mma(p0, b, KfBf16::mma(p1, b, KfBf16::mma(p2, b, c))); }
+  __device__ __forceinline__ kf_f32x4 mma_right(kf_bf16x8 a, kf_f32x4 c) const { return KfBf16::mma(a, p0, KfBf16::mma(a, p1, KfBf16::mma(a, p2, c))); }
 };
 
 // 16 bytes at any element's address (global accesses need no alignment beyond the element's)
