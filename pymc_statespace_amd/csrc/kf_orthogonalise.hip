@@ -398,7 +398,7 @@ struct Product {
   int n, d, L, dP, LP;      // sizes; rows and columns are padded to dP and LP, multiples of 128
   int tiles_m, tiles_n;     // of one matrix's output
   int depth;
-  long works;
+  long works, whole;        // tiles, of which the first `whole` are done by one workgroup each, the others (of 128) by four
   const _Float16 *P, *Q;    // left operand, rows over the depth; right: rows over the depth (GRAM, POLY), or depth x columns (UPDATE)
   const _Float16 *Dh, *Dl;  // what is added: A (POLY), X (UPDATE)
   _Float16 *Ch, *Cl;        // output in parts
@@ -413,29 +413,14 @@ struct Product {
 // 16-byte pieces inside a buffer is permuted by row so that the fragment reads meet different banks.  GRAM and POLY are symmetric:
 // tiles on and below the diagonal, stored twice.
 // PARTS 1: hi parts only, stored apart from the lo parts; 2: hi and lo parts, stored together (`place`).
+constexpr int product_ring(int tile) { return tile == 128 ? 2 : 3; }  // two workgroups (three of the small tiles) fit a compute unit's 160 KB
 template <typename T, int TILE, int PARTS, int MODE, bool LAST>
-__global__ __launch_bounds__(256, 2) void orth_product_kernel(Product p) {
+static __device__ __forceinline__ void product_tile(const Product& p, const long z, const int tm, const int tn, _Float16* const store) {
   constexpr int BK = PARTS == 1 ? 64 : 32;
   constexpr int WT = TILE / 32, PER = TILE * 8 / 256, GR = TILE * PARTS / 16;  // pieces of an operand for each thread; 32-byte groups of a depth's row
   constexpr bool NN = MODE == UPDATE;
-  constexpr int RING = TILE == 128 ? 2 : 3, LOADS = 2 * PER;  // two workgroups (three of the small tiles) fit a compute unit's 160 KB
-  __shared__ __attribute__((aligned(16))) _Float16 lds[RING][2][TILE * 64];
-  const long per = (p.works + 7) >> 3, work = (blockIdx.x & 7) * per + (blockIdx.x >> 3);  // neighbours on one die
-  if (work >= p.works) return;
-  const long tiles = p.works / p.n, z = work / tiles;
-  const int x = (int)(work - z * tiles);
-  int tm, tn;
-  if (MODE == UPDATE) {  // bands of 8 tiles, so that what one die works on shares rows and columns
-    const int width = 8 * p.tiles_n, band = x / width, in = x - band * width;
-    const int rows = p.tiles_m - 8 * band < 8 ? p.tiles_m - 8 * band : 8;
-    tm = 8 * band + in % rows;
-    tn = in / rows;
-  } else {
-    tm = (int)((sqrtf(8.f * x + 1.f) - 1.f) * 0.5f);
-    while ((tm + 1) * (tm + 2) / 2 <= x) ++tm;
-    while (tm * (tm + 1) / 2 > x) --tm;
-    tn = x - tm * (tm + 1) / 2;
-  }
+  constexpr int RING = product_ring(TILE), LOADS = 2 * PER;
+  _Float16 (*const lds)[2][TILE * 64] = reinterpret_cast<_Float16 (*)[2][TILE * 64]>(store);
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, i = l & 15, g = l >> 4;
   const int wm = (w & 1) * (TILE / 2), wn = (w >> 1) * (TILE / 2);
   const long ldP = MODE == GRAM ? p.LP : p.dP, ldQ = MODE == POLY ? p.dP : p.LP;
@@ -526,8 +511,8 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(Product p) {
   // accumulators, 8 bytes of 16 rows at a time: a third of the time of 4 updates of 768 x 2048, 30 us where this takes 22).  Pieces of 4
   // numbers, permuted so that 16 rows written, neighbours read and 8 rows by 8 columns read all meet different banks.
   constexpr int IT = TILE * TILE / 8 / 256;
-  float* tile = reinterpret_cast<float*>(&lds[0][0][0]);
-  static_assert(sizeof(lds) >= TILE * TILE * 4, "");
+  float* tile = reinterpret_cast<float*>(store);
+  static_assert(RING * 2 * 64 * 2 >= TILE * 4, "");
   auto spot = [](int r, int c) { return r * TILE + 4 * ((c >> 2) ^ ((r & 15) ^ ((r >> 3) & 6))) + (c & 3); };
   const int ld = MODE == UPDATE ? p.LP : p.dP;
   const long zC = z * PARTS * (long)p.dP * ld;
@@ -595,6 +580,36 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(Product p) {
   }
 }
 
+template <typename T, int TILE, int PARTS, int MODE, bool LAST>
+__global__ __launch_bounds__(256, 2) void orth_product_kernel(Product p) {
+  __shared__ __attribute__((aligned(16))) _Float16 lds[product_ring(TILE) * 2 * TILE * 64];
+  const long per = (p.whole + 7) >> 3, first = 8 * per;
+  const bool quarter = TILE == 128 && blockIdx.x >= first;
+  const long part = blockIdx.x - first, work = quarter ? p.whole + (part >> 2) : (blockIdx.x & 7) * per + (blockIdx.x >> 3);  // neighbours on one die
+  if (work >= (quarter ? p.works : p.whole)) return;
+  const long tiles = p.works / p.n, z = work / tiles;
+  const int x = (int)(work - z * tiles);
+  int tm, tn;
+  if (MODE == UPDATE) {  // bands of 8 tiles, so that what one die works on shares rows and columns
+    const int width = 8 * p.tiles_n, band = x / width, in = x - band * width;
+    const int rows = p.tiles_m - 8 * band < 8 ? p.tiles_m - 8 * band : 8;
+    tm = 8 * band + in % rows;
+    tn = in / rows;
+  } else {
+    tm = (int)((sqrtf(8.f * x + 1.f) - 1.f) * 0.5f);
+    while ((tm + 1) * (tm + 2) / 2 <= x) ++tm;
+    while (tm * (tm + 1) / 2 > x) --tm;
+    tn = x - tm * (tm + 1) / 2;
+  }
+  if (quarter) {
+    tm = 2 * tm + (int)(part >> 1 & 1);
+    tn = 2 * tn + (int)(part & 1);
+    if (MODE == UPDATE || tn <= tm) product_tile<T, 64, PARTS, MODE, LAST>(p, z, tm, tn, lds);
+  } else {
+    product_tile<T, TILE, PARTS, MODE, LAST>(p, z, tm, tn, lds);
+  }
+}
+
 struct PartsPlan { int dP, LP; size_t x, aa, norm; };
 PartsPlan parts_plan(const KfOrthArgs& a) {
   PartsPlan p;
@@ -621,7 +636,11 @@ void launch_product(const kf_handle* h, Product& p, hipStream_t stream) {
   count(128);
   const bool small = p.works < cu;
   if (small) count(64);
-  const dim3 grid((unsigned)(8 * ((p.works + 7) / 8)));
+  // Two tiles of 128 at a time on each compute unit: a few that are left over would take one more round all by themselves, and are cut
+  // in four (4096 x 4096, 528 tiles on 256 units: 250 us, with the last 16 cut in four 199).
+  const long over = small ? 0 : p.works % (2 * cu);
+  p.whole = p.works > over && 4 * over <= cu ? p.works - over : p.works;
+  const dim3 grid((unsigned)(8 * ((p.whole + 7) / 8) + 4 * (p.works - p.whole)));
   if (small) hipLaunchKernelGGL((orth_product_kernel<T, 64, PARTS, MODE, LAST>), grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL((orth_product_kernel<T, 128, PARTS, MODE, LAST>), grid, dim3(256), 0, stream, p);
 }

@@ -414,6 +414,14 @@ def test_orthogonalise(eng, shape, dtype):
     _check_orth(eng, 1e-2 * rng.standard_normal(shape), dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", [(523, 100, 120), (530, 140, 70)], ids=str)
+def test_orthogonalise_a_few_tiles_over(eng, shape, dtype):
+    """More tiles than the card takes at once, and a few: those are cut in four."""
+    rng = np.random.default_rng(77)
+    _check_orth(eng, rng.standard_normal(shape), dtype)
+
+
 @pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16], ids=str)
 @pytest.mark.parametrize("shape", [(2, 12, 20), (1, 140, 90), (1, 96, 300)], ids=str)
 def test_orthogonalise_of_low_rank(eng, shape, dtype):
