@@ -703,17 +703,21 @@ class KalmanEngine:
 
 
     # ------------------------------------------------------------- sequence layers
-    def _seq(self, x, name, ndim, shape=None, dtype=None):
-        """A sequence operand on this device: last axis contiguous (copied if it is not), any other strides as they are.  Only its
-        address and strides are used, so a tensor that is in place already is taken as it is.  ``shape``: its first axes."""
+    def _seq(self, x, name, ndim, dtype=None, shape=None):
+        """A sequence operand on this device, and its strides: last axis contiguous (copied if it is not), any other strides as they are.
+        Only its address and strides are used, so a tensor that is in place already is taken as it is."""
         t = x if isinstance(x, torch.Tensor) else torch.as_tensor(np.ascontiguousarray(x))
-        if t.ndim != ndim or (shape is not None and t.shape[:len(shape)] != shape):
-            raise ValueError(f"{name}: expected {ndim} axes{'' if shape is None else f', the first {tuple(shape)}'}, got {tuple(t.shape)}")
+        if t.ndim != ndim or (shape is not None and t.shape != shape):
+            raise ValueError(f"{name}: expected {f'{ndim} axes' if shape is None else f'shape {tuple(shape)}'}, got {tuple(t.shape)}")
         if dtype is not None and t.dtype != dtype:
             raise TypeError(f"{name} is {t.dtype}, q is {dtype}: q, k, v and g_o share one type")
         if t.device != self.device:
             t = t.detach().to(self.device)
-        return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and (ndim == 3 or t.stride(1) < 1 << 24) else t.detach().contiguous()
+        strides = t.stride()
+        if (strides[-1] != 1 and t.shape[-1] != 1) or (ndim == 4 and strides[1] >= 1 << 24):
+            t = t.detach().contiguous()
+            strides = t.stride()
+        return t, strides
 
     def _seq_f32(self, x, name, shape):
         """An fp32 operand (log decays, states), contiguous; other types are converted."""
@@ -736,30 +740,31 @@ class KalmanEngine:
             t = t.clamp(-1, 2**31 - 1)
         return t.to(self.device, torch.int32).contiguous()
 
-    def _attention_args(self, q, k, v, log_decay, scale, step=False, g_o=None):
-        ndim = 3 if step else 4
-        q = self._seq(q, "q", ndim)
+    def _attention_args(self, q, k, v, log_decay, scale, g_o=None, ndim=4):
+        """Operands of a linear attention call, checked -> its packed dimensions, (B, H, K, V), and the operands on this device."""
+        q, sq = self._seq(q, "q", ndim)
         dtype, shape = q.dtype, q.shape
         code = _SEQ_DTYPES.get(dtype)
         if not code:
             raise TypeError(f"q is {dtype}: float32, bfloat16 or float16")
-        lead, G, K = shape[:-2], shape[-2], shape[-1]
-        k = self._seq(k, "k", ndim, shape, dtype)
-        v = self._seq(v, "v", ndim, lead, dtype)
-        H, V = v.shape[-2:]
+        k, sk = self._seq(k, "k", ndim, dtype, shape)
+        v, sv = self._seq(v, "v", ndim, dtype)
+        *lead, G, K = shape
+        *v_lead, H, V = v.shape
+        if v_lead != lead:
+            raise ValueError(f"v: expected {ndim} axes, the first {tuple(lead)}, got {tuple(v.shape)}")
         per_token = getattr(log_decay, "ndim", 1) > 1
         g = self._seq_f32(log_decay, "log_decay", (*lead, H) if per_token else (H,))
         if scale is None:
             scale = 1.0 / max(K, 1) ** 0.5
-        if step:
-            strides = [(s[0], 0, s[1]) for s in (q.stride(), k.stride(), v.stride())]
-            return _lib.KfAttentionDims(lead[0], 1, G, H, K, V, code, per_token, scale, *strides), q, k, v, g
-        strides = [s[:3] for s in (q.stride(), k.stride(), v.stride())]
-        d = (*lead, G, H, K, V, code, per_token, scale, *strides)
+        sizes = (lead[0], H, K, V)
+        if ndim == 3:  # one token of each sequence
+            d = _lib.pack_attention_dims(lead[0], 1, G, H, K, V, code, per_token, scale, sq[0], 0, sq[1], sk[0], 0, sk[1], sv[0], 0, sv[1], 0, 0, 0)
+            return d, sizes, q, k, v, g
         if g_o is None:
-            return _lib.KfAttentionDims(*d), q, k, v, g
-        g_o = self._seq(g_o, "g_o", ndim, v.shape, dtype)
-        return _lib.KfAttentionDims(*d, g_o.stride()[:3]), q, k, v, g, g_o
+            return _lib.pack_attention_dims(*lead, G, H, K, V, code, per_token, scale, *sq[:3], *sk[:3], *sv[:3], 0, 0, 0), sizes, q, k, v, g
+        g_o, so = self._seq(g_o, "g_o", ndim, dtype, v.shape)
+        return _lib.pack_attention_dims(*lead, G, H, K, V, code, per_token, scale, *sq[:3], *sk[:3], *sv[:3], *so[:3]), sizes, q, k, v, g, g_o
 
     def _scratch(self, nbytes):
         """Workspace of one call.  From torch's allocator each time: on the current stream, and inside a graph's capture from that
@@ -773,15 +778,15 @@ class KalmanEngine:
         q, k (B,T,G,K), v (B,T,H,V): float32, bfloat16 or float16, one type; head h reads group h // (H // G); K, V <= 128.
         log_decay (B,T,H), or (H,) for fixed decays: fp32, <= 0 (-inf resets the state).  scale: K ** -0.5 by default.
         initial_state (B,H,K,V): what an earlier call left.  lengths (B,): tokens from there on are not read (o is zero there)."""
-        d, q, k, v, g = self._attention_args(q, k, v, log_decay, scale)
-        s0 = self._seq_f32(initial_state, "initial_state", (d.B, d.H, d.K, d.V))
-        lengths = self._seq_i32(lengths, "lengths", d.B)
-        o = torch.empty(v.shape, device=self.device, dtype=q.dtype)
-        state = torch.empty(d.B, d.H, d.K, d.V, device=self.device, dtype=torch.float32)
+        d, sizes, q, k, v, g = self._attention_args(q, k, v, log_decay, scale)
+        s0 = self._seq_f32(initial_state, "initial_state", sizes)
+        lengths = self._seq_i32(lengths, "lengths", sizes[0])
+        o = v.new_empty(v.shape)
+        state = g.new_empty(sizes)
         nbytes = C.c_size_t(0)
-        self._check(self.lib.kf_linear_attention_workspace(self._h, C.byref(d), 0, C.byref(nbytes)), "kf_linear_attention")
+        self._check(self.lib.kf_linear_attention_workspace(self._h, d, 0, C.byref(nbytes)), "kf_linear_attention")
         ws = self._scratch(nbytes)
-        rc = self.lib.kf_linear_attention(self._h, C.byref(d), *_addresses(q, k, v, g, s0, lengths, o, state, ws),
+        rc = self.lib.kf_linear_attention(self._h, d, *_addresses(q, k, v, g, s0, lengths, o, state, ws),
                                           nbytes.value, self._stream())
         self._check(rc, "kf_linear_attention")
         return o, state
@@ -790,18 +795,17 @@ class KalmanEngine:
         """kf_linear_attention_backward: the gradient of <g_o, o> + <g_final_state, state> of ``linear_attention`` on the same
         arguments -> dict(q, k, v, log_decay, initial_state) (initial_state None when none was given); q, k, v in their type,
         the others fp32.  Nothing of the forward call is needed."""
-        d, q, k, v, g, go = self._attention_args(q, k, v, log_decay, scale, g_o=g_o)
-        s0 = self._seq_f32(initial_state, "initial_state", (d.B, d.H, d.K, d.V))
-        gs = self._seq_f32(g_final_state, "g_final_state", (d.B, d.H, d.K, d.V))
-        lengths = self._seq_i32(lengths, "lengths", d.B)
-        out = dict(q=torch.empty(q.shape, device=self.device, dtype=q.dtype), k=torch.empty(k.shape, device=self.device, dtype=q.dtype),
-                   v=torch.empty(v.shape, device=self.device, dtype=q.dtype), log_decay=torch.empty_like(g),
-                   initial_state=None if s0 is None else torch.empty_like(s0))
+        d, sizes, q, k, v, g, go = self._attention_args(q, k, v, log_decay, scale, g_o)
+        s0 = self._seq_f32(initial_state, "initial_state", sizes)
+        gs = self._seq_f32(g_final_state, "g_final_state", sizes)
+        lengths = self._seq_i32(lengths, "lengths", sizes[0])
+        out = dict(q=q.new_empty(q.shape), k=k.new_empty(k.shape), v=v.new_empty(v.shape), log_decay=g.new_empty(g.shape),
+                   initial_state=None if s0 is None else s0.new_empty(sizes))
         nbytes = C.c_size_t(0)
-        self._check(self.lib.kf_linear_attention_workspace(self._h, C.byref(d), 1, C.byref(nbytes)), "kf_linear_attention_backward")
+        self._check(self.lib.kf_linear_attention_workspace(self._h, d, 1, C.byref(nbytes)), "kf_linear_attention_backward")
         ws = self._scratch(nbytes)
         rc = self.lib.kf_linear_attention_backward(
-            self._h, C.byref(d), *_addresses(q, k, v, g, s0, lengths, go, gs, *out.values(), ws), nbytes.value, self._stream())
+            self._h, d, *_addresses(q, k, v, g, s0, lengths, go, gs, *out.values(), ws), nbytes.value, self._stream())
         self._check(rc, "kf_linear_attention_backward")
         return out
 
@@ -810,20 +814,20 @@ class KalmanEngine:
         q, k (B,G,K), v (B,H,V), log_decay (B,H) or (H,); state (N,H,K,V) fp32 is advanced in place, or into ``state_out`` (slots
         that no row names are not touched).  slots (B,): the pool's entry of each row (None: row b has entry b); a negative one is an
         empty row (o zero), one >= N as well, with info 1; rows with the same slot are consecutive tokens of that sequence."""
-        d, q, k, v, g = self._attention_args(q, k, v, log_decay, scale, step=True)
+        d, (B, H, K, V), q, k, v, g = self._attention_args(q, k, v, log_decay, scale, ndim=3)
         N = state.shape[0] if getattr(state, "ndim", 0) else 0
         out = state if state_out is None else state_out
         for name, t in (("state", state), ("state_out", out)):
             if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != self.device or not t.is_contiguous() or \
-                    t.shape != (N, d.H, d.K, d.V):
-                raise ValueError(f"{name} must be a contiguous fp32 tensor (N, {d.H}, {d.K}, {d.V}) on {self.device}: it is used in place")
+                    t.shape != (N, H, K, V):
+                raise ValueError(f"{name} must be a contiguous fp32 tensor (N, {H}, {K}, {V}) on {self.device}: it is used in place")
         here, there = state.data_ptr(), out.data_ptr()
         if here != there and abs(here - there) < 4 * state.numel():
             raise ValueError("state_out overlaps state without being it")
-        slots = self._seq_i32(slots, "slots", d.B)
-        o = torch.empty(v.shape, device=self.device, dtype=q.dtype)
-        info = torch.empty(d.B, device=self.device, dtype=torch.int32)
-        rc = self.lib.kf_linear_attention_step(self._h, C.byref(d), *_addresses(q, k, v, g, slots), N, here, there, *_addresses(o, info),
+        slots = self._seq_i32(slots, "slots", B)
+        o = v.new_empty(v.shape)
+        info = torch.empty(B, device=self.device, dtype=torch.int32)
+        rc = self.lib.kf_linear_attention_step(self._h, d, *_addresses(q, k, v, g, slots), N, here, there, *_addresses(o, info),
                                                self._stream())
         self._check(rc, "kf_linear_attention_step")
         return o, info
@@ -844,7 +848,7 @@ class KalmanEngine:
             t = t.detach().to(self.device).contiguous()
         rows, cols = t.shape[-2:]
         n = t.numel() // (rows * cols)
-        X = torch.empty(t.shape, device=self.device, dtype=t.dtype)
+        X = t.new_empty(t.shape)
         nbytes = C.c_size_t(0)
         self._check(self.lib.kf_orthogonalise_workspace(self._h, n, rows, cols, code, C.byref(nbytes)), "kf_orthogonalise")
         ws = self._scratch(nbytes)
