@@ -492,7 +492,7 @@ enum {
 
 /* Sizes, types and layouts of the kf_linear_attention entry points.  q, k: [B][T][G][K], v: [B][T][H][V]; head h reads the queries
  * and keys of group h / (H / G).  Strides are in elements, for the axes batch, token, head (group) in this order; the last axis is
- * contiguous.  A stride of 0 repeats a row; tokens are less than 2^24 elements apart.  1 <= K, V <= 128, H a multiple of G, B H < 2^31. */
+ * contiguous.  A stride of 0 repeats a row; tokens are less than 2^24 elements apart.  1 <= K, V <= 128, H a multiple of G, B H < 2^22. */
 typedef struct kf_attention_dims {
   int64_t B, T;
   int32_t G, H, K, V;
@@ -508,17 +508,20 @@ KF_API int kf_linear_attention_workspace(kf_handle* h, const kf_attention_dims* 
 
 /* Linear attention with a decay for each head, over whole sequences:
  *     S_t = exp(log_decay_t) S_{t-1} + k_t v_t',   o_t = s S_t' q_t,   S_0 = s0 (NULL: zero)
- * o [B][T][H][V]; sT [B][H][K][V] fp32, the state behind each sequence's last token (may be NULL; may be s0).  log_decay is fp32 and
- * meant to be <= 0; anything below -1e4, -infinity included, is a reset of the state.  lengths [B] int32 (NULL: all T): tokens from
+ * o [B][T][H][V]; sT [B][H][K][V] fp32, the state behind each sequence's last token (may be NULL).  No output overlaps an input or
+ * another output.  log_decay is fp32 and meant to be <= 0 (a positive one is a growth, right while its product over 64 tokens stays in
+ * fp32); anything below -1e4, -infinity included, is a reset of the state.  lengths [B] int32 (NULL: all T): tokens from
  * lengths[b] on (clamped to 0 .. T) are not read, o is zero there and the state stays.  The state, its sums and the decays are held
- * in 32 bits; o is rounded once more than the state where dtype is 16 bits wide (see kf_attention_forward.hip). */
+ * in 32 bits.  For bf16, o is computed from the state and the weighted scores rounded to bf16 (fp16 and fp32: in 32 bits throughout).
+ * An infinity or NaN reaches only the outputs that the formula carries it to, those of its own and later tokens of its head. */
 KF_API int kf_linear_attention(kf_handle* h, const kf_attention_dims* dims, const void* q, const void* k, const void* v,
                                const float* log_decay, const float* s0, const int32_t* lengths, void* o, float* sT,
                                void* workspace, size_t workspace_bytes, void* stream);
 
 /* Its gradient: of <g_o, o> + <g_sT, sT> (g_sT NULL: zero) with respect to q, k, v (contiguous, in dtype; summed over the heads of a
  * group), log_decay (fp32, shaped like it) and s0 (fp32; NULL: not wanted).  Nothing of the forward call is needed.  Rows behind a
- * sequence's end are zero.  The same inputs give the same bits (no atomics). */
+ * sequence's end are zero.  The same inputs give the same bits (no atomics).  An infinity or NaN may make any gradient of its head
+ * not finite. */
 KF_API int kf_linear_attention_backward(kf_handle* h, const kf_attention_dims* dims, const void* q, const void* k, const void* v,
                                         const float* log_decay, const float* s0, const int32_t* lengths, const void* g_o,
                                         const float* g_sT, void* g_q, void* g_k, void* g_v, float* g_log_decay, float* g_s0,

@@ -1578,9 +1578,10 @@ static int attention_args(kf_handle* h, const kf_attention_dims* d, const char* 
     KF_SET_ERR(h, "%s: dtype %d is none of KF_DTYPE_F32, _BF16, _F16", which, d->dtype);
     return KF_ERR_UNSUPPORTED;
   }
-  // (a sequence of 2^31 tokens would not fit the memory in any type; its bound keeps every product of sizes below in 63 bits)
-  if (d->B > 0x7fffffffL / d->H || d->T > 0x7fffffffL || d->B * d->T > (1L << 40) / d->H) {
-    KF_SET_ERR(h, "%s: B=%ld T=%ld H=%d: B H must be below 2^31, B T H below 2^40", which, (long)d->B, (long)d->T, d->H);
+  // (a launch has fewer than 2^32 threads, up to 1024 of them for each head; a sequence of 2^31 tokens would not fit the memory in any
+  // type, and its bound keeps every product of sizes below in 63 bits)
+  if (d->B > ((1L << 22) - 1) / d->H || d->T > 0x7fffffffL || d->B * d->T > (1L << 40) / d->H) {
+    KF_SET_ERR(h, "%s: B=%ld T=%ld H=%d: B H must be below 2^22, B T H below 2^40", which, (long)d->B, (long)d->T, d->H);
     return KF_ERR_UNSUPPORTED;
   }
   if (!(fabs(d->scale) <= 3.0e38)) {
@@ -1618,6 +1619,18 @@ static int workspace_ok(kf_handle* h, const char* which, size_t need, const void
   return KF_OK;
 }
 
+// two buffers of the same size that share memory
+static bool overlapping(const void* a, const void* b, size_t bytes) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return a && b && (x < y ? y - x : x - y) < bytes;
+}
+static int state_apart(kf_handle* h, const char* which, const KfAttnArgs& a, const float* in, const float* out) {
+  // (some workgroups may still read the one when others write the other)
+  if (!overlapping(in, out, (size_t)a.B * a.H * a.K * a.V * 4)) return KF_OK;
+  KF_SET_ERR(h, "%s: the state that is written overlaps the one that is read", which);
+  return KF_ERR_ARG;
+}
+
 extern "C" int kf_linear_attention_workspace(kf_handle* h, const kf_attention_dims* dims, int backward, size_t* bytes) {
   KfAttnArgs a;
   const int rc = attention_args(h, dims, "kf_linear_attention_workspace", &a);
@@ -1641,6 +1654,7 @@ extern "C" int kf_linear_attention(kf_handle* h, const kf_attention_dims* dims, 
     return KF_ERR_ARG;
   }
   rc = workspace_ok(h, "kf_linear_attention", kf_attention_forward_workspace(h, a), workspace, workspace_bytes);
+  if (!rc) rc = state_apart(h, "kf_linear_attention", a, s0, sT);
   if (rc) return rc;
   KF_ON_DEVICE(h);
   a.q = q; a.k = k; a.v = v; a.log_decay = log_decay; a.s0 = s0; a.lengths = lengths; a.o = o; a.sT = sT;
@@ -1667,6 +1681,8 @@ extern "C" int kf_linear_attention_backward(kf_handle* h, const kf_attention_dim
     return KF_ERR_UNSUPPORTED;
   }
   rc = workspace_ok(h, "kf_linear_attention_backward", kf_attention_backward_workspace(h, a), workspace, workspace_bytes);
+  if (!rc) rc = state_apart(h, "kf_linear_attention_backward", a, s0, g_s0);
+  if (!rc) rc = state_apart(h, "kf_linear_attention_backward", a, g_sT, g_s0);
   if (rc) return rc;
   KF_ON_DEVICE(h);
   a.q = q; a.k = k; a.v = v; a.log_decay = log_decay; a.s0 = s0; a.lengths = lengths; a.g_o = g_o; a.g_sT = g_sT;
@@ -1694,6 +1710,10 @@ extern "C" int kf_linear_attention_step(kf_handle* h, const kf_attention_dims* d
     KF_SET_ERR(h, "kf_linear_attention_step: n_slots=%ld for B=%ld rows%s", (long)n_slots, (long)c.B, slots ? "" : " without slots");
     return KF_ERR_ARG;
   }
+  if (state != state_out && overlapping(state, state_out, (size_t)n_slots * c.H * c.K * c.V * 4)) {
+    KF_SET_ERR(h, "kf_linear_attention_step: state_out overlaps state without being it");
+    return KF_ERR_ARG;
+  }
   KF_ON_DEVICE(h);
   KfAttnStepArgs a;
   a.B = c.B; a.n_slots = n_slots; a.G = c.G; a.H = c.H; a.K = c.K; a.V = c.V; a.dtype = c.dtype; a.per_row = c.per_token; a.scale = c.scale;
@@ -1709,7 +1729,7 @@ static int orthogonalise_args(kf_handle* h, int64_t n, int32_t rows, int32_t col
     return KF_ERR_ARG;
   }
   if (n > 65535 * 64L || rows > (1 << 17) || cols > (1 << 24) || (rows > cols && (rows > (1 << 24) || cols > (1 << 17))) ||
-      (double)n * rows * cols > 4.0e11) {
+      (int64_t)rows * cols > 1L << 31 || (double)n * rows * cols > 4.0e11) {
     KF_SET_ERR(h, "%s: n=%ld rows=%d cols=%d is too large", which, (long)n, rows, cols);
     return KF_ERR_UNSUPPORTED;
   }
@@ -1767,7 +1787,8 @@ extern "C" int kf_orthogonalise(kf_handle* h, int64_t n, int32_t rows, int32_t c
   KfOrthArgs a;
   int rc = orthogonalise_args(h, n, rows, cols, dtype, "kf_orthogonalise", &a);
   if (rc) return rc;
-  if (n_steps < 1 || n_steps > KF_ORTHOGONALISE_STEPS_MAX || !coefficients || !M || !X || M == X || !(eps >= 0.0 && eps < 1e300)) {
+  const size_t bytes = (size_t)n * rows * cols * (dtype == KF_DTYPE_F64 ? 8 : dtype == KF_DTYPE_F32 ? 4 : 2);
+  if (n_steps < 1 || n_steps > KF_ORTHOGONALISE_STEPS_MAX || !coefficients || !M || !X || overlapping(M, X, bytes) || !(eps >= 0.0 && eps < 1e300)) {
     KF_SET_ERR(h, "kf_orthogonalise: needs 1 <= n_steps <= %d, coefficients, M, X apart from M, and a finite eps >= 0",
                KF_ORTHOGONALISE_STEPS_MAX);
     return KF_ERR_ARG;

@@ -130,7 +130,7 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
         out[(2 * u) * TH] = acc[2 * u];
         out[(2 * u + 1) * TH] = acc[2 * u + 1];
       }
-      if (s + 1 == steps && seg == sp.segments - 1) break;  // the state behind the last token is not asked for
+      if (s + 1 == steps) break;  // (the next segment starts from what was summed up for it)
     }
     rx.put(sX, at(s) * C, n, a.K);
     ry.put(sY, at(s) * C, n, a.V);
@@ -490,16 +490,17 @@ __global__ __launch_bounds__(4 * D, 2) void attention_gradient_kernel(KfAttnArgs
 // sums a group's heads into the type of q / k
 template <typename T>
 __global__ __launch_bounds__(256) void attention_group_kernel(KfAttnArgs a, const float* part_q, const float* part_k) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
   const long total = a.B * a.T * a.G * a.K;
-  if (i >= total) return;
   const float* part = blockIdx.y ? part_k : part_q;
-  const int c = (int)(i % a.K);
-  const long row = i / a.K, bt = row / a.G;
-  const int g = (int)(row - bt * a.G), per = a.H / a.G;
-  float s = 0.f;
-  for (int j = 0; j < per; ++j) s += part[(bt * a.H + g * per + j) * a.K + c];
-  ((T*)(blockIdx.y ? a.g_k : a.g_q))[i] = kf_from_float<T>(s);
+  const int per = a.H / a.G;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256l) {
+    const int c = (int)(i % a.K);
+    const long row = i / a.K, bt = row / a.G;
+    const int g = (int)(row - bt * a.G);
+    float s = 0.f;
+    for (int j = 0; j < per; ++j) s += part[(bt * a.H + g * per + j) * a.K + c];
+    ((T*)(blockIdx.y ? a.g_k : a.g_q))[i] = kf_from_float<T>(s);
+  }
 }
 
 // fixed decays: sums over sequences and segments, one wave for each head
@@ -566,8 +567,8 @@ int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream)
                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   hipLaunchKernelGGL((attention_gradient_kernel<A, T, D, MODE>), dim3(kf_xcd_grid(s.works)), dim3(4 * D), lds, stream, a, s);
   if (a.G != a.H) {
-    const long total = a.B * a.T * a.G * a.K;
-    hipLaunchKernelGGL(attention_group_kernel<T>, dim3((unsigned)((total + 255) / 256), 2), dim3(256), 0, stream, a, s.part_q, s.part_k);
+    const long blocks = (a.B * a.T * a.G * a.K + 255) / 256;
+    hipLaunchKernelGGL(attention_group_kernel<T>, dim3((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20), 2), dim3(256), 0, stream, a, s.part_q, s.part_k);
   }
   if (!a.per_token) hipLaunchKernelGGL(attention_decay_kernel, dim3(a.H), dim3(64), 0, stream, a, s.part_decay, s.segments);
   KF_HIP_CHECK(h, hipGetLastError());

@@ -45,8 +45,7 @@ struct KfChunkDecay {
       to_tile_end[l] = __expf((float)((row == 0 ? end[0] : row == 1 ? end[1] : row == 2 ? end[2] : end[3]) - G));
 #pragma unroll
       for (int t = 0; t < C / 16 - 1; ++t) {
-        const float d = (float)(G - end[t]);
-        from_tile[t][l] = __expf(d > 0.f ? 0.f : d);  // (a NaN stays one)
+        from_tile[t][l] = row > t ? __expf((float)(G - end[t])) : 0.f;
       }
       hi[l] = (float)G;
       lo[l] = (float)(G - (double)hi[l]);

@@ -17,7 +17,7 @@ __global__ __launch_bounds__(TH) void attention_step_kernel(KfAttnStepArgs a) {
   typedef typename Vec<VEC>::type W;
   constexpr int RP = TH / LV, PASSES = MAXD / RP > 0 ? MAXD / RP : 1;
   __shared__ float sq[MAXD], sk[MAXD];
-  __shared__ float red[TH / 64][LV * VEC];
+  __shared__ __attribute__((aligned(16))) float red[TH / 64][LV * VEC];
   const long b0 = blockIdx.x / a.H;
   const int h = (int)(blockIdx.x - b0 * a.H), g = h / (a.H / a.G);
   const int tid = threadIdx.x, c = (tid % LV) * VEC, r0 = tid / LV;

@@ -177,6 +177,24 @@ def test_a_long_sequence(eng, dtype):
     _check_backward(eng, p, TYPES[dtype])
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(1, 1100, 2, 2, 5, 70), (1, 1100, 1, 3, 77, 3)], ids=str)
+def test_long_and_narrow(eng, shape, dtype):
+    """Rows shorter than 16 bytes, over many segments."""
+    p = _make(15, *shape, TYPES[dtype])
+    _check_forward(eng, p, TYPES[dtype])
+    _check_backward(eng, p, TYPES[dtype])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_decays_that_grow(eng, dtype):
+    """Positive log decays are a growth, as the recurrence has it."""
+    p = _make(16, 2, 200, 1, 2, 24, 40, TYPES[dtype])
+    p["log_decay"] = np.random.default_rng(17).uniform(-0.05, 0.04, p["log_decay"].shape).astype(np.float32).astype(np.float64)
+    _check_forward(eng, p, TYPES[dtype])
+    _check_backward(eng, p, TYPES[dtype])
+
+
 def test_no_decay_at_all(eng):
     """log_decay = 0: a plain running sum, the state grows with the length."""
     p = _make(6, 1, 700, 1, 1, 16, 16, torch.float32)

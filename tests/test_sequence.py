@@ -91,7 +91,7 @@ def _dims(**kw):
     (dict(K=129), -4), (dict(V=200), -4), (dict(dtype=0), -4), (dict(dtype=7), -4), (dict(scale=float("nan")), -1),
     (dict(scale=float("inf")), -1), (dict(scale=1e39), -1), (dict(B=2**31), -4), (dict(T=2**31), -4), (dict(B=2**30, H=4), -4),
     (dict(q_stride=(0, -1, 0)), -1), (dict(k_stride=(-8, 8, 8)), -1), (dict(v_stride=(8, 8, -8)), -1),
-    (dict(k_stride=(0, 1 << 24, 0)), -4)])
+    (dict(k_stride=(0, 1 << 24, 0)), -4), (dict(B=2**21), -4)])
 def test_sizes_that_are_refused(lib, handle, bad, rc):
     d, n, one = _dims(**bad), C.c_size_t(), C.c_void_p(16)
     assert lib.kf_linear_attention_workspace(handle, C.byref(d), 0, C.byref(n)) == rc
@@ -124,9 +124,27 @@ def test_pointers_and_workspaces_that_are_refused(lib, handle):
         assert lib.kf_linear_attention_step(handle, C.byref(_dims(B=2)), one, one, one, one, slots, count, *[one] * 4, None) == -1
 
 
+def test_buffers_that_share_memory_are_refused(lib, handle):
+    d, one, far = _dims(), C.c_void_p(1 << 12), C.c_void_p(1 << 30)
+    state = 2 * 8 * 8 * 4  # bytes, of _dims()
+    for off in (0, 4, state - 4, 4 - state):
+        near = C.c_void_p((1 << 30) + off)
+        assert lib.kf_linear_attention(handle, C.byref(d), one, one, one, one, far, None, one, near, one, 1 << 30, None) == -1
+        assert b"overlaps" in lib.kf_last_error(handle)
+        for s0, gs in ((far, None), (None, far)):
+            assert lib.kf_linear_attention_backward(handle, C.byref(d), one, one, one, one, s0, None, one, gs, *[one] * 4, near, one, 1 << 30, None) == -1
+            assert b"overlaps" in lib.kf_last_error(handle)
+        if off:
+            assert lib.kf_linear_attention_step(handle, C.byref(d), one, one, one, one, None, 1, far, near, one, one, None) == -1
+            assert b"overlaps" in lib.kf_last_error(handle)
+    coef = (C.c_double * 3)(1.5, -0.5, 0.0)
+    for off in (0, 2, 5 * 96 * 96 * 2 - 2):
+        assert lib.kf_orthogonalise(handle, 5, 96, 96, 2, 1, coef, 1e-7, far, C.c_void_p((1 << 30) + off), one, 1 << 40, None) == -1
+
+
 @pytest.mark.parametrize("n, rows, cols, dtype, rc", [
     (0, 4, 4, 1, -1), (1, 0, 4, 1, -1), (1, 4, -1, 1, -1), (1, 4, 4, 4, -4), (1, 4, 4, -1, -4), (1, 1 << 18, 1 << 18, 1, -4),
-    (1 << 40, 4, 4, 1, -4), (4, 1 << 17, 1 << 24, 1, -4), (65536, 80, 80, 1, -4)])
+    (1 << 40, 4, 4, 1, -4), (4, 1 << 17, 1 << 24, 1, -4), (1, 1 << 16, (1 << 15) + 1, 0, -4), (65536, 80, 80, 1, -4)])
 def test_matrices_that_are_refused(lib, handle, n, rows, cols, dtype, rc):
     size, one = C.c_size_t(), C.c_void_p(16)
     coef = (C.c_double * 3)(1.5, -0.5, 0.0)
