@@ -77,6 +77,8 @@ _SEQ_DTYPES = {torch.float64: 0, torch.float32: 1, torch.bfloat16: 2, torch.floa
 def _newton_schulz(coefficients, steps):
     """(number of steps, double[steps][3]) of ``KalmanEngine.orthogonalise``'s arguments."""
     most = _lib.KF_ORTHOGONALISE_STEPS_MAX
+    if type(coefficients) is tuple and len(coefficients) == 3 and type(coefficients[0]) is float and type(steps) is int and 1 <= steps <= most:
+        return steps, (C.c_double * (3 * steps))(*(coefficients * steps))  # (as below, without numpy's 3 us)
     c = np.asarray(coefficients, dtype=np.float64)
     if c.shape == (3,):
         if not 1 <= int(steps) <= most:
@@ -186,7 +188,8 @@ class KalmanEngine:
         self.__dict__.pop("_ws", None)
 
     def _stream(self):
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        # (torch.cuda.current_stream(device).cuda_stream without the Stream object around it: 2 us of calls that take about 12)
+        return C.c_void_p(torch._C._cuda_getCurrentRawStream(self.device.index))
 
     def to_device(self, x, shape=None):
         if x is None:
@@ -781,7 +784,7 @@ class KalmanEngine:
         d, sizes, q, k, v, g = self._attention_args(q, k, v, log_decay, scale)
         s0 = self._seq_f32(initial_state, "initial_state", sizes)
         lengths = self._seq_i32(lengths, "lengths", sizes[0])
-        o = v.new_empty(v.shape)
+        o = torch.empty_like(v, memory_format=torch.contiguous_format)
         state = g.new_empty(sizes)
         nbytes = C.c_size_t(0)
         self._check(self.lib.kf_linear_attention_workspace(self._h, d, 0, C.byref(nbytes)), "kf_linear_attention")
@@ -799,8 +802,8 @@ class KalmanEngine:
         s0 = self._seq_f32(initial_state, "initial_state", sizes)
         gs = self._seq_f32(g_final_state, "g_final_state", sizes)
         lengths = self._seq_i32(lengths, "lengths", sizes[0])
-        out = dict(q=q.new_empty(q.shape), k=k.new_empty(k.shape), v=v.new_empty(v.shape), log_decay=g.new_empty(g.shape),
-                   initial_state=None if s0 is None else s0.new_empty(sizes))
+        out = {n: None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
+               for n, t in (("q", q), ("k", k), ("v", v), ("log_decay", g), ("initial_state", s0))}
         nbytes = C.c_size_t(0)
         self._check(self.lib.kf_linear_attention_workspace(self._h, d, 1, C.byref(nbytes)), "kf_linear_attention_backward")
         ws = self._scratch(nbytes)
@@ -825,7 +828,7 @@ class KalmanEngine:
         if here != there and abs(here - there) < 4 * state.numel():
             raise ValueError("state_out overlaps state without being it")
         slots = self._seq_i32(slots, "slots", B)
-        o = v.new_empty(v.shape)
+        o = torch.empty_like(v, memory_format=torch.contiguous_format)
         info = torch.empty(B, device=self.device, dtype=torch.int32)
         rc = self.lib.kf_linear_attention_step(self._h, d, *_addresses(q, k, v, g, slots), N, here, there, *_addresses(o, info),
                                                self._stream())
@@ -848,7 +851,7 @@ class KalmanEngine:
             t = t.detach().to(self.device).contiguous()
         rows, cols = t.shape[-2:]
         n = t.numel() // (rows * cols)
-        X = t.new_empty(t.shape)
+        X = torch.empty_like(t, memory_format=torch.contiguous_format)
         nbytes = C.c_size_t(0)
         self._check(self.lib.kf_orthogonalise_workspace(self._h, n, rows, cols, code, C.byref(nbytes)), "kf_orthogonalise")
         ws = self._scratch(nbytes)
