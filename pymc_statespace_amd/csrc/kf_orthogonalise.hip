@@ -43,22 +43,25 @@ template <typename X> static __device__ __forceinline__ X block_sum(X s, X* red)
 
 // ------------------------------------------------------------------------------------- in the registers of one wave
 // d <= 16, L <= 16 NT.  Tiles of 16 x 16 as v_mfma_*_16x16x4 leave them: lane (g, c) holds column c of rows r(s, g), s = 0 .. 3.
-// The same registers are the right operand of a product that runs over those rows, and the left operand's transpose.  X is kept in
-// both orientations, x = X, y = X': A = y'y, A A and B X = (B)'x, X'B = (x)'B then need no other lane's values.
+// The same registers are the right operand of a product that runs over those rows, and the left operand's transpose: with y = X' (X's
+// tiles transposed through LDS once a step), A = y'y, A A and B X = (B)'x need no other lane's values.  The fp64 instructions' 64 cycles
+// bound it (each SIMD has four matrices of 4096): four of them only where the depth is above 12 (4096 matrices of 10 x 10: 14 us with
+// four each time and X' by a product of its own, 10 now).
 template <typename C> struct Tile;
 template <> struct Tile<double> {
   typedef double type __attribute__((ext_vector_type(4)));
   static __device__ __forceinline__ int row(int s, int g) { return 4 * s + g; }
-  static __device__ __forceinline__ type mma(type a, type b, type c) {
+  static __device__ __forceinline__ type mma(type a, type b, type c, int depth) {  // (step s: depths 4 s .. 4 s + 3)
 #pragma unroll
-    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s], b[s], c, 0, 0, 0);
+    for (int s = 0; s < 4; ++s)
+      if (4 * s < depth) c = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s], b[s], c, 0, 0, 0);
     return c;
   }
 };
 template <> struct Tile<float> {
   typedef f4 type;
   static __device__ __forceinline__ int row(int s, int g) { return 4 * g + s; }
-  static __device__ __forceinline__ type mma(type a, type b, type c) {
+  static __device__ __forceinline__ type mma(type a, type b, type c, int) {  // (step s: depths s, 4 + s, 8 + s, 12 + s)
 #pragma unroll
     for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
     return c;
@@ -70,6 +73,7 @@ __global__ __launch_bounds__(256) void orth_wave_kernel(KfOrthArgs a) {
   typedef typename Acc<T>::type C;
   typedef Tile<C> Q;
   typedef typename Q::type V;
+  __shared__ C turn[4][16][17];  // one tile for each wave; 17: rows and columns meet different banks
   const long z = blockIdx.x * 4l + (threadIdx.x >> 6);
   if (z >= a.n) return;
   const int l = threadIdx.x & 63, g = l >> 4, c = l & 15;
@@ -77,7 +81,7 @@ __global__ __launch_bounds__(256) void orth_wave_kernel(KfOrthArgs a) {
   const int d = tall ? a.cols : a.rows, L = tall ? a.rows : a.cols;
   const int sr = tall ? 1 : a.cols, sc = tall ? a.cols : 1;  // strides of X's rows and columns in M
   const T* M = (const T*)a.M + z * d * L;
-  V x[NT], y[NT];
+  V x[NT];
   double sum = 0.;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -85,7 +89,6 @@ __global__ __launch_bounds__(256) void orth_wave_kernel(KfOrthArgs a) {
     for (int s = 0; s < 4; ++s) {
       const int r = Q::row(s, g);
       x[t][s] = r < d && 16 * t + c < L ? to_acc(M[r * sr + (16 * t + c) * sc]) : C(0);
-      y[t][s] = c < d && 16 * t + r < L ? to_acc(M[c * sr + (16 * t + r) * sc]) : C(0);
       sum += (double)x[t][s] * (double)x[t][s];
     }
 #pragma unroll
@@ -94,23 +97,27 @@ __global__ __launch_bounds__(256) void orth_wave_kernel(KfOrthArgs a) {
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      x[t][s] = (C)((double)x[t][s] * f);
-      y[t][s] = (C)((double)y[t][s] * f);
-    }
+    for (int s = 0; s < 4; ++s) x[t][s] = (C)((double)x[t][s] * f);
+  C(*const tile)[17] = turn[threadIdx.x >> 6];
   const V zero = {C(0), C(0), C(0), C(0)};
   for (int step = 0; step < a.steps; ++step) {
     const C ca = (C)a.coef[step][0], cb = (C)a.coef[step][1], cc = (C)a.coef[step][2];
     V A = zero;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) A = Q::mma(y[t], y[t], A);
-    const V B = cb * A + cc * Q::mma(A, A, zero);
-#pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const V u = ca * x[t], v = ca * y[t];
-      y[t] = Q::mma(x[t], B, v);
-      x[t] = Q::mma(B, x[t], u);
+      // (a wave's LDS operations are done in their order; the fences, which cost no instruction, keep the compiler to it)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int s = 0; s < 4; ++s) tile[Q::row(s, g)][c] = x[t][s];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      V y;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) y[s] = tile[c][Q::row(s, g)];
+      A = Q::mma(y, y, A, L - 16 * t);
     }
+    const V B = cb * A + cc * Q::mma(A, A, zero, d);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) x[t] = Q::mma(B, x[t], ca * x[t], d);
   }
   T* out = (T*)a.X + z * d * L;
 #pragma unroll
