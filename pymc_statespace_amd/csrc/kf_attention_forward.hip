@@ -310,6 +310,8 @@ Plan plan(const kf_handle* h, const KfAttnArgs& a) {
   p.mode = kf_rows_mode(a.K, a.V);
   const bool narrow = p.mode == KF_ROWS_NARROW;  // one kernel, of the largest K
   p.KP = narrow ? 128 : a.K <= 32 ? 32 : a.K <= 64 ? 64 : 128;
+  // (128 columns at a time would take scores and weighted keys once for each head, but need all 256 registers and twice as many
+  // segments: 4 x 2048 tokens, V = 128, 52 us instead of 48)
   p.VT = a.dtype == KF_DTYPE_BF16 && a.V > 32 && !narrow ? 64 : 32;
   KfAttnSplit& s = p.sp;
   s.v_tiles = (a.V + p.VT - 1) / p.VT;

@@ -85,11 +85,13 @@ struct KfF32 {
   static __device__ __forceinline__ float get(const elem* p) { return *p; }
 };
 
-// Rows of COLS elements in LDS.  The 16-byte pieces of a row are permuted (by exclusive or) so that each of the reads below meets
-// different banks: 8 rows' pieces at the same depth, and 32 bytes of 4 neighbouring rows, fill the 128 bytes of a cycle.
+// Rows of COLS elements in LDS, 64 banks of 4 bytes.  The 16-byte pieces of a row are permuted (by exclusive or) so that what is read
+// or written at a time meets different banks: a piece of 16 neighbouring rows, of which rows 4 to 11 read the next lane group's depth
+// (16-byte reads take the lanes in that order: measured by their conflicts); 32 bytes of 8 rows (16-bit columns); 64 bytes of every
+// fourth row (32-bit columns; rows of 128 bytes meet the same half of the banks there, two cycles).
 //
-// A lane's part of an address is computed once (KfLanes, in bytes); row, column and depth of the tile come in as constants: whole 8
-// pieces and rows as an offset, the pieces inside 8 by exclusive or.
+// A lane's part of an address is computed once (KfLanes, in bytes); row, column and depth of the tile come in as constants: rows (a
+// multiple of 16) and whole 16 pieces as an offset, the pieces inside 16 by exclusive or.
 struct KfLanes { int row, row_t, col; };
 static __device__ __forceinline__ KfLanes kf_fresh(const KfLanes& x) { return {kf_fresh(x.row), kf_fresh(x.row_t), kf_fresh(x.col)}; }
 template <typename A, int COLS> struct KfTile {
@@ -97,17 +99,21 @@ template <typename A, int COLS> struct KfTile {
   typedef typename A::frag F;
   static constexpr int SZ = sizeof(E), PIECE = 16 / SZ, PIECES = COLS / PIECE;
   static_assert(PIECES >= 4, "a row of 64 bytes at least");
+  static constexpr int turn(int r) {
+    const int b1 = (r >> 1) & 1, b2 = (r >> 2) & 1, b3 = (r >> 3) & 1;
+    if (SZ == 4) return PIECES >= 16 ? r & 15 : (b2 ^ b3) * 4 + b3 * 2 + b1;
+    return PIECES >= 16 ? (b2 ^ b3) * 8 + (r & 3) * 2 + b3 : PIECES == 8 ? (b2 ^ b3) * 4 + b1 * 2 + b3 : (b2 ^ b3) * 2 + b3;
+  }
   static __device__ __forceinline__ int at(int r, int c) {  // element
-    const int x = PIECES >= 8 ? ((r & 3) << 1) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1);
-    return r * COLS + (((c / PIECE) ^ x) * PIECE) + c % PIECE;
+    return r * COLS + (((c / PIECE) ^ turn(r)) * PIECE) + c % PIECE;
   }
   static __device__ __forceinline__ KfLanes lanes(int i, int g) {
     return {at(i, 8 * g) * SZ, at(i, 4 * g) * SZ, (SZ == 2 ? at(4 * g + (i >> 2), 4 * (i & 3)) : at(4 * g, i)) * SZ};
   }
-  // byte address of a lane's part at row r (a multiple of 8) and column c (a multiple of what the lanes' parts span)
+  // byte address of a lane's part at row r (a multiple of 16) and column c (a multiple of what the lanes' parts span)
   static __device__ __forceinline__ int mix(int lane, int r, int c) {
     const int p = c / PIECE;
-    return (lane ^ ((p & 7) * 16)) + (p >> 3) * 128 + r * (COLS * SZ);
+    return (lane ^ ((p & 15) * 16)) + (p >> 4) * 256 + r * (COLS * SZ);
   }
   template <typename X> static __device__ __forceinline__ X read(const E* p, int byte) { return *reinterpret_cast<const X*>(reinterpret_cast<const char*>(p) + byte); }
   template <typename X> static __device__ __forceinline__ void write(E* p, int byte, X x) { *reinterpret_cast<X*>(reinterpret_cast<char*>(p) + byte) = x; }
@@ -138,7 +144,7 @@ template <typename A, int COLS> struct KfTile {
     } else {
       F f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = read<float>(p, (mix(L.col, r, c) ^ (32 * (e & 3))) + (16 * (e >> 2) + (e & 3)) * COLS * SZ);
+      for (int e = 0; e < 8; ++e) f[e] = read<float>(p, (mix(L.col, r, c) ^ (16 * turn(e & 3))) + (16 * (e >> 2) + (e & 3)) * COLS * SZ);
       return f;
     }
   }
