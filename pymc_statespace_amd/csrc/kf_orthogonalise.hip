@@ -303,7 +303,7 @@ int launch_chip(kf_handle* h, const KfOrthArgs& a, const ChipPlan& p, hipStream_
 }
 
 // ------------------------------------------------------------------------------------- |M|_F^2 in 64 bits, by parts
-constexpr int NORM_PARTS = 256;
+constexpr int NORM_PARTS = 1024;
 template <typename T>
 __global__ __launch_bounds__(256) void orth_norm_kernel(const T* M, long size, double* part) {
   constexpr int V = 16 / sizeof(T);
@@ -330,7 +330,9 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(const T* M, long size, d
 }
 // by a whole workgroup, the same order everywhere
 static __device__ __forceinline__ double norm_factor(const double* part, int parts, double eps, double* red) {
-  const double s = block_sum((int)threadIdx.x < parts ? part[threadIdx.x] : 0., red);
+  double s = 0.;
+  for (int x = threadIdx.x; x < parts; x += blockDim.x) s += part[x];
+  s = block_sum(s, red);
   return 1.0 / (sqrt(s) + eps);
 }
 static inline int norm_parts(long size) {  // about 16 elements a thread
@@ -353,13 +355,14 @@ static __device__ __forceinline__ void parts_of(f4 x, h4* hi, h4* lo) {
   *lo = __builtin_convertvector(x - __builtin_convertvector(*hi, f4), h4);
 }
 
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Eight { T v[8]; };  // at any element's address
 // 8 neighbours of a row of the result, of which `left` are inside it; at any element's address
 template <typename T> static __device__ __forceinline__ void store_row(T* to, f4 x, f4 y, int left) {
-  struct __attribute__((packed, aligned(sizeof(T)))) Eight { T v[8]; } o;
+  Eight<T> o;
 #pragma unroll
   for (int j = 0; j < 4; ++j) o.v[j] = from_acc<T>(x[j]), o.v[4 + j] = from_acc<T>(y[j]);
   if (left >= 8) {
-    *reinterpret_cast<Eight*>(to) = o;
+    *reinterpret_cast<Eight<T>*>(to) = o;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -385,17 +388,35 @@ __global__ __launch_bounds__(256) void orth_parts_kernel(KfOrthArgs a, const dou
     }
     __syncthreads();
   }
-  for (int e = threadIdx.x; e < 1024; e += 256) {
-    const int r = e >> 4, c = 4 * (e & 15);
-    f4 x;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      x[j] = tall ? tile[r][c + j] : r0 + r < d && c0 + c + j < L ? (float)((double)to_acc(M[(r0 + r) * (long)L + c0 + c + j]) * f) : 0.f;
-    h4 xh, xl;
+  for (int u = 0; u < 2; ++u) {
+    const int e = threadIdx.x + 256 * u, r = e >> 3, c = 8 * (e & 7);
+    f4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+    if (tall) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = tile[r][c + j], y[j] = tile[r][c + 4 + j];
+    } else if (r0 + r < d) {
+      const T* m = M + (r0 + r) * (long)L + c0 + c;
+      const int left = L - c0 - c;
+      Eight<T> in;
+      if (left >= 8) {
+        in = *reinterpret_cast<const Eight<T>*>(m);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) in.v[j] = j < left ? m[j] : from_acc<T>(0.f);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = (float)((double)to_acc(in.v[j]) * f);
+        y[j] = (float)((double)to_acc(in.v[4 + j]) * f);
+      }
+    }
+    h4 xh, xl, yh, yl;
     parts_of(x, &xh, &xl);
+    parts_of(y, &yh, &yl);
     const long to = at + place<STORED>(r0 + r, c0 + c, LP);
-    *(h4*)(hi + to) = xh;
-    *(h4*)(lo + to) = xl;
+    *(h8*)(hi + to) = __builtin_shufflevector(xh, yh, 0, 1, 2, 3, 4, 5, 6, 7);
+    *(h8*)(lo + to) = __builtin_shufflevector(xl, yl, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
 
@@ -434,6 +455,8 @@ static __device__ __forceinline__ void product_tile(const Product& p, const long
   const _Float16* P = p.P + z * PARTS * (long)p.dP * ldP;
   const _Float16* Q = p.Q + z * PARTS * (long)p.dP * ldQ;
 
+  // how the 32-byte groups of depth k's row are permuted: depths 0 .. 3 and 8 .. 11, which are read at a time, meet different banks
+  auto turn = [](int k) { return GR >= 8 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2); };
   // source of each 16-byte piece this lane brings in; a step further on along the depth it is 64 entries on, or BK rows
   const _Float16 *srcP[PER], *srcQ[PER];
   const long stepQ = NN ? (long)BK * PARTS * p.LP : 64;
@@ -442,7 +465,7 @@ static __device__ __forceinline__ void product_tile(const Product& p, const long
     const int s = tid + 256 * u, r = s >> 3, c = (s & 7) ^ (r & 7);
     srcP[u] = P + (tm * TILE + r) * PARTS * ldP + 8 * c;
     if (NN) {
-      const int k = s / (2 * GR), pos = s % (2 * GR), gr = (pos >> 1) ^ (k & 7 & (GR - 1));
+      const int k = s / (2 * GR), pos = s % (2 * GR), gr = (pos >> 1) ^ turn(k);
       srcQ[u] = Q + k * PARTS * ldQ + tn * TILE * PARTS + 16 * gr + 8 * (pos & 1);
     } else {
       srcQ[u] = Q + (tn * TILE + r) * PARTS * ldQ + 8 * c;
@@ -465,8 +488,8 @@ static __device__ __forceinline__ void product_tile(const Product& p, const long
     typedef __attribute__((address_space(3))) s4* lp;
     const int k = (PARTS == 1 ? 32 * half : 0) + 8 * g + (i >> 2);  // 4 rows for 16 lanes, and the 4 behind them
     const int gr = PARTS == 1 ? c >> 4 : ((c >> 5) << 2) + 2 * half + ((c >> 4) & 1);
-    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + k * TILE * PARTS + 16 * (gr ^ (k & 7 & (GR - 1))) + 4 * (i & 3)));
-    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + (k + 4) * TILE * PARTS + 16 * (gr ^ ((k + 4) & 7 & (GR - 1))) + 4 * (i & 3)));
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + k * TILE * PARTS + 16 * (gr ^ turn(k)) + 4 * (i & 3)));
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + (k + 4) * TILE * PARTS + 16 * (gr ^ turn(k + 4)) + 4 * (i & 3)));
     return __builtin_bit_cast(h8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
