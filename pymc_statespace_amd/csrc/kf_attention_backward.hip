@@ -9,6 +9,16 @@
 // with W_ij = s D_ij A_ij B_ij: what passes through the decay of token t.  All of it from this chunk's own numbers (the shorter form,
 // a running sum of q.dq - k.dk over the whole sequence, loses what those sums share).  Then R <- E R + sum_i s e^{G_i} q_i do_i'.
 //
+// Roundings (bf16 data): scores times their decays, and R where the keys meet it for dv, 2^-9 each, like the gradients themselves.  What
+// enters fp32 results -- dq and dk through the states, whose products with q and k are part of the decays' gradient, and the sums of S
+// and R -- is multiplied in three exact parts.  fp32 and fp16 data: fp32 throughout.
+//
+// Measured: 4 x 2048 tokens, 16 heads of 128 x 128, bf16: 42 + 40 + 118 us for 236 MB (50 us at the 4.7 TB/s of a large copy); 134 MB of
+// starts are written and read on top.  16 x 128 tokens, 8 heads of 64 x 64, fp16: 9 + 6 + 17 us.  3 x 333 ragged tokens, 6 heads of 40 x 72
+// on 2 groups, fp32: 13 + 9 + 7 + 23 + 4 + 4 us.  The gradient kernel has one workgroup on a compute unit (148 KB of LDS, 256 registers), whose
+// 8 waves go through the chunk's phases together: 1750 vector instructions a wave and chunk are 44 % of its time, LDS 36 %, the matrix
+// pipe 19 %, and they hardly overlap.  Without the fences between depths the compiler holds all of them at once and spills: 325 us in all.
+//
 // Launches: (1) where the time axis is cut into segments, what each segment adds to S and to R; (2) S at every chunk's start, kept
 // as the accumulators that hold it; (3) the chunks of each segment from its last to its first, R in registers; (4) sums over
 // the heads that share queries and keys, and over tokens for fixed decays.

@@ -1,9 +1,19 @@
 // kf_attention_forward.hip -- linear attention with a decay for each head over whole sequences, in chunks of 64 tokens:
 //     o_i = s [ e^{G_i} S' q_i + sum_{j <= i} e^{G_i - G_j} (q_i . k_j) v_j ],   S <- e^{G_63} S + sum_j e^{G_63 - G_j} k_j v_j'
 // (S the state at the chunk's start).  One workgroup of four waves walks the chunks of one segment of one head with its K x VT part
-// of the state in accumulator registers; every input is read once, o written once.  Where sequences and heads are too few to fill
-// the card the time axis is cut into segments: a first launch computes what each segment adds to the state, and the second starts
-// each segment from the sum of what came before it.
+// of the state in accumulator registers.  Where sequences and heads are too few to fill the card the time axis is cut into segments: a
+// first launch computes what each segment adds to the state, and the second starts each segment from the sum of what came before it
+// (k and v are then read twice; one segment reads every input once).
+//
+// Roundings (bf16 data; fp32 and fp16 data are multiplied in fp32): the state's copy that the queries meet and the scores times their
+// decays, 2^-9 each, like o itself -- together 2.3e-3 of o where o's own rounding is 1.7e-3.  The state is exact to fp32's sums:
+// weighted keys enter it in three parts (KfSplit).
+//
+// Measured: 4 x 2048 tokens, 16 heads of 128 x 128, bf16: 25 + 48 us for 139 MB (30 us at the 4.7 TB/s of a large copy).  32768 tokens, 32
+// heads of 128 x 64: 88 + 7 + 158 us for 408 MB (87 us).  5 x 1000 ragged tokens, 6 heads of 72 x 56, fp32: 12 + 32 us.  What bounds the
+// second launch is issue: two waves on a SIMD (196 registers) spend 46 % of its cycles on vector instructions -- 290 of 670 for each
+// chunk cut the weighted keys --, the matrix pipe is busy 23 %, LDS 25 %, and between the chunk's two barriers little overlaps.  A third
+// wave (168 registers) spills and gains nothing: 47.5 us.  Loads alone take 18 us, scores 8, the state's products with q 7, its update 10.
 #include "kf_attention_chunk.h"
 
 namespace {

@@ -2,7 +2,7 @@
 //     X = M / (|M|_F + eps);   per step   A = X X',   X <- a X + (b A + c A A) X
 // on the transpose where there are more rows than columns: X is d x L with d <= L.  Four ways, by size and type:
 //   * d <= 16, L <= 64: one wave for each matrix, all steps in its registers
-//   * d <= 64 and both copies of X in LDS: one workgroup for each matrix, all steps on chip, in 32 bits (64 for fp64)
+//   * d <= 80 and X in LDS: one workgroup for each matrix, all steps on chip, in 32 bits (64 for fp64)
 //   * larger, up to 32 bits: tiled products on v_mfma_f32_16x16x32_f16, numbers held in fp16 parts (below)
 //   * larger, fp64: tiled products in fp64
 //
@@ -43,6 +43,7 @@ template <typename X> static __device__ __forceinline__ X block_sum(X s, X* red)
 
 // ------------------------------------------------------------------------------------- in the registers of one wave
 // d <= 16, L <= 16 NT.  Tiles of 16 x 16 as v_mfma_*_16x16x4 leave them: lane (g, c) holds column c of rows r(s, g), s = 0 .. 3.
+// Measured against one workgroup for each matrix (below): 512 of 16 x 64 in fp32 9 and 27 us, 4096 of 16 x 64 in fp64 36 and 132.
 // The same registers are the right operand of a product that runs over those rows, and the left operand's transpose: with y = X' (X's
 // tiles transposed through LDS once a step), A = y'y, A A and B X = (B)'x need no other lane's values.  The fp64 instructions' 64 cycles
 // bound it (each SIMD has four matrices of 4096): four of them only where the depth is above 12 (4096 matrices of 10 x 10: 14 us with
@@ -142,164 +143,169 @@ int launch_wave(kf_handle* h, const KfOrthArgs& a, hipStream_t stream) {
 static inline bool fits_wave(const KfOrthArgs& a) { return (a.rows <= 16 && a.cols <= 64) || (a.cols <= 16 && a.rows <= 64); }
 
 // ----------------------------------------------------------------------------------------------------- on chip
-// Output tiles of RT x RT for each thread.  Where there are fewer tiles of A than threads the sum over L is cut into `slices`.
-template <typename T, int RT>
-__global__ __launch_bounds__(256) void orth_chip_kernel(KfOrthArgs a, int slices) {
+// d <= 80 and X, A and B in LDS, padded with zeros to whole tiles of 16 x 16; one workgroup for each matrix.  A product's
+// operand is read along the depth, 4 numbers of one row for each lane (depth 4 g + s in step s, the same for both operands), or, X as the
+// right operand of B X, 4 numbers of one column.  B X stays in registers until every wave has read X.  Rows are an odd number of 16-byte
+// pieces apart: neighbouring rows meet different banks.  Where A has fewer tiles than there are waves the sum over L is cut into
+// `slices`, which meet in LDS.  Measured against the tiled products below, fp32: 256 matrices of 24 x 24 11 and 143 us, 256 of 64 x 64 42 and
+// 145, 256 of 64 x 250 79 and 189, one of 64 x 250 71 and 63, one of 80 x 150 69 and 75; fp64: 256 of 80 x 80 74 and 510 us.  Bound by the
+// waits between its three products a step, each short: the matrix pipe of a 64 x 64 matrix is busy 20 of 40 us.
+template <typename C> struct ChipRow { static __host__ __device__ constexpr int stride(int n) { return sizeof(C) == 8 ? (n & ~1) | 2 : (n & ~3) | 4; } };
+
+// WAVES x HELD tiles of X at most, HELD for each wave.
+template <typename T, int WAVES, int HELD>
+__global__ __launch_bounds__(64 * WAVES, HELD == 4 ? 4 : 2) void orth_chip_kernel(KfOrthArgs a, int slices) {
   typedef typename Acc<T>::type C;
-  constexpr int TH = 256;
+  typedef Tile<C> Q;
+  typedef typename Q::type V;
+  constexpr int TH = 64 * WAVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ double red[TH / 64];
+  __shared__ double red[WAVES];
   const bool tall = a.rows > a.cols;
   const int d = tall ? a.cols : a.rows, L = tall ? a.rows : a.cols;
-  const int lx = L | 1, la = d | 1;  // odd rows: different banks
+  const int td = (d + 15) / 16, tl = (L + 15) / 16, ts = td * (td + 1) / 2;
+  const int lx = ChipRow<C>::stride(16 * tl), la = ChipRow<C>::stride(16 * td);
   C* X = (C*)smem;
-  C* Y = X + d * lx;
-  C* A = Y + d * lx;
-  C* B = A + d * la;
-  C* part = B + d * la;  // [slices][d d]
+  C* A = X + 16 * td * lx;
+  C* B = A + 16 * td * la;
+  C* part = B + 16 * td * la;  // [slices][ts][256]
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, i = l & 15, g = l >> 4;
   const long size = (long)d * L;
   const T* M = (const T*)a.M + blockIdx.x * size;
   T* out = (T*)a.X + blockIdx.x * size;
-  double s = 0.;
-  for (int e = threadIdx.x; e < size; e += TH) {
+  for (int e = tid; e < 16 * td * lx; e += TH) X[e] = C(0);
+  __syncthreads();
+  double sum = 0.;
+  for (int e = tid; e < size; e += TH) {
     const C x = to_acc(M[e]);
     const int r = e / a.cols, c = e - r * a.cols;
     X[tall ? c * lx + r : r * lx + c] = x;
-    s += (double)x * (double)x;
+    sum += (double)x * (double)x;
   }
-  const double f = 1.0 / (sqrt(block_sum(s, red)) + a.eps);
-  for (int e = threadIdx.x; e < size; e += TH) {
-    C& x = X[(e / L) * lx + e % L];
-    x = (C)((double)x * f);
-  }
+  const double f = 1.0 / (sqrt(block_sum(sum, red)) + a.eps);
+  for (int e = tid; e < 16 * td * lx; e += TH) X[e] = (C)((double)X[e] * f);  // (f = inf of a matrix of zeros with eps = 0: NaN, as it should be)
   __syncthreads();
-  const int td = (d + RT - 1) / RT, tl = (L + RT - 1) / RT, ts = td * (td + 1) / 2;
-  auto below = [](int t, int* r, int* c) {
-    int x = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-    x += (x + 1) * (x + 2) / 2 <= t;
-    x -= x * (x + 1) / 2 > t;
-    *r = x * RT;
-    *c = (t - x * (x + 1) / 2) * RT;
+  typedef V V16 __attribute__((aligned(16)));
+  auto row = [&](const C* p, int ld, int r, int k) { return (V)*reinterpret_cast<const V16*>(p + (r + i) * ld + k + 4 * g); };
+  auto below = [](int t, int* r, int* c) {  // tile t on or below the diagonal
+    int x = 0;
+    while ((x + 1) * (x + 2) / 2 <= t) ++x;
+    *r = 16 * x;
+    *c = 16 * (t - x * (x + 1) / 2);
   };
+  auto store = [&](C* p, int r0, int c0, V v) {  // and its mirror image
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int r = r0 + Q::row(s, g);
+      p[r * la + c0 + i] = v[s];
+      p[(c0 + i) * la + r] = v[s];
+    }
+  };
+  const V zero = {C(0), C(0), C(0), C(0)};
   for (int step = 0; step < a.steps; ++step) {
     const C ca = (C)a.coef[step][0], cb = (C)a.coef[step][1], cc = (C)a.coef[step][2];
-    // A = X X', tiles on and below the diagonal
-    for (int w = threadIdx.x; w < ts * slices; w += TH) {
-      const int t = w / slices, sl = w - t * slices;
+    // A = X X'
+    for (int x = w; x < ts * slices; x += WAVES) {
+      const int t = x % ts, sl = x / ts;
       int r0, c0;
       below(t, &r0, &c0);
-      C acc[RT][RT] = {};
-      const C *xr[RT], *xc[RT];
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        xr[i] = X + (r0 + i < d ? r0 + i : d - 1) * lx;
-        xc[i] = X + (c0 + i < d ? c0 + i : d - 1) * lx;
-      }
-      for (int k = sl; k < L; k += slices) {
-        C u[RT], v[RT];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) u[i] = xr[i][k], v[i] = xc[i][k];
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int j = 0; j < RT; ++j) acc[i][j] += u[i] * v[j];
-      }
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < RT; ++j)
-          if (r0 + i < d && c0 + j < d) {
-            if (slices > 1) part[sl * d * d + (r0 + i) * d + c0 + j] = part[sl * d * d + (c0 + j) * d + r0 + i] = acc[i][j];
-            else A[(r0 + i) * la + c0 + j] = A[(c0 + j) * la + r0 + i] = acc[i][j];
-          }
+      V acc = zero;
+      for (int k = 16 * sl; k < 16 * tl; k += 16 * slices) acc = Q::mma(row(X, lx, r0, k), row(X, lx, c0, k), acc, 16);
+      if (slices > 1) reinterpret_cast<V16*>(part)[x * 64 + l] = acc;
+      else store(A, r0, c0, acc);
     }
     __syncthreads();
     if (slices > 1) {
-      for (int e = threadIdx.x; e < d * d; e += TH) {
-        C x = 0;
-        for (int sl = 0; sl < slices; ++sl) x += part[sl * d * d + e];
-        A[(e / d) * la + e % d] = x;
+      for (int t = w; t < ts; t += WAVES) {
+        int r0, c0;
+        below(t, &r0, &c0);
+        V acc = zero;
+        for (int sl = 0; sl < slices; ++sl) acc += reinterpret_cast<const V16*>(part)[(sl * ts + t) * 64 + l];
+        store(A, r0, c0, acc);
       }
       __syncthreads();
     }
     // B = b A + c A A (A is symmetric: rows for columns)
-    for (int t = threadIdx.x; t < ts; t += TH) {
+    for (int t = w; t < ts; t += WAVES) {
       int r0, c0;
       below(t, &r0, &c0);
-      C acc[RT][RT] = {};
-      for (int k = 0; k < d; ++k) {
-        C u[RT], v[RT];
+      V acc = zero;
+      for (int k = 0; k < 16 * td; k += 16) acc = Q::mma(row(A, la, r0, k), row(A, la, c0, k), acc, 16);
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          u[i] = A[(r0 + i < d ? r0 + i : d - 1) * la + k];
-          v[i] = A[(c0 + i < d ? c0 + i : d - 1) * la + k];
-        }
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int j = 0; j < RT; ++j) acc[i][j] += u[i] * v[j];
-      }
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < RT; ++j)
-          if (r0 + i < d && c0 + j < d) B[(r0 + i) * la + c0 + j] = B[(c0 + j) * la + r0 + i] = cb * A[(r0 + i) * la + c0 + j] + cc * acc[i][j];
+      for (int s = 0; s < 4; ++s) acc[s] = cb * A[(r0 + Q::row(s, g)) * la + c0 + i] + cc * acc[s];
+      store(B, r0, c0, acc);
     }
     __syncthreads();
-    // Y = a X + B X
-    for (int t = threadIdx.x; t < td * tl; t += TH) {
-      const int r0 = t / tl * RT, c0 = t % tl * RT;
-      C acc[RT][RT] = {};
-      for (int k = 0; k < d; ++k) {
-        C u[RT], v[RT];
+    // a X + B X
+    V held[HELD];
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          u[i] = B[(r0 + i < d ? r0 + i : d - 1) * la + k];
-          v[i] = X[k * lx + (c0 + i < L ? c0 + i : L - 1)];
+    for (int u = 0; u < HELD; ++u) {
+      const int t = w + u * WAVES;
+      held[u] = zero;
+      if (t < td * tl) {
+        const int r0 = t / tl * 16, c0 = t % tl * 16;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) held[u][s] = ca * X[(r0 + Q::row(s, g)) * lx + c0 + i];
+        for (int k = 0; k < 16 * td; k += 16) {
+          V x;
+#pragma unroll
+          for (int s = 0; s < 4; ++s) x[s] = X[(k + 4 * g + s) * lx + c0 + i];
+          held[u] = Q::mma(row(B, la, r0, k), x, held[u], 16);
         }
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int j = 0; j < RT; ++j) acc[i][j] += u[i] * v[j];
       }
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < RT; ++j)
-          if (r0 + i < d && c0 + j < L) Y[(r0 + i) * lx + c0 + j] = ca * X[(r0 + i) * lx + c0 + j] + acc[i][j];
     }
     __syncthreads();
-    C* t = X; X = Y; Y = t;
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) {
+      const int t = w + u * WAVES;
+      if (t < td * tl) {
+        const int r0 = t / tl * 16, c0 = t % tl * 16;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) X[(r0 + Q::row(s, g)) * lx + c0 + i] = held[u][s];
+      }
+    }
+    __syncthreads();
   }
-  for (int e = threadIdx.x; e < size; e += TH) {
+  for (int e = tid; e < size; e += TH) {
     const int r = e / a.cols, c = e - r * a.cols;
     out[e] = from_acc<T>(X[tall ? c * lx + r : r * lx + c]);
   }
 }
 
-struct ChipPlan { int rt, slices; size_t lds; bool fits; };
+struct ChipPlan { int waves, held, slices; size_t lds; bool fits; };
 ChipPlan chip_plan(const KfOrthArgs& a) {
   ChipPlan p;
-  const long d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
-  const size_t e = a.dtype == KF_DTYPE_F64 ? 8 : 4;
+  const int d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
   p.fits = false;
-  if (d > 64 || L > 40000) return p;
-  p.rt = d <= 32 ? 2 : 4;  // (LDS bandwidth bounds these products: tiles of 2 x 2 halve it, and still leave every thread one)
-  const long td = (d + p.rt - 1) / p.rt, tiles = td * (td + 1) / 2;
-  p.slices = 1;
-  while (2 * p.slices * tiles <= 256 && 2 * p.slices <= L / 8) p.slices *= 2;
-  p.lds = e * (2 * d * (L | 1) + 2 * d * (d | 1) + (p.slices > 1 ? p.slices * d * d : 0));
-  p.fits = p.lds <= 156 * 1024;
+  if (d > 80 || L > 10000) return p;
+  const int td = (d + 15) / 16, tl = (L + 15) / 16, ts = td * (td + 1) / 2;
+  const bool wide = a.dtype == KF_DTYPE_F64;
+  auto stride = [&](int n) { return wide ? ChipRow<double>::stride(n) : ChipRow<float>::stride(n); };
+  // as few registers as hold the tiles, so that several matrices share a compute unit (1024 of 24 x 100: 87 us with 8 waves that could hold
+  // 16 tiles each, 39 with 4 of 4 tiles; 1024 of 40 x 100: 124 us, with 8 of 4 tiles 79)
+  const int tiles = td * tl;
+  p.waves = tiles <= 16 ? 4 : 8;
+  p.held = tiles <= 32 ? 4 : tiles <= 64 ? 8 : 16;
+  p.slices = p.waves / ts < 1 ? 1 : p.waves / ts;
+  p.lds = (wide ? 8 : 4) * ((size_t)16 * td * (stride(16 * tl) + 2 * stride(16 * td)) + (p.slices > 1 ? p.slices * ts * 256 : 0));
+  p.fits = p.lds <= 156 * 1024 && tiles <= 8 * (wide ? 8 : 16);
   return p;
 }
 
-template <typename T, int RT>
+template <typename T, int WAVES, int HELD>
 int launch_chip(kf_handle* h, const KfOrthArgs& a, const ChipPlan& p, hipStream_t stream) {
-  KF_HIP_CHECK(h, hipFuncSetAttribute(reinterpret_cast<const void*>(orth_chip_kernel<T, RT>),
-                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds));
-  hipLaunchKernelGGL((orth_chip_kernel<T, RT>), dim3((unsigned)a.n), dim3(256), p.lds, stream, a, p.slices);
+  KF_HIP_CHECK(h, hipFuncSetAttribute(reinterpret_cast<const void*>(orth_chip_kernel<T, WAVES, HELD>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds));
+  hipLaunchKernelGGL((orth_chip_kernel<T, WAVES, HELD>), dim3((unsigned)a.n), dim3(64 * WAVES), p.lds, stream, a, p.slices);
   KF_HIP_CHECK(h, hipGetLastError());
   return KF_OK;
+}
+template <typename T>
+int launch_chip(kf_handle* h, const KfOrthArgs& a, const ChipPlan& p, hipStream_t stream) {
+  if (p.waves == 4) return launch_chip<T, 4, 4>(h, a, p, stream);
+  if (p.held == 4) return launch_chip<T, 8, 4>(h, a, p, stream);
+  if constexpr (sizeof(typename Acc<T>::type) == 4)
+    if (p.held == 16) return launch_chip<T, 8, 16>(h, a, p, stream);
+  return launch_chip<T, 8, 8>(h, a, p, stream);
 }
 
 // ------------------------------------------------------------------------------------- |M|_F^2 in 64 bits, by parts
@@ -808,7 +814,7 @@ template <typename T>
 int launch_t(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
   if (fits_wave(a)) return launch_wave<T>(h, a, stream);
   const ChipPlan c = chip_plan(a);
-  if (c.fits) return c.rt == 2 ? launch_chip<T, 2>(h, a, c, stream) : launch_chip<T, 4>(h, a, c, stream);
+  if (c.fits) return launch_chip<T>(h, a, c, stream);
   return launch_parts<T, std::is_same<T, __hip_bfloat16>::value ? 1 : 2>(h, a, parts_plan(a), ws, stream);
 }
 
@@ -831,7 +837,7 @@ int kf_launch_orthogonalise(kf_handle* h, const KfOrthArgs& a, void* ws, hipStre
       if (fits_wave(a)) return launch_wave<double>(h, a, stream);
       const ChipPlan c = chip_plan(a);
       if (!c.fits) return launch64(h, a, ws, stream);
-      return c.rt == 2 ? launch_chip<double, 2>(h, a, c, stream) : launch_chip<double, 4>(h, a, c, stream);
+      return launch_chip<double>(h, a, c, stream);
     }
     case KF_DTYPE_F32: return launch_t<float>(h, a, ws, stream);
     case KF_DTYPE_BF16: return launch_t<__hip_bfloat16>(h, a, ws, stream);

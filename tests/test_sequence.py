@@ -144,7 +144,7 @@ def test_buffers_that_share_memory_are_refused(lib, handle):
 
 @pytest.mark.parametrize("n, rows, cols, dtype, rc", [
     (0, 4, 4, 1, -1), (1, 0, 4, 1, -1), (1, 4, -1, 1, -1), (1, 4, 4, 4, -4), (1, 4, 4, -1, -4), (1, 1 << 18, 1 << 18, 1, -4),
-    (1 << 40, 4, 4, 1, -4), (4, 1 << 17, 1 << 24, 1, -4), (1, 1 << 16, (1 << 15) + 1, 0, -4), (65536, 80, 80, 1, -4)])
+    (1 << 40, 4, 4, 1, -4), (4, 1 << 17, 1 << 24, 1, -4), (1, 1 << 16, (1 << 15) + 1, 0, -4), (65536, 100, 100, 1, -4)])
 def test_matrices_that_are_refused(lib, handle, n, rows, cols, dtype, rc):
     size, one = C.c_size_t(), C.c_void_p(16)
     coef = (C.c_double * 3)(1.5, -0.5, 0.0)
