@@ -4,7 +4,7 @@
 //   * d <= 16, L <= 64: one wave for each matrix, all steps in its registers
 //   * d <= 80 and X in LDS: one workgroup for each matrix, all steps on chip, in 32 bits (64 for fp64)
 //   * larger, up to 32 bits: tiled products on v_mfma_f32_16x16x32_f16, numbers held in fp16 parts (below)
-//   * larger, fp64: tiled products in fp64
+//   * larger, fp64: tiled products on v_mfma_f64_16x16x4
 //
 // Numbers in fp16 parts.  The singular values stay within 1.9 (checked on the host), so entries of X, A = X X' and B = b A + c A A are
 // bounded and a power of two for each brings them to the top of fp16's range: hi = fp16(x), lo = fp16(x - hi) hold 22 bits and
@@ -149,7 +149,7 @@ static inline bool fits_wave(const KfOrthArgs& a) { return (a.rows <= 16 && a.co
 // pieces apart: neighbouring rows meet different banks.  Where A has fewer tiles than there are waves the sum over L is cut into
 // `slices`, which meet in LDS.  Measured against the tiled products below, fp32: 256 matrices of 24 x 24 11 and 143 us, 256 of 64 x 64 42 and
 // 145, 256 of 64 x 250 79 and 189, one of 64 x 250 71 and 63, one of 80 x 150 69 and 75; fp64: 256 of 80 x 80 74 and 510 us.  Bound by the
-// waits between its three products a step, each short: the matrix pipe of a 64 x 64 matrix is busy 20 of 40 us.
+// waits between its three products a step, each short: the matrix pipe is busy 10 us of a 64 x 64 matrix's 40.
 template <typename C> struct ChipRow { static __host__ __device__ constexpr int stride(int n) { return sizeof(C) == 8 ? (n & ~1) | 2 : (n & ~3) | 4; } };
 
 // WAVES x HELD tiles of X at most, HELD for each wave.
@@ -744,43 +744,148 @@ __global__ __launch_bounds__(256) void orth_scale64_kernel(KfOrthArgs a, const d
   X[a.rows > a.cols ? z * size + (e % a.cols) * a.rows + e / a.cols : i] = ((const double*)a.M)[i] * f;
 }
 
-// C (m x n) = alpha op(A B) + beta D, A (m x k) row-major, B (k x n) row-major or (NT) given as (n x k); `tall`: C is stored transposed
-template <bool NT>
-__global__ __launch_bounds__(256) void orth_product64_kernel(int m, int n, int k, const double* A, const double* B, const double* D, double* out,
-                                                             double alpha, double beta, int tall) {
-  __shared__ double sa[16][65], sb[16][65];
+// out (m x n) = alpha A B + beta D: A (m x k) row-major, B (k x n) row-major or (NT) given as (n x k); `tall`: stored transposed.  64 x 64 of
+// it for each workgroup of 2 x 2 waves, v_mfma_f64_16x16x4 on operands in LDS, 32 depths at a time, the 64 behind them on their way (with a
+// wait for each load, 128 x 128: 318 us instead of 195).  SYM: the
+// result is symmetric, tiles on and below the diagonal, stored twice.  Where there are few tiles the depth is cut into `slices`, each of
+// which leaves its sum in `parts`, [slices][matrices][m n].
+struct Product64 {
+  int m, n, k, tiles_n, slices, tall;
+  const double *A, *B, *D;
+  double *out, *parts;
+  double alpha, beta;
+};
+template <bool NT, bool SYM>
+__global__ __launch_bounds__(256) void orth_product64_kernel(Product64 p) {
+  typedef Tile<double> Q;
+  typedef Q::type V;
+  typedef V V16 __attribute__((aligned(16)));
+  constexpr int BK = 32, SA = BK + 2, SB = NT ? SA : 66;  // rows an odd number of 16-byte pieces apart
+  __shared__ __attribute__((aligned(16))) double sa[64 * SA], sb[NT ? 64 * SA : BK * SB];
   const long z = blockIdx.z;
-  A += z * m * (long)k;
-  B += z * n * (long)k;
-  D += z * m * (long)n;
-  out += z * m * (long)n;
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  double acc[4][4] = {};
-  for (int k0 = 0; k0 < k; k0 += 16) {
-    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-      const int kk = i & 15, r = i >> 4;
-      sa[kk][r] = r0 + r < m && k0 + kk < k ? A[(long)(r0 + r) * k + k0 + kk] : 0.;
-      if (NT) {
-        sb[kk][r] = c0 + r < n && k0 + kk < k ? B[(long)(c0 + r) * k + k0 + kk] : 0.;
-      } else {
-        const int cc = i & 63, k2 = i >> 6;
-        sb[k2][cc] = c0 + cc < n && k0 + k2 < k ? B[(long)(k0 + k2) * n + c0 + cc] : 0.;
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < 16; ++kk)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += sa[kk][ty + 16 * i] * sb[kk][tx + 16 * j];
-    __syncthreads();
+  const double *A = p.A + z * p.m * (long)p.k, *B = p.B + z * p.n * (long)p.k;
+  int tm, tn;
+  const int x = blockIdx.x;
+  if (SYM) {
+    tm = (int)((sqrtf(8.f * x + 1.f) - 1.f) * 0.5f);
+    while ((tm + 1) * (tm + 2) / 2 <= x) ++tm;
+    while (tm * (tm + 1) / 2 > x) --tm;
+    tn = x - tm * (tm + 1) / 2;
+  } else {
+    tm = x / p.tiles_n;
+    tn = x - tm * p.tiles_n;
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int r = r0 + ty + 16 * i, c = c0 + tx + 16 * j;
-      if (r < m && c < n) out[tall ? (long)c * m + r : (long)r * n + c] = alpha * acc[i][j] + (beta != 0. ? beta * D[(long)r * n + c] : 0.);
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, i = l & 15, g = l >> 4, r0 = 64 * tm, c0 = 64 * tn;
+  const int wm = 32 * (w & 1), wn = 32 * (w >> 1);
+  // 4 neighbours of a row along the depth (or, NN, along B's columns), and, when they are needed (a select behind the load would wait for
+  // it), zeros for what is outside
+  auto four = [](const double* p, int row, int rows, int col, int cols) {
+    V v;
+    const double* q = p + (long)(row < rows ? row : rows - 1) * cols;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = q[col + e < cols ? col + e : cols - 1];
+    return v;
+  };
+  auto inside = [](V v, int row, int rows, int col, int cols) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = row < rows && col + e < cols ? v[e] : 0.;
+    return v;
+  };
+  const int ar = tid >> 3, ak = 4 * (tid & 7), bk = tid >> 4, bc = 4 * (tid & 15);
+  const int blocks = (p.k + BK - 1) / BK, per = (blocks + p.slices - 1) / p.slices;
+  const int first = blockIdx.y * per, last = first + per < blocks ? first + per : blocks;
+  V va[2][2], vb[2][2];
+  auto load = [&](int b, V (&x)[2], V (&y)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      x[u] = four(A, r0 + ar + 32 * u, p.m, BK * b + ak, p.k);
+      y[u] = NT ? four(B, c0 + ar + 32 * u, p.n, BK * b + ak, p.k) : four(B, BK * b + bk + 16 * u, p.k, c0 + bc, p.n);
     }
+  };
+  V acc[2][2] = {};
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (first + h < last) load(first + h, va[h], vb[h]);
+  for (int b0 = first; b0 < last; b0 += 2) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (b0 + h >= last) break;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int k0 = BK * (b0 + h);
+        *reinterpret_cast<V16*>(sa + (ar + 32 * u) * SA + ak) = inside(va[h][u], r0 + ar + 32 * u, p.m, k0 + ak, p.k);
+        *reinterpret_cast<V16*>(sb + (NT ? (ar + 32 * u) * SB + ak : (bk + 16 * u) * SB + bc)) =
+            NT ? inside(vb[h][u], c0 + ar + 32 * u, p.n, k0 + ak, p.k) : inside(vb[h][u], k0 + bk + 16 * u, p.k, c0 + bc, p.n);
+      }
+      // (not __syncthreads, which would wait for the loads under way)
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      load(b0 + h + 2 < last ? b0 + h + 2 : b0 + h, va[h], vb[h]);
+#pragma unroll
+      for (int kk = 0; kk < BK; kk += 16) {
+        V pa[2], qb[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          pa[t] = *reinterpret_cast<const V16*>(sa + (wm + 16 * t + i) * SA + kk + 4 * g);
+          if (NT) {
+            qb[t] = *reinterpret_cast<const V16*>(sb + (wn + 16 * t + i) * SB + kk + 4 * g);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qb[t][e] = sb[(kk + 4 * g + e) * SB + wn + 16 * t + i];
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) acc[t][u] = Q::mma(pa[t], qb[u], acc[t][u], 16);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+  }
+  const double* D = p.D + z * p.m * (long)p.n;
+  double* out = p.slices > 1 ? p.parts + (blockIdx.y * (long)gridDim.z + z) * p.m * p.n : p.out + z * p.m * (long)p.n;
+  const bool tall = p.tall && p.slices == 1;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = r0 + wm + 16 * t + Q::row(e, g), c = c0 + wn + 16 * u + i;
+        if (r >= p.m || c >= p.n) continue;
+        double v = acc[t][u][e];
+        if (p.slices == 1) v = p.alpha * v + (p.beta != 0. ? p.beta * D[(long)r * p.n + c] : 0.);
+        out[tall ? (long)c * p.m + r : (long)r * p.n + c] = v;
+        if (SYM && tm != tn) out[(long)c * p.n + r] = v;
+      }
+}
+__global__ __launch_bounds__(256) void orth_slices64_kernel(Product64 p, long size) {
+  const long e = (long)blockIdx.x * 256 + threadIdx.x;
+  if (e >= size) return;
+  double s = 0.;
+  for (int x = 0; x < p.slices; ++x) s += p.parts[x * size + e];
+  const long cells = (long)p.m * p.n, z = e / cells, i = e - z * cells, r = i / p.n, c = i - r * p.n;
+  p.out[p.tall ? z * cells + c * p.m + r : e] = p.alpha * s + (p.beta != 0. ? p.beta * p.D[e] : 0.);
+}
+
+// how a product's depth is cut where it has few tiles: two workgroups for each compute unit, at least 128 depths for each (one matrix of
+// 100 x 4000: 1173 us uncut, 255 cut; one of 512 x 512: 498 and 295; its library products take 571 and 295)
+int slices64(const kf_handle* h, long n, int d, int cols, int depth) {
+  const long cu = h->n_cu > 0 ? h->n_cu : 256, td = (d + 63) / 64, tiles = n * (cols == d ? td * (td + 1) / 2 : td * ((cols + 63) / 64));
+  const long most = depth / 128, want = 2 * cu / tiles;
+  const long s = want < most ? want : most;
+  return s < 1 ? 1 : (int)s;
+}
+size_t cut64(const kf_handle* h, long n, int d, int L) {  // bytes for the parts of the product that needs most
+  size_t most = 0;
+  auto take = [&](int cols, int depth) {
+    const int s = slices64(h, n, d, cols, depth);
+    const size_t bytes = s > 1 ? (size_t)s * n * d * cols * 8 : 0;
+    most = bytes > most ? bytes : most;
+  };
+  take(d, L);
+  take(d, d);
+  take(L, d);
+  return kf_seq_round(most);
 }
 
 int launch64(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
@@ -792,18 +897,27 @@ int launch64(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
   double* X = (double*)w; w += big;
   double* Y = (double*)w; w += big;
   double* A = (double*)w; w += small;
-  double* B = (double*)w;
+  double* B = (double*)w; w += small;
+  double* cut = (double*)w;
   const long size = (long)d * L;
   const int parts = norm_parts(size);
   hipLaunchKernelGGL(orth_norm_kernel<double>, dim3(parts, (unsigned)a.n), dim3(256), 0, stream, (const double*)a.M, size, norm);
   hipLaunchKernelGGL(orth_scale64_kernel, dim3((unsigned)((size + 255) / 256), (unsigned)a.n), dim3(256), 0, stream, a, norm, parts, X);
   const unsigned td = (d + 63) / 64, tl = (L + 63) / 64, z = (unsigned)a.n;
+  auto run = [&](Product64 p, bool symmetric) {
+    p.tiles_n = (int)tl;
+    p.parts = cut;
+    p.slices = symmetric ? slices64(h, a.n, d, d, p.k) : slices64(h, a.n, d, L, p.k);
+    if (symmetric) hipLaunchKernelGGL((orth_product64_kernel<true, true>), dim3(td * (td + 1) / 2, p.slices, z), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((orth_product64_kernel<false, false>), dim3(td * tl, p.slices, z), dim3(256), 0, stream, p);
+    const long cells = a.n * p.m * (long)p.n;
+    if (p.slices > 1) hipLaunchKernelGGL(orth_slices64_kernel, dim3((unsigned)((cells + 255) / 256)), dim3(256), 0, stream, p, cells);
+  };
   for (int s = 0; s < a.steps; ++s) {
     const bool last = s + 1 == a.steps;
-    hipLaunchKernelGGL(orth_product64_kernel<true>, dim3(td, td, z), dim3(256), 0, stream, d, d, L, X, X, A, A, 1., 0., 0);
-    hipLaunchKernelGGL(orth_product64_kernel<true>, dim3(td, td, z), dim3(256), 0, stream, d, d, d, A, A, A, B, a.coef[s][2], a.coef[s][1], 0);
-    hipLaunchKernelGGL(orth_product64_kernel<false>, dim3(tl, td, z), dim3(256), 0, stream, d, L, d, B, X, X, last ? (double*)a.X : Y, 1., a.coef[s][0],
-                       last && tall);
+    run({d, d, L, 0, 1, 0, X, X, A, A, nullptr, 1., 0.}, true);
+    run({d, d, d, 0, 1, 0, A, A, A, B, nullptr, a.coef[s][2], a.coef[s][1]}, true);
+    run({d, L, d, 0, 1, last && tall, B, X, X, last ? (double*)a.X : Y, nullptr, 1., a.coef[s][0]}, false);
     double* t = X; X = Y; Y = t;
   }
   KF_HIP_CHECK(h, hipGetLastError());
@@ -822,11 +936,12 @@ int launch_t(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
 
 bool kf_orthogonalise_on_chip(const KfOrthArgs& a) { return fits_wave(a) || chip_plan(a).fits; }
 
-size_t kf_orthogonalise_ws(const kf_handle*, const KfOrthArgs& a) {
+size_t kf_orthogonalise_ws(const kf_handle* h, const KfOrthArgs& a) {
   if (kf_orthogonalise_on_chip(a)) return 0;
   const size_t d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
   if (a.dtype == KF_DTYPE_F64)
-    return kf_seq_round((size_t)a.n * NORM_PARTS * 8) + 2 * kf_seq_round((size_t)a.n * d * L * 8) + 2 * kf_seq_round((size_t)a.n * d * d * 8);
+    return kf_seq_round((size_t)a.n * NORM_PARTS * 8) + 2 * kf_seq_round((size_t)a.n * d * L * 8) + 2 * kf_seq_round((size_t)a.n * d * d * 8) +
+           cut64(h, a.n, (int)d, (int)L);
   const PartsPlan p = parts_plan(a);
   return p.norm + 4 * p.x + 4 * p.aa;
 }

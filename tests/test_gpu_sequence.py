@@ -432,6 +432,13 @@ def test_orthogonalise(eng, shape, dtype):
     _check_orth(eng, 1e-2 * rng.standard_normal(shape), dtype)
 
 
+@pytest.mark.parametrize("shape", [(2, 100, 1501), (1, 1300, 66), (3, 150, 290), (1, 65, 4000)], ids=str)
+def test_orthogonalise_in_64_bits(eng, shape):
+    """Tiled products, the sums over a long side cut into parts."""
+    rng = np.random.default_rng(79)
+    _check_orth(eng, rng.standard_normal(shape), torch.float64)
+
+
 @pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16], ids=str)
 @pytest.mark.parametrize("shape", [(9, 24, 100), (2, 10, 300), (2, 100, 40), (3, 64, 250), (2, 70, 400), (2, 480, 32), (3, 80, 150), (2, 17, 17)], ids=str)
 def test_orthogonalise_on_chip(eng, shape, dtype):
