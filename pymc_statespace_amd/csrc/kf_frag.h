@@ -87,11 +87,12 @@ struct KfF32 {
 
 // Rows of COLS elements in LDS, 64 banks of 4 bytes.  The 16-byte pieces of a row are permuted (by exclusive or) so that what is read
 // or written at a time meets different banks: a piece of 16 neighbouring rows, of which rows 4 to 11 read the next lane group's depth
-// (16-byte reads take the lanes in that order: measured by their conflicts); 32 bytes of 8 rows (16-bit columns); 64 bytes of every
-// fourth row (32-bit columns; rows of 128 bytes meet the same half of the banks there, two cycles).
+// (16-byte reads take the lanes in that order: measured by their conflicts), and 32 bytes of 8 rows for columns.  32-bit elements: only 8
+// pieces are permuted among each other.  16 would leave a sixth of the conflicts, but the reads of columns then need twice as many
+// addresses, and that costs more: gradient of 3 x 333 tokens 59.5 us instead of 58.
 //
 // A lane's part of an address is computed once (KfLanes, in bytes); row, column and depth of the tile come in as constants: rows (a
-// multiple of 16) and whole 16 pieces as an offset, the pieces inside 16 by exclusive or.
+// multiple of 16) and whole TURNS pieces as an offset, the pieces inside by exclusive or.
 struct KfLanes { int row, row_t, col; };
 static __device__ __forceinline__ KfLanes kf_fresh(const KfLanes& x) { return {kf_fresh(x.row), kf_fresh(x.row_t), kf_fresh(x.col)}; }
 template <typename A, int COLS> struct KfTile {
@@ -99,9 +100,10 @@ template <typename A, int COLS> struct KfTile {
   typedef typename A::frag F;
   static constexpr int SZ = sizeof(E), PIECE = 16 / SZ, PIECES = COLS / PIECE;
   static_assert(PIECES >= 4, "a row of 64 bytes at least");
+  static constexpr int TURNS = SZ == 4 ? 8 : 16;  // pieces that are permuted among each other
   static constexpr int turn(int r) {
     const int b1 = (r >> 1) & 1, b2 = (r >> 2) & 1, b3 = (r >> 3) & 1;
-    if (SZ == 4) return PIECES >= 16 ? r & 15 : (b2 ^ b3) * 4 + b3 * 2 + b1;
+    if (SZ == 4) return ((r & 3) << 1) | b2;
     return PIECES >= 16 ? (b2 ^ b3) * 8 + (r & 3) * 2 + b3 : PIECES == 8 ? (b2 ^ b3) * 4 + b1 * 2 + b3 : (b2 ^ b3) * 2 + b3;
   }
   static __device__ __forceinline__ int at(int r, int c) {  // element
@@ -113,7 +115,7 @@ template <typename A, int COLS> struct KfTile {
   // byte address of a lane's part at row r (a multiple of 16) and column c (a multiple of what the lanes' parts span)
   static __device__ __forceinline__ int mix(int lane, int r, int c) {
     const int p = c / PIECE;
-    return (lane ^ ((p & 15) * 16)) + (p >> 4) * 256 + r * (COLS * SZ);
+    return (lane ^ ((p & (TURNS - 1)) * 16)) + (p / TURNS) * (16 * TURNS) + r * (COLS * SZ);
   }
   template <typename X> static __device__ __forceinline__ X read(const E* p, int byte) { return *reinterpret_cast<const X*>(reinterpret_cast<const char*>(p) + byte); }
   template <typename X> static __device__ __forceinline__ void write(E* p, int byte, X x) { *reinterpret_cast<X*>(reinterpret_cast<char*>(p) + byte) = x; }
