@@ -3,7 +3,8 @@
 // Bound by reading and writing S.  One workgroup for each (row, head): a thread holds VEC neighbouring columns of every RP-th row of
 // S, all of them loaded before the first is used, and the sums over the rows meet in LDS.  96 rows (10 % of them empty), 32 heads of
 // 128 x 128: 78 us for 362 MB, 4.6 TB/s, the rate of a large copy.  One row, 8 heads of 64 x 64: 5 us, the latency of a launch and of the
-// loads (4 bytes a lane instead of 16: 91 us and 5 us).  All in fp32; only o is rounded.
+// loads.  A row of S after the other, 4 bytes a lane: 178 us.  V that is no multiple of 4, or a state off its 16 bytes, takes 4 bytes a lane:
+// V = 126 72 us, V = 128 62 (96 rows, none empty, the state in the caches), V = 33 48 us, V = 32 18.  All in fp32; only o is rounded.
 #include "kf_sequence.h"
 
 namespace {
