@@ -34,6 +34,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
   constexpr int WK = KP / 16 < 4 ? KP / 16 : 4, WN = 4 / WK;  // the state's tiles: WK waves along K, WN along V
   constexpr int SM = KP / 16 / WK, SN = NT / WN;
   constexpr int RK = 2048 / KP, RV = 2048 / VT;
+  constexpr int AT = sizeof(typename A::elem) == 2 ? 2 : 1;  // tiles at a time
   __shared__ __attribute__((aligned(16))) E sK[KF_CHUNK * KP];
   __shared__ __attribute__((aligned(16))) E sV[KF_CHUNK * VT];
   __shared__ __attribute__((aligned(16))) E sS[OUT ? VT * KP : 8];  // the state's transpose as an operand
@@ -164,18 +165,32 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
 #pragma unroll
         for (int u = 0; u < KK; ++u) fq[u] = Row::finish(rq[u], 32 * u + 8 * g, a.K, row <= last);
       }
-      // scores, transposed: rows j, columns i; as operands, two tiles each.  (w is the same for a whole wave.)
+      // scores, transposed: rows j, columns i; as operands, two tiles each.  (w is the same for a whole wave.)  Here and below all of a
+      // tile's (bf16: two tiles') operands are asked for before its first product: by itself the compiler asks for one at a time.
       F p[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        kf_f32x4 two[2];
+        kf_f32x4 two[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int y0 = 0; y0 < 2; y0 += AT)
+          if (2 * x + y0 <= w) {
+            F fk[AT][KK];
+#pragma unroll
+            for (int y = 0; y < AT; ++y)
+#pragma unroll
+              for (int u = 0; u < KK; ++u) fk[y][u] = TK::row(sK, lk, 16 * (2 * x + y0 + y), 32 * u);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < KK; ++u)
+#pragma unroll
+              for (int y = 0; y < AT; ++y) two[y0 + y] = A::mma(fk[y][u], fq[u], two[y0 + y]);
+          }
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           const int jt = 2 * x + y;
           kf_f32x4 s = {0, 0, 0, 0};
           if (jt <= w) {
-#pragma unroll
-            for (int u = 0; u < KK; ++u) s = A::mma(TK::row(sK, lk, 16 * jt, 32 * u), fq[u], s);
+            s = two[y];
             if (jt < w) {
               s *= D.from_tile[jt < 3 ? jt : 2][row] * a.scale;
               s *= *reinterpret_cast<const kf_f32x4*>(&D.to_tile_end[16 * jt + 4 * g]);
@@ -205,13 +220,32 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
       for (int u = 0; u < NT; u += 2) {
         kf_f32x4 o[2];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          o[y] = from_state(16 * (u + y));
+        for (int y0 = 0; y0 < 2; y0 += AT) {
+          F fS[AT][KK], fv[AT][2];
+          kf_f32x4 before[AT] = {}, inside[AT] = {};
 #pragma unroll
-          for (int x = 0; x < 2; ++x) o[y] = A::mma(TV::col(sV, lv, 32 * x, 16 * (u + y)), p[x], o[y]);
+          for (int y = 0; y < AT; ++y) {
+#pragma unroll
+            for (int x = 0; x < KK; ++x) fS[y][x] = TK::row(sS, lk, 16 * (u + y0 + y), 32 * x);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) fv[y][x] = TV::col(sV, lv, 32 * x, 16 * (u + y0 + y));
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int x = 0; x < KK; ++x)
+#pragma unroll
+            for (int y = 0; y < AT; ++y) before[y] = A::mma(fS[y][x], fq[x], before[y]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int y = 0; y < AT; ++y) inside[y] = A::mma(fv[y][x], p[x], inside[y]);
+#pragma unroll
+          for (int y = 0; y < AT; ++y) o[y0 + y] = before[y] * fs + inside[y];
+        }
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
           for (int r = 0; r < 4; ++r) check = fmaf(o[y][r], 0.f, check);
-        }
         if (!plain) {  // (a row behind the end has a query of zeros; the state may be infinite all the same)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
