@@ -336,7 +336,7 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(const T* M, long size, d
     s += x * x;
   }
   s = block_sum(s, red);
-  if (threadIdx.x == 0) part[blockIdx.y * NORM_PARTS + blockIdx.x] = s;
+  if (threadIdx.x == 0) part[blockIdx.y * (long)gridDim.x + blockIdx.x] = s;
 }
 // by a whole workgroup, the same order everywhere
 static __device__ __forceinline__ double norm_factor(const double* part, int parts, double eps, double* red) {
@@ -349,6 +349,7 @@ static inline int norm_parts(long size) {  // about 16 elements a thread
   const long p = (size + 4095) / 4096;
   return p < NORM_PARTS ? (int)p : NORM_PARTS;
 }
+static inline size_t norm_bytes(const KfOrthArgs& a) { return kf_seq_round((size_t)a.n * norm_parts((long)a.rows * a.cols) * 8); }
 
 // ------------------------------------------------------------------------------------------------ fp16 parts
 constexpr float SCALE_X = 16384.f;  // 2^14: |x| <= 1.9 comes to 31130 of fp16's 65504
@@ -389,7 +390,7 @@ __global__ __launch_bounds__(256) void orth_parts_kernel(KfOrthArgs a, const dou
   const long z = blockIdx.z, at = z * dP * (long)LP * STORED;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
   __shared__ double red[4];
-  const double f = norm_factor(part + z * NORM_PARTS, parts, a.eps, red) * SCALE_X;
+  const double f = norm_factor(part + z * parts, parts, a.eps, red) * SCALE_X;
   const T* M = (const T*)a.M + z * d * (long)L;
   if (tall) {
     for (int e = threadIdx.x; e < 4096; e += 256) {
@@ -658,7 +659,7 @@ PartsPlan parts_plan(const KfOrthArgs& a) {
   p.LP = (L + 127) / 128 * 128;
   p.x = kf_seq_round((size_t)a.n * p.dP * p.LP * 2);
   p.aa = kf_seq_round((size_t)a.n * p.dP * p.dP * 2);
-  p.norm = kf_seq_round((size_t)a.n * NORM_PARTS * 8);
+  p.norm = norm_bytes(a);
   return p;
 }
 
@@ -748,7 +749,7 @@ int launch_parts(kf_handle* h, const KfOrthArgs& a, const PartsPlan& pl, void* w
 __global__ __launch_bounds__(256) void orth_scale64_kernel(KfOrthArgs a, const double* part, int parts, double* X) {
   __shared__ double red[4];
   const long e = (long)blockIdx.x * 256 + threadIdx.x, size = (long)a.rows * a.cols, z = blockIdx.y, i = z * size + e;
-  const double f = norm_factor(part + z * NORM_PARTS, parts, a.eps, red);
+  const double f = norm_factor(part + z * parts, parts, a.eps, red);
   if (e >= size) return;
   X[a.rows > a.cols ? z * size + (e % a.cols) * a.rows + e / a.cols : i] = ((const double*)a.M)[i] * f;
 }
@@ -902,7 +903,7 @@ int launch64(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {
   const int d = tall ? a.cols : a.rows, L = tall ? a.rows : a.cols;
   const size_t big = kf_seq_round((size_t)a.n * d * L * 8), small = kf_seq_round((size_t)a.n * d * d * 8);
   char* w = (char*)ws;
-  double* norm = (double*)w; w += kf_seq_round((size_t)a.n * NORM_PARTS * 8);
+  double* norm = (double*)w; w += norm_bytes(a);
   double* X = (double*)w; w += big;
   double* Y = (double*)w; w += big;
   double* A = (double*)w; w += small;
@@ -949,7 +950,7 @@ size_t kf_orthogonalise_ws(const kf_handle* h, const KfOrthArgs& a) {
   if (kf_orthogonalise_on_chip(a)) return 0;
   const size_t d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
   if (a.dtype == KF_DTYPE_F64)
-    return kf_seq_round((size_t)a.n * NORM_PARTS * 8) + 2 * kf_seq_round((size_t)a.n * d * L * 8) + 2 * kf_seq_round((size_t)a.n * d * d * 8) +
+    return norm_bytes(a) + 2 * kf_seq_round((size_t)a.n * d * L * 8) + 2 * kf_seq_round((size_t)a.n * d * d * 8) +
            cut64(h, a.n, (int)d, (int)L);
   const PartsPlan p = parts_plan(a);
   return p.norm + 4 * p.x + 4 * p.aa;
