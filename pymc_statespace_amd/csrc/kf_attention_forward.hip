@@ -208,12 +208,6 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
       const long t = t0 + row;
       T* out = (T*)a.o + ((b * a.T + t) * a.H + h) * (long)a.V + v0;
       // columns 16 u .. 16 u + 31 of V as two tiles, of which a lane has 8 neighbours: 16 u + 8 g .. + 7
-      auto from_state = [&](int v1) {
-        kf_f32x4 o = {0, 0, 0, 0};
-#pragma unroll
-        for (int x = 0; x < KK; ++x) o = A::mma(TK::row(sS, lk, v1, 32 * x), fq[x], o);
-        return o * fs;
-      };
       KfOut8<T> ready[NT / 2];
       float check = 0.f;
 #pragma unroll
@@ -258,13 +252,17 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
       const bool strange = __any(check != 0.f);  // something is not finite
       if (strange) {
         // A token's infinity or NaN in v would reach the rows before it as 0 x inf: the products once more without such values, and
-        // these added only to the rows from their token on.
+        // these added only to the rows from their token on.  (The same operations as above: rows that no such value reaches keep their bits.)
 #pragma unroll 1
         for (int v1 = 0; v1 < VT; v1 += 16) {
-          kf_f32x4 o = from_state(v1);
+          kf_f32x4 before = {0, 0, 0, 0}, inside = {0, 0, 0, 0};
+#pragma unroll
+          for (int x = 0; x < KK; ++x) before = A::mma(TK::row(sS, lk, v1, 32 * x), fq[x], before);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) inside = A::mma(A::finite(TV::col(sV, lv, 32 * x, v1)), p[x], inside);
+          kf_f32x4 o = before * fs + inside;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            o = A::mma(A::finite(TV::col(sV, lv, 32 * x, v1)), p[x], o);
 #pragma unroll 1
             for (int j = 0; j < 32; ++j) {  // token 32 x + j: value e = 4 (j / 16) + j % 4 of lane group (j % 16) / 4
               float pj = 0.f;
