@@ -116,8 +116,8 @@ def _check_backward(eng, p, dtype, lengths=None):
         _near(got["initial_state"], ref["initial_state"], n * mag["initial_state"] + 1e-30, "dS0")
     else:
         assert got["initial_state"] is None
-    # d log a: pairs inside a chunk are summed as a running difference, of the size of what the chunk's tokens read and write.  In
-    # the products with the state 16-bit types take the state in two halves, 2 x 8 bits: 2^-17 of the terms
+    # d log a: pairs inside a chunk are summed as a running difference, of the size of what the chunk's tokens read and write.  (In
+    # the products with the states 16-bit types take them in exact parts: nothing is added to the sums' own roundings.)
     per = H // G
     aq, ak = np.repeat(_abs(p["q"]), per, 2), np.repeat(_abs(p["k"]), per, 2)
     single = sn.attention_gradient(aq, ak, _abs(p["v"]), np.broadcast_to(p["log_decay"], (B, T, H)), _abs(p["g_o"]), p["scale"],
@@ -125,7 +125,7 @@ def _check_backward(eng, p, dtype, lengths=None):
     size = (aq * single["q"]).sum(-1) + (ak * single["k"]).sum(-1)
     size = np.concatenate([size, np.zeros((B, 64, H))], 1)
     size = np.stack([size[:, t:t + 64].sum(1) for t in range(T)], 1) + single["log_decay"]
-    bound = (n + (0 if dtype == torch.float32 else 2.0 ** -17)) * size
+    bound = n * size
     if p["log_decay"].ndim == 1:
         bound = bound.sum((0, 1))
     _near(got["log_decay"], ref["log_decay"], bound + 1e-30, "d log_decay")
