@@ -19,8 +19,8 @@
 // 8 waves go through the chunk's phases together: 1590 vector instructions a wave and chunk (split operands: 440) are 41 % of its time,
 // LDS 20 %, the matrix pipe 19 %, waits 40 %.  Without the fences between depths the compiler holds all of them at once and spills: 325 us.
 //
-// Launches: (1) where the time axis is cut into segments, what each segment adds to S and to R; (2) S at every chunk's start, kept
-// as the accumulators that hold it; (3) the chunks of each segment from its last to its first, R in registers; (4) sums over
+// Launches: (1) where the time axis is cut into segments, what each segment adds to S and to R; (2) where segments have several chunks,
+// S at every chunk's start, kept as the accumulators that hold it; (3) the chunks of each segment from its last to its first, R in registers; (4) sums over
 // the heads that share queries and keys, and over tokens for fixed decays.
 #include "kf_attention_chunk.h"
 
@@ -279,16 +279,38 @@ __global__ __launch_bounds__(4 * D, 2) void attention_gradient_kernel(KfAttnArgs
     rv.load(v, a.vs[1], c * C, n, a.V);
     rd.load(go, a.gs[1], c * C, n, a.V);
   };
-  auto load_start = [&](long c) {
-    const kf_f32x4* in = sp.starts + (bh * sp.chunks + c) * (D / 32 * 2 * TH) + tid;
+  const bool single = sp.seg_chunks == 1;
+  auto load_start = [&](long c) {  // (a segment of one chunk: not asked for, but loaded without a branch, the same line each time)
+    const kf_f32x4* in = sp.starts + (single ? 0 : (bh * sp.chunks + c) * (D / 32 * 2 * TH)) + tid;
+    const int step = single ? 0 : TH;
 #pragma unroll
-    for (int u = 0; u < NT; ++u) S0[u] = in[u * TH];
+    for (int u = 0; u < NT; ++u) S0[u] = in[u * step];
   };
   const long ld_step = a.per_token ? a.H : 0;
   auto decay_of = [&](long c) { return ld[(c * C + l < 0 ? 0 : c * C + l < n ? c * C + l : n - 1) * ld_step]; };  // (in bounds for any c)
   if (last > c0) {
     load(last - 1);
-    load_start(last - 1);
+    if (single) {
+      // the state at the segment's start, as the sweep over starts has it
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        S0[t] = kf_f32x4{0, 0, 0, 0};
+        const int kk = 16 * w + i;
+        if (a.s0 && kk < a.K) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * t + 4 * g + r < a.V) S0[t][r] = a.s0[(bh * a.K + kk) * a.V + 16 * t + 4 * g + r];
+        }
+      }
+      for (int s = summed && seg ? seg - 1 : 0; s < seg; ++s) {
+        const float f = summed ? sp.products_s[bh * (sp.segments - 1) + s] : sp.factors[bh * sp.segments + s];
+        const kf_f32x4* u = reinterpret_cast<const kf_f32x4*>(sp.adds_s) + (bh * (sp.segments - 1) + s) * (D * D / 4) + tid;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) S0[t] = S0[t] * f + u[t * TH];
+      }
+    } else {
+      load_start(last - 1);
+    }
     rg = decay_of(last - 2);
     if (w == 0) dec[0].fill(decay_of(last - 1), l < C && (last - 1) * C + l < n);
   }
@@ -552,7 +574,7 @@ Plan plan(const kf_handle* h, const KfAttnArgs& a) {
   p.adds = kf_seq_round(rows * (s.segments - 1) * state);
   p.factors = kf_seq_round((size_t)rows * s.segments * 4);
   p.products = kf_seq_round((size_t)rows * (s.segments - 1) * 4);
-  p.starts = kf_seq_round((size_t)rows * s.chunks * state);
+  p.starts = kf_seq_round(s.seg_chunks > 1 ? (size_t)rows * s.chunks * state : (size_t)4 * p.D * 16);
   p.part = a.G != a.H ? kf_seq_round((size_t)a.B * a.T * a.H * a.K * 4) : 0;
   p.decay = a.per_token ? 0 : kf_seq_round((size_t)rows * s.segments * 8);
   return p;
@@ -572,7 +594,9 @@ int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream)
     if (s.segments > KF_FUSED_SEGMENTS)
       kf_attention_scan(s.adds_s, s.adds_r, s.factors, s.products_s, s.products_r, a.B * a.H, s.segments - 1, (long)D * D, s.segments, stream);
   }
-  hipLaunchKernelGGL((attention_sweep_kernel<A, T, D, MODE, true>), dim3(kf_xcd_grid(s.works)), dim3(4 * D), 0, stream, a, s);
+  // (segments of one chunk start from what the first launch left: 16 x 128 tokens, 8 heads of 64 x 64, fp16, 31 us with this launch,
+  // 26 without; 3 x 333 tokens, fp32, 58 and 52)
+  if (s.seg_chunks > 1) hipLaunchKernelGGL((attention_sweep_kernel<A, T, D, MODE, true>), dim3(kf_xcd_grid(s.works)), dim3(4 * D), 0, stream, a, s);
   KF_HIP_CHECK(h, hipFuncSetAttribute(reinterpret_cast<const void*>(attention_gradient_kernel<A, T, D, MODE>),
                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   hipLaunchKernelGGL((attention_gradient_kernel<A, T, D, MODE>), dim3(kf_xcd_grid(s.works)), dim3(4 * D), lds, stream, a, s);
