@@ -519,30 +519,31 @@ __global__ __launch_bounds__(4 * D, 2) void attention_gradient_kernel(KfAttnArgs
   }
 }
 
-// sums a group's heads into the type of q / k
+// What is summed over workgroups: a group's heads, into the type of q and k (the first 2 `blocks` workgroups, if heads share them), and,
+// for fixed decays, sequences and segments, one wave for each head (the rest).
 template <typename T>
-__global__ __launch_bounds__(256) void attention_group_kernel(KfAttnArgs a, const float* part_q, const float* part_k) {
-  const long total = a.B * a.T * a.G * a.K;
-  const float* part = blockIdx.y ? part_k : part_q;
-  const int per = a.H / a.G;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256l) {
-    const int c = (int)(i % a.K);
-    const long row = i / a.K, bt = row / a.G;
-    const int g = (int)(row - bt * a.G);
-    float s = 0.f;
-    for (int j = 0; j < per; ++j) s += part[(bt * a.H + g * per + j) * a.K + c];
-    ((T*)(blockIdx.y ? a.g_k : a.g_q))[i] = kf_from_float<T>(s);
-  }
-}
-
-// fixed decays: sums over sequences and segments, one wave for each head
-__global__ __launch_bounds__(64) void attention_decay_kernel(KfAttnArgs a, const double* part, int segments) {
-  const int h = blockIdx.x;
-  double s = 0.;
-  for (long x = threadIdx.x; x < a.B * segments; x += 64) s += part[((x / segments) * a.H + h) * segments + x % segments];
+__global__ __launch_bounds__(256) void attention_join_kernel(KfAttnArgs a, const float* part_q, const float* part_k, const double* part_decay, unsigned blocks, int segments) {
+  if (blockIdx.x < 2 * blocks) {
+    const long total = a.B * a.T * a.G * a.K;
+    const bool second = blockIdx.x >= blocks;
+    const float* part = second ? part_k : part_q;
+    const int per = a.H / a.G;
+    for (long i = (long)(blockIdx.x - (second ? blocks : 0)) * 256 + threadIdx.x; i < total; i += blocks * 256l) {
+      const int c = (int)(i % a.K);
+      const long row = i / a.K, bt = row / a.G;
+      const int g = (int)(row - bt * a.G);
+      float s = 0.f;
+      for (int j = 0; j < per; ++j) s += part[(bt * a.H + g * per + j) * a.K + c];
+      ((T*)(second ? a.g_k : a.g_q))[i] = kf_from_float<T>(s);
+    }
+  } else if (threadIdx.x < 64) {
+    const int h = (int)(blockIdx.x - 2 * blocks);
+    double s = 0.;
+    for (long x = threadIdx.x; x < a.B * segments; x += 64) s += part_decay[((x / segments) * a.H + h) * segments + x % segments];
 #pragma unroll
-  for (int m = 1; m < 64; m *= 2) s += __shfl_xor(s, m);
-  if (threadIdx.x == 0) a.g_decay[h] = (float)s;
+    for (int m = 1; m < 64; m *= 2) s += __shfl_xor(s, m);
+    if (threadIdx.x == 0) a.g_decay[h] = (float)s;
+  }
 }
 
 struct Plan {
@@ -600,11 +601,10 @@ int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream)
   KF_HIP_CHECK(h, hipFuncSetAttribute(reinterpret_cast<const void*>(attention_gradient_kernel<A, T, D, MODE>),
                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   hipLaunchKernelGGL((attention_gradient_kernel<A, T, D, MODE>), dim3(kf_xcd_grid(s.works)), dim3(4 * D), lds, stream, a, s);
-  if (a.G != a.H) {
-    const long blocks = (a.B * a.T * a.G * a.K + 255) / 256;
-    hipLaunchKernelGGL(attention_group_kernel<T>, dim3((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20), 2), dim3(256), 0, stream, a, s.part_q, s.part_k);
-  }
-  if (!a.per_token) hipLaunchKernelGGL(attention_decay_kernel, dim3(a.H), dim3(64), 0, stream, a, s.part_decay, s.segments);
+  const long cells = (a.B * a.T * a.G * a.K + 255) / 256;
+  const unsigned blocks = a.G == a.H ? 0 : (unsigned)(cells < 1 << 20 ? cells : 1 << 20), heads = a.per_token ? 0 : (unsigned)a.H;
+  if (blocks || heads)
+    hipLaunchKernelGGL(attention_join_kernel<T>, dim3(2 * blocks + heads), dim3(256), 0, stream, a, s.part_q, s.part_k, s.part_decay, blocks, s.segments);
   KF_HIP_CHECK(h, hipGetLastError());
   return KF_OK;
 }
