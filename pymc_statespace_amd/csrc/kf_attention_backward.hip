@@ -99,6 +99,13 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
   const long c0 = (long)seg * sp.seg_chunks, c1 = c0 + sp.seg_chunks < sp.chunks ? c0 + sp.seg_chunks : sp.chunks;
   const long live = (n + C - 1) / C, last = c1 < live ? c1 : live;  // chunks that hold tokens: c0 .. last - 1
 
+  // tiles of nothing but padding are not kept; where one would be read, the first one is, which is there already, and left out
+  auto real = [&](int t) { return 16 * t < a.V && 16 * w < a.K; };
+  auto add = [&](kf_f32x4& x, float f, const kf_f32x4* u, int t) {
+    const kf_f32x4 y = u[real(t) ? t * TH : 0];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = real(t) ? x[r] * f + y[r] : x[r];
+  };
   kf_f32x4 acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -116,7 +123,7 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
       const float f = summed ? sp.products_s[bh * (sp.segments - 1) + s] : sp.factors[bh * sp.segments + s];
       const kf_f32x4* u = reinterpret_cast<const kf_f32x4*>(sp.adds_s) + (bh * (sp.segments - 1) + s) * (D * D / 4) + tid;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t] = acc[t] * f + u[t * TH];
+      for (int t = 0; t < NT; ++t) add(acc[t], f, u, t);
     }
   }
   float through = 1.f;
@@ -175,7 +182,8 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
   if (!STARTS) {
     kf_f32x4* u = reinterpret_cast<kf_f32x4*>(back ? sp.adds_r : sp.adds_s) + (bh * (sp.segments - 1) + s0) * (D * D / 4) + tid;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) u[t * TH] = acc[t];
+    for (int t = 0; t < NT; ++t)
+      if (real(t)) u[t * TH] = acc[t];
     // (each segment's decay from one of the sweeps that pass through it: the first from S, the others from R)
     if (tid == 0 && (back || s0 == 0)) sp.factors[bh * sp.segments + seg] = through;
   }
@@ -230,6 +238,12 @@ __global__ __launch_bounds__(4 * D, 2) void attention_gradient_kernel(KfAttnArgs
   const long live = (n + C - 1) / C, last = c1 < live ? c1 : live;
   const bool shared_heads = a.G != a.H;
 
+  auto real = [&](int t) { return 16 * t < a.V && 16 * w < a.K; };
+  auto add = [&](kf_f32x4& x, float f, const kf_f32x4* u, int t) {  // as in the sweeps
+    const kf_f32x4 y = u[real(t) ? t * TH : 0];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = real(t) ? x[r] * f + y[r] : x[r];
+  };
   kf_f32x4 R[NT];  // rows v, columns k
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -246,7 +260,7 @@ __global__ __launch_bounds__(4 * D, 2) void attention_gradient_kernel(KfAttnArgs
     const float f = summed ? sp.products_r[bh * (sp.segments - 1) + s - 1] : sp.factors[bh * sp.segments + s];
     const kf_f32x4* u = reinterpret_cast<const kf_f32x4*>(sp.adds_r) + (bh * (sp.segments - 1) + s - 1) * (D * D / 4) + tid;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) R[t] = R[t] * f + u[t * TH];
+    for (int t = 0; t < NT; ++t) add(R[t], f, u, t);
   }
 
   // gradients of rows behind the sequence's end
@@ -306,7 +320,7 @@ __global__ __launch_bounds__(4 * D, 2) void attention_gradient_kernel(KfAttnArgs
         const float f = summed ? sp.products_s[bh * (sp.segments - 1) + s] : sp.factors[bh * sp.segments + s];
         const kf_f32x4* u = reinterpret_cast<const kf_f32x4*>(sp.adds_s) + (bh * (sp.segments - 1) + s) * (D * D / 4) + tid;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) S0[t] = S0[t] * f + u[t * TH];
+        for (int t = 0; t < NT; ++t) add(S0[t], f, u, t);
       }
     } else {
       load_start(last - 1);
@@ -593,7 +607,7 @@ int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, hipStream_t stream)
     two.works = 2 * (s.works / s.segments) * (s.segments - 1);
     hipLaunchKernelGGL((attention_sweep_kernel<A, T, D, MODE, false>), dim3(kf_xcd_grid(two.works)), dim3(4 * D), 0, stream, a, two);
     if (s.segments > KF_FUSED_SEGMENTS)
-      kf_attention_scan(s.adds_s, s.adds_r, s.factors, s.products_s, s.products_r, a.B * a.H, s.segments - 1, (long)D * D, s.segments, stream);
+      kf_attention_scan(s.adds_s, s.adds_r, s.factors, s.products_s, s.products_r, a.B * a.H, s.segments - 1, (long)D * D, s.segments, 4 * D, a.V, a.K, stream);
   }
   // (segments of one chunk start from what the first launch left: 16 x 128 tokens, 8 heads of 64 x 64, fp16, 31 us with this launch,
   // 26 without; 3 x 333 tokens, fp32, 58 and 52)

@@ -68,13 +68,18 @@ struct KfChunkDecay {
 // (about 0.4 us for each 64 KB); beyond, this kernel (4 to 6 us) is the shorter way and keeps the sum linear in their number.
 constexpr int KF_FUSED_SEGMENTS = 8;
 static __global__ __launch_bounds__(256) void kf_attention_scan_kernel(kf_f32x4* adds_s, kf_f32x4* adds_r, const float* factors, float* products_s,
-                                                                       float* products_r, long heads, int n, long cells, int factor_stride) {
+                                                                       float* products_r, long heads, int n, long cells, int factor_stride,
+                                                                       int threads, int V, int K) {
   const long x = (long)blockIdx.x * 256 + threadIdx.x;
   if (x >= heads * cells) return;
   const bool back = blockIdx.y;  // (the gradient's second state)
   kf_f32x4* adds = back ? adds_r : adds_s;
   float* products = back ? products_r : products_s;
   const long head = x / cells, e = x - head * cells;
+  if (threads) {  // (the gradient's states: tile e / threads of V, tile of K by wave; those of nothing but padding are not kept)
+    const int t = (int)(e / threads), w = (int)(e - (long)t * threads) >> 6;
+    if (16 * t >= V || 16 * w >= K) return;
+  }
   kf_f32x4* a = adds + head * n * cells + e;
   const float* f = factors + head * factor_stride + (back ? 1 : 0);
   kf_f32x4 sum = {0, 0, 0, 0};
@@ -100,9 +105,9 @@ static __global__ __launch_bounds__(256) void kf_attention_scan_kernel(kf_f32x4*
   }
 }
 static inline void kf_attention_scan(float* adds_s, float* adds_r, const float* factors, float* products_s, float* products_r, long heads, int n,
-                                     long floats, int factor_stride, hipStream_t stream) {
+                                     long floats, int factor_stride, int threads, int V, int K, hipStream_t stream) {
   hipLaunchKernelGGL(kf_attention_scan_kernel, dim3((unsigned)((heads * (floats / 4) + 255) / 256), adds_r ? 2 : 1), dim3(256), 0, stream,
-                     (kf_f32x4*)adds_s, (kf_f32x4*)adds_r, factors, products_s, products_r, heads, n, floats / 4, factor_stride);
+                     (kf_f32x4*)adds_s, (kf_f32x4*)adds_r, factors, products_s, products_r, heads, n, floats / 4, factor_stride, threads, V, K);
 }
 
 struct KfAttnSplit {

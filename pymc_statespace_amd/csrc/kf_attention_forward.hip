@@ -383,7 +383,7 @@ int launch(kf_handle* h, const KfAttnArgs& a, const Plan& p, void* ws, hipStream
     s.works = p.sp.works / p.sp.segments * (p.sp.segments - 1);
     hipLaunchKernelGGL((attention_chunk_kernel<A, T, KP, VT, MODE, false>), dim3(kf_xcd_grid(s.works)), dim3(256), 0, stream, a, s, adds, factors, products);
     if (s.segments > KF_FUSED_SEGMENTS)
-      kf_attention_scan(adds, nullptr, factors, products, nullptr, a.B * a.H, s.segments - 1, (long)s.v_tiles * KP * VT, s.segments - 1, stream);
+      kf_attention_scan(adds, nullptr, factors, products, nullptr, a.B * a.H, s.segments - 1, (long)s.v_tiles * KP * VT, s.segments - 1, 0, 0, 0, stream);
   }
   hipLaunchKernelGGL((attention_chunk_kernel<A, T, KP, VT, MODE, true>), dim3(kf_xcd_grid(p.sp.works)), dim3(256), 0, stream, a, p.sp, adds, factors, products);
   KF_HIP_CHECK(h, hipGetLastError());
