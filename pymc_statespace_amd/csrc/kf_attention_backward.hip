@@ -14,8 +14,8 @@
 // and R -- is multiplied in three exact parts.  fp32 and fp16 data: fp32 throughout.
 //
 // Measured: 4 x 2048 tokens, 16 heads of 128 x 128, bf16: 41 + 40 + 117 us (187 without a profiler) for 236 MB (50 us at the 4.7 TB/s of a large copy); 134 MB of
-// starts are written and read on top.  16 x 128 tokens, 8 heads of 64 x 64, fp16: 9 + 6 + 17 us.  3 x 333 ragged tokens, 6 heads of 40 x 72
-// on 2 groups, fp32: 13 + 9 + 7 + 23 + 4 + 4 us.  The gradient kernel has one workgroup on a compute unit (148 KB of LDS, 256 registers), whose
+// starts are written and read on top.  16 x 128 tokens, 8 heads of 64 x 64, fp16: 9 + 18 us.  3 x 333 ragged tokens, 6 heads of 40 x 72
+// on 2 groups, fp32: 12 + 7 + 24 + 4 us.  The gradient kernel has one workgroup on a compute unit (148 KB of LDS, 256 registers), whose
 // 8 waves go through the chunk's phases together: 1590 vector instructions a wave and chunk (split operands: 440) are 41 % of its time,
 // LDS 20 %, the matrix pipe 19 %, waits 40 %.  Without the fences between depths the compiler holds all of them at once and spills: 325 us.
 //
