@@ -1762,16 +1762,15 @@ extern "C" int kf_orthogonalise_workspace(kf_handle* h, int64_t n, int32_t rows,
 static double quintic_top(const double* p, double top) {
   const double a = p[0], b = p[1], c = p[2];
   double best = fabs(top * (a + top * top * (b + c * top * top)));
+  // Both roots without a difference of nearly equal numbers: the larger of -3 b and its root of the discriminant is kept (t), the other
+  // root is a / t.  (With a small c, (-3 b + sqrt) / (10 c) is 0 or nothing but rounding; c = 0 leaves the cubic's own, a / t.)
   double u[2];
   int n = 0;
-  if (c != 0.0) {
-    const double disc = 9 * b * b - 20 * a * c;
-    if (disc >= 0) {
-      u[n++] = (-3 * b + sqrt(disc)) / (10 * c);
-      u[n++] = (-3 * b - sqrt(disc)) / (10 * c);
-    }
-  } else if (b != 0.0) {
-    u[n++] = -a / (3 * b);
+  const double disc = 9 * b * b - 20 * a * c;
+  if (disc >= 0) {
+    const double t = -0.5 * (3 * b + copysign(sqrt(disc), b));
+    if (c != 0.0) u[n++] = t / (5 * c);
+    if (t != 0.0) u[n++] = a / t;
   }
   for (int i = 0; i < n; ++i)
     if (u[i] > 0 && u[i] < top * top) {

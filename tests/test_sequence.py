@@ -174,6 +174,32 @@ def test_coefficients_that_are_refused(lib, handle):
     assert call([(6.0, -6.0, 0.0)]) == -1       # 2.31 there, 0 at both ends
 
 
+@pytest.mark.parametrize("coef", [(6.0, -6.0, 1e-17), (100.0, -100.0, 1e-16), (100.0, -100.0, -1e-16), (6.0, -6.0, 1e-300), (-6.0, 6.0, 1e-17)])
+def test_a_quintic_that_is_nearly_a_cubic_is_refused(lib, handle, coef):
+    """The maximum inside the interval is found however small the quintic's own coefficient: 2.31 and 38 at s = 0.577."""
+    one, two = C.c_void_p(16), C.c_void_p(1 << 20)
+    assert lib.kf_orthogonalise(handle, 1, 96, 96, 1, 1, (C.c_double * 3)(*coef), 1e-7, one, two, one, 1 << 40, None) == -1
+    assert b"singular value" in lib.kf_last_error(handle)
+
+
+def test_the_bound_of_a_step_is_its_polynomials_maximum(lib, handle):
+    """Random lists: refused exactly where a fine grid finds a value above the bound in some step.  (The workspace is left out, so that
+    a list that is taken ends there.)"""
+    rng = np.random.default_rng(6)
+    one, two = C.c_void_p(16), C.c_void_p(1 << 20)
+    taken = 0
+    for _ in range(2000):
+        coef = rng.uniform(-6, 6, 3) * np.where(rng.random(3) < 0.5, 1.0, 10.0 ** -rng.integers(0, 18, 3))
+        s = np.linspace(0.0, 1.0, 4001)
+        top = np.abs(s * (coef[0] + s * s * (coef[1] + s * s * coef[2]))).max()
+        if 1.85 < top < 2.05:  # (on the bound, or a grid's step away from it)
+            continue
+        rc = lib.kf_orthogonalise(handle, 1, 96, 96, 1, 1, (C.c_double * 3)(*coef), 1e-7, one, two, None, 0, None)
+        assert rc == (-3 if top < 1.9 else -1), (coef, top)
+        taken += rc == -3
+    assert 200 < taken < 1900
+
+
 # ---------------------------------------------------------------------------------------------- refusals, in the engine
 @pytest.fixture
 def engine():
