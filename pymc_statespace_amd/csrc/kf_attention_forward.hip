@@ -273,7 +273,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                   const float z = A::get(sV + TV::at(32 * x + j, v1 + 4 * g + r));
-                  if (!(fabsf(z) <= 3.4e38f)) o[r] += pj * z;
+                  if (!kf_finite(z)) o[r] += pj * z;
                 }
             }
           }

@@ -39,6 +39,7 @@ static __device__ __forceinline__ float kf_row_sum(float x) {
 
 static __device__ __forceinline__ unsigned kf_bits(float x) { return __builtin_bit_cast(unsigned, x); }
 static __device__ __forceinline__ float kf_float_of(unsigned x) { return __builtin_bit_cast(float, x); }
+static __device__ __forceinline__ bool kf_finite(float x) { return (kf_bits(x) & 0x7f800000u) != 0x7f800000u; }
 // two floats rounded to nearest even, packed (v_cvt_pk_bf16_f32)
 typedef __bf16 kf_bf16x2 __attribute__((ext_vector_type(2)));
 typedef float kf_f32x2 __attribute__((ext_vector_type(2)));
@@ -79,7 +80,7 @@ struct KfF32 {
   static __device__ __forceinline__ float value(frag a, int e) { return a[e]; }
   static __device__ __forceinline__ frag finite(frag a) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a[e] = (kf_bits(a[e]) & 0x7f800000u) == 0x7f800000u ? 0.f : a[e];
+    for (int e = 0; e < 8; ++e) a[e] = kf_finite(a[e]) ? a[e] : 0.f;
     return a;
   }
   static __device__ __forceinline__ float get(const elem* p) { return *p; }

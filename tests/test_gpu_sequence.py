@@ -234,6 +234,38 @@ def test_a_later_token_never_reaches_an_earlier_one(eng, dtype, name, value):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("sign", [1, -1])
+def test_values_up_to_the_types_largest_next_to_a_nan(eng, dtype, sign):
+    """A value of the type's largest size is finite: beside a token that is not, it counts once, as without that token."""
+    t, at = TYPES[dtype], 83
+    p = _make(18, 1, 150, 1, 2, 24, 40, t)
+    # weights exp(..) s (q . k) below 1 / 8, and a state that stays finite: |k| <= 1e-3
+    p["k"] = torch.from_numpy(1e-3 * np.clip(p["k"], -1, 1)).to(t).double().numpy()
+    p["q"] = torch.from_numpy(np.clip(p["q"], -1, 1)).to(t).double().numpy()
+    p["s0"] = None
+    p["v"][0, 70, :, ::3] = sign * torch.finfo(t).max
+    want, _ = _forward(eng, p, t)
+    assert torch.isfinite(want).all() and float(want[0, 70:].abs().max()) > 1.0
+    p["v"][0, at] = np.nan
+    got, _ = _forward(eng, p, t)
+    assert torch.equal(got[:, :at], want[:, :at])
+    assert torch.isnan(got[:, at:]).all()
+    # and in rows that see both: the NaN reaches one head's columns only where it stands
+    p["v"][0, at] = 0.0
+    clean, _ = _forward(eng, p, t)
+    p["v"][0, at, 0, 1] = np.inf
+    got, _ = _forward(eng, p, t)
+    keep = np.arange(40) != 1
+    # columns without the infinity: the same sums, their terms in another order (the products, and what is added to them)
+    off = (got[:, :, 0][..., keep].double() - clean[:, :, 0][..., keep].double()).abs()
+    u = _u(t)
+    ao, _ = sn.attention(_abs(p["q"]), _abs(p["k"]), np.where(np.isfinite(p["v"]), np.abs(p["v"]), 0.0), p["log_decay"], p["scale"])
+    bound = torch.from_numpy(2 * (u + (0 if t == torch.float32 else 2 * u) + _terms(150, 24, 40) * U32) * ao[:, :, 0][..., keep]).cuda() + 2 * _least(t)
+    assert (off <= bound).all()
+    assert torch.equal(got[:, :, 1], clean[:, :, 1])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_views_of_a_fused_projection(eng, dtype):
     """q, k, v as slices of one tensor, heads before tokens, odd offsets: strides are read, nothing is assumed of alignment."""
     t, p = TYPES[dtype], _make(9, 2, 77, 2, 4, 24, 40, TYPES[dtype])
