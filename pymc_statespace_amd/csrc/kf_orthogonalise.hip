@@ -13,6 +13,10 @@
 // only: the products' rounding (2^-12 a factor) then stays below that of the bf16 result, 1.1e-3 to 1.8e-3 against 1.7e-3 of |X|, also
 // where M is of low rank (X in one part grows its rounding by a for each step in the missing directions: 4e-2 there).
 //
+// Where |M|_F is far below eps, X starts far below 1 and its parts would leave fp16's range at the lower end (|M| = 1e-7 eps, 150 x 200 in
+// fp32: 1.8e-3 off).  Each matrix then carries 2^k X, with k >= 0 from its norm, and k falls by what a step can grow X by until it is 0: with
+// Y = 2^k X a step is a Y + (4^-k b (YY') + 16^-k c (YY')^2) Y.  k = 0 multiplies by 1: no bit of other matrices changes.
+//
 // Measured: one 4096 x 4096 in fp32 3.7 ms, at 1101 TFLOP/s (the fp16 rate of a large library product) its 4.1 TFLOP take 3.75 ms; its fp32
 // library products 14.5 ms.  Four of 768 x 2048 in bf16 221 us, 74 at that rate: with 312 tiles of 64 (A, B) and 384 of 128 (X) for 256
 // compute units, the units that have two bound each product by the 64 bytes a cycle they can read, 15 + 8 + 22 us a step.
@@ -339,11 +343,12 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(const T* M, long size, d
   if (threadIdx.x == 0) part[blockIdx.y * (long)gridDim.x + blockIdx.x] = s;
 }
 // by a whole workgroup, the same order everywhere
-static __device__ __forceinline__ double norm_factor(const double* part, int parts, double eps, double* red) {
+static __device__ __forceinline__ double norm_factor(const double* part, int parts, double eps, double* red, double* norm = nullptr) {
   double s = 0.;
   for (int x = threadIdx.x; x < parts; x += blockDim.x) s += part[x];
-  s = block_sum(s, red);
-  return 1.0 / (sqrt(s) + eps);
+  s = sqrt(block_sum(s, red));
+  if (norm) *norm = s;
+  return 1.0 / (s + eps);
 }
 static inline int norm_parts(long size) {  // about 16 elements a thread
   const long p = (size + 4095) / 4096;
@@ -381,16 +386,21 @@ template <typename T> static __device__ __forceinline__ void store_row(T* to, f4
   }
 }
 
-// M (rows x cols) times its factor, in parts: dP x LP, zeros behind d and L, transposed where M is tall
+// M (rows x cols) times its factor, in parts: dP x LP, zeros behind d and L, transposed where M is tall; shift: each matrix's first k
 template <typename T, int STORED>
-__global__ __launch_bounds__(256) void orth_parts_kernel(KfOrthArgs a, const double* part, int parts, int dP, int LP, _Float16* hi, _Float16* lo) {
+__global__ __launch_bounds__(256) void orth_parts_kernel(KfOrthArgs a, const double* part, int parts, int dP, int LP, _Float16* hi, _Float16* lo,
+                                                         int* shift) {
   __shared__ float tile[64][65];
   const bool tall = a.rows > a.cols;
   const int d = tall ? a.cols : a.rows, L = tall ? a.rows : a.cols;
   const long z = blockIdx.z, at = z * dP * (long)LP * STORED;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
   __shared__ double red[4];
-  const double f = norm_factor(part + z * parts, parts, a.eps, red) * SCALE_X;
+  double norm, f = norm_factor(part + z * parts, parts, a.eps, red, &norm);
+  const double size = norm * f;  // |X|_F; 2^k of it in [1/2, 1)
+  const int k = size > 0. && size < 0.5 ? -1 - ilogb(size) : 0;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) shift[z] = k;
+  f = ldexp(f * SCALE_X, k);
   const T* M = (const T*)a.M + z * d * (long)L;
   if (tall) {
     for (int e = threadIdx.x; e < 4096; e += 256) {
@@ -445,6 +455,8 @@ struct Product {
   int tall;
   float unscale;            // accumulator -> the output's scale
   float add;                // factor of what is added
+  const int* shift;         // each matrix's first k; in this step it is lower by k_before, in the next one by k_after (not below 0)
+  int k_before, k_after;
 };
 
 // out = unscale P Q + add D, TILE x TILE of it for each workgroup of 2 x 2 waves.  Depth in steps of BK through a ring of LDS buffers
@@ -465,6 +477,7 @@ static __device__ __forceinline__ void product_tile(const Product& p, const long
   const long ldP = MODE == GRAM ? p.LP : p.dP, ldQ = MODE == POLY ? p.dP : p.LP;
   const _Float16* P = p.P + z * PARTS * (long)p.dP * ldP;
   const _Float16* Q = p.Q + z * PARTS * (long)p.dP * ldQ;
+  const int first = MODE == GRAM ? 0 : p.shift[z];
 
   // how the 32-byte groups of depth k's row are permuted: depths 0 .. 3 and 8 .. 11, which are read at a time, meet different banks
   auto turn = [](int k) { return GR >= 8 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2); };
@@ -554,6 +567,19 @@ static __device__ __forceinline__ void product_tile(const Product& p, const long
   constexpr int IT = TILE * TILE / 8 / 256;
   float* tile = reinterpret_cast<float*>(store);
   static_assert(RING * 2 * 64 * 2 >= TILE * 4, "");
+  float unscale = p.unscale, add = p.add;
+  int k = 0;
+  if (MODE != GRAM) {
+    k = first > p.k_before ? first - p.k_before : 0;
+    if (MODE == POLY) {
+      unscale = ldexpf(unscale, -4 * k);
+      add = ldexpf(add, -2 * k);
+    } else if (!LAST) {
+      const int down = (first > p.k_after ? first - p.k_after : 0) - k;
+      unscale = ldexpf(unscale, down);
+      add = ldexpf(add, down);
+    }
+  }
   auto spot = [](int r, int c) { return r * TILE + 4 * ((c >> 2) ^ ((r & 15) ^ ((r >> 3) & 6))) + (c & 3); };
   const int ld = MODE == UPDATE ? p.LP : p.dP;
   const long zC = z * PARTS * (long)p.dP * ld;
@@ -571,7 +597,7 @@ static __device__ __forceinline__ void product_tile(const Product& p, const long
 #pragma unroll
   for (int m = 0; m < WT; ++m)
 #pragma unroll
-    for (int n = 0; n < WT; ++n) *(f4*)(tile + spot(wm + 16 * m + i, wn + 16 * n + 4 * g)) = acc[m][n] * p.unscale;
+    for (int n = 0; n < WT; ++n) *(f4*)(tile + spot(wm + 16 * m + i, wn + 16 * n + 4 * g)) = acc[m][n] * unscale;
   __syncthreads();
   const bool turned = LAST ? p.tall : MODE != UPDATE && tm != tn;
 #pragma unroll
@@ -581,11 +607,15 @@ static __device__ __forceinline__ void product_tile(const Product& p, const long
     f4 *const p0 = (f4*)(tile + spot(r, c)), *const p1 = (f4*)(tile + spot(r, c + 4));
     f4 v0 = *p0, v1 = *p1;
     if (MODE != GRAM) {
-      v0 += p.add * __builtin_convertvector(__builtin_shufflevector(dh[u], dh[u], 0, 1, 2, 3), f4);
-      v1 += p.add * __builtin_convertvector(__builtin_shufflevector(dh[u], dh[u], 4, 5, 6, 7), f4);
+      v0 += add * __builtin_convertvector(__builtin_shufflevector(dh[u], dh[u], 0, 1, 2, 3), f4);
+      v1 += add * __builtin_convertvector(__builtin_shufflevector(dh[u], dh[u], 4, 5, 6, 7), f4);
       if (MODE == UPDATE || PARTS == 2) {
-        v0 += p.add * __builtin_convertvector(__builtin_shufflevector(dl[u], dl[u], 0, 1, 2, 3), f4);
-        v1 += p.add * __builtin_convertvector(__builtin_shufflevector(dl[u], dl[u], 4, 5, 6, 7), f4);
+        v0 += add * __builtin_convertvector(__builtin_shufflevector(dl[u], dl[u], 0, 1, 2, 3), f4);
+        v1 += add * __builtin_convertvector(__builtin_shufflevector(dl[u], dl[u], 4, 5, 6, 7), f4);
+      }
+      if (LAST) {  // (here, and not in the factors: those could leave fp32's normal numbers where the result does not)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v0[j] = ldexpf(v0[j], -k), v1[j] = ldexpf(v1[j], -k);
       }
       if (turned) *p0 = v0, *p1 = v1;
     }
@@ -651,7 +681,7 @@ __global__ __launch_bounds__(256, 2) void orth_product_kernel(Product p) {
   }
 }
 
-struct PartsPlan { int dP, LP; size_t x, aa, norm; };
+struct PartsPlan { int dP, LP; size_t x, aa, norm, shift; };
 PartsPlan parts_plan(const KfOrthArgs& a) {
   PartsPlan p;
   const int d = a.rows < a.cols ? a.rows : a.cols, L = a.rows < a.cols ? a.cols : a.rows;
@@ -660,6 +690,7 @@ PartsPlan parts_plan(const KfOrthArgs& a) {
   p.x = kf_seq_round((size_t)a.n * p.dP * p.LP * 2);
   p.aa = kf_seq_round((size_t)a.n * p.dP * p.dP * 2);
   p.norm = norm_bytes(a);
+  p.shift = kf_seq_round((size_t)a.n * 4);
   return p;
 }
 
@@ -695,6 +726,7 @@ template <typename T, int PARTS>
 int launch_parts(kf_handle* h, const KfOrthArgs& a, const PartsPlan& pl, void* ws, hipStream_t stream) {
   char* w = (char*)ws;
   double* norm = (double*)w; w += pl.norm;
+  int* shift = (int*)w; w += pl.shift;
   _Float16 *X[2][2], *A[2], *B[2];  // hi, lo
   // (stored together, the lo parts are 32 entries behind the hi parts)
   auto take = [&](size_t bytes, _Float16** q) {
@@ -712,15 +744,24 @@ int launch_parts(kf_handle* h, const KfOrthArgs& a, const PartsPlan& pl, void* w
   p.L = p.tall ? a.rows : a.cols;
   p.dP = pl.dP; p.LP = pl.LP;
   p.out = a.X;
+  p.shift = shift;
   hipLaunchKernelGGL(orth_norm_kernel<T>, dim3(parts, (unsigned)a.n), dim3(256), 0, stream, (const T*)a.M, size, norm);
-  hipLaunchKernelGGL((orth_parts_kernel<T, PARTS>), dim3(pl.LP / 64, pl.dP / 64, (unsigned)a.n), dim3(256), 0, stream, a, norm, parts, pl.dP, pl.LP, X[0][0], X[0][1]);
+  hipLaunchKernelGGL((orth_parts_kernel<T, PARTS>), dim3(pl.LP / 64, pl.dP / 64, (unsigned)a.n), dim3(256), 0, stream, a, norm, parts, pl.dP, pl.LP, X[0][0], X[0][1],
+                     shift);
+  double grown = 0.;  // log2 of what the steps so far can have multiplied a singular value by
   for (int s = 0; s < a.steps; ++s) {
     const double ca = a.coef[s][0], cb = a.coef[s][1], cc = a.coef[s][2];
     const int from = s & 1, to = from ^ 1;
     const double top = a.top[s];
-    // |B| <= the largest |b u + c u^2|, u = s^2 <= top^2
-    double bound = fabs(top * top * (cb + cc * top * top));
-    if (cc != 0.0 && -cb / (2 * cc) > 0 && -cb / (2 * cc) < top * top) bound = fmax(bound, fabs(cb * cb / (4 * cc)));
+    // |B| <= the largest |b u + c u^2|, and a singular value grows by at most the largest |a + b u + c u^2|, u = s^2 <= top^2
+    double bound = fabs(top * top * (cb + cc * top * top)), most = fmax(fabs(ca), fabs(ca + top * top * (cb + cc * top * top)));
+    if (cc != 0.0 && -cb / (2 * cc) > 0 && -cb / (2 * cc) < top * top) {
+      bound = fmax(bound, fabs(cb * cb / (4 * cc)));
+      most = fmax(most, fabs(ca - cb * cb / (4 * cc)));
+    }
+    p.k_before = (int)ceil(grown);
+    grown += fmax(log2(most), 0.);
+    p.k_after = (int)ceil(grown);
     int e = 0;
     frexp(fmax(bound, 1e-6), &e);
     const double scale_b = ldexp(1.0, 14 - e);  // |B| comes to at most 2^14: room for what A's rounding adds
@@ -953,7 +994,7 @@ size_t kf_orthogonalise_ws(const kf_handle* h, const KfOrthArgs& a) {
     return norm_bytes(a) + 2 * kf_seq_round((size_t)a.n * d * L * 8) + 2 * kf_seq_round((size_t)a.n * d * d * 8) +
            cut64(h, a.n, (int)d, (int)L);
   const PartsPlan p = parts_plan(a);
-  return p.norm + 4 * p.x + 4 * p.aa;
+  return p.norm + p.shift + 4 * p.x + 4 * p.aa;
 }
 
 int kf_launch_orthogonalise(kf_handle* h, const KfOrthArgs& a, void* ws, hipStream_t stream) {

@@ -530,6 +530,44 @@ def test_orthogonalise_zeros_and_not_a_number(eng):
                 assert torch.isnan(got[1]).all() and torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2])
 
 
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("shape", [(2, 10, 14), (2, 70, 60), (2, 150, 200), (1, 210, 130)], ids=str)
+@pytest.mark.parametrize("rho", [1e-2, 1e-4, 1e-7, 1e-15, 1e-28])
+def test_orthogonalise_far_below_eps(eng, shape, dtype, rho):
+    """|M|_F much smaller than eps: X starts at |M| / eps and every step still works on it to its own precision, not to that of 1.
+
+    A step's products are held in 22 bits (64-bit data: 52), and an error of that size relative to X leaves a step at most as large,
+    relative to what X has become, as the largest over the smallest growth of a singular value in it.  All of them are below 485 rho, so
+    that ratio is (1 + O((485 rho)^2)) for rho <= 1e-4, and for 1e-2 at most the product of the steps' ratios, computed below.  (bf16
+    products take hi parts, 2^-11, of B X alone, whose size relative to a X is computed too.)"""
+    rng = np.random.default_rng(81)
+    eps = 1.0
+    M = rng.standard_normal(shape)
+    M *= rho / np.linalg.norm(M, axis=(-2, -1), keepdims=True)
+    if dtype == torch.float16 and rho < 1e-3:
+        M, eps = M * 2.0 ** 20, 2.0 ** 20  # (its smallest numbers are 6e-8)
+    x = torch.from_numpy(M).to(dtype)
+    M = x.double().numpy()
+    # the result is about 485 rho for |X| = 1 spread over the matrix: well inside the normal numbers of all types here but fp16
+    got, want = eng.orthogonalise(x.cuda(), eps=eps), sn.orthogonalise(M, [NS] * 5, eps)
+    assert got.dtype == dtype
+    got = got.double().cpu().numpy()
+    for m, a, b in zip(M, got, want):
+        S = np.linalg.svd(m, compute_uv=False) / (np.linalg.norm(m) + eps)
+        total, ratio = 0.0, 1.0
+        for c0, c1, c2 in [NS] * 5:
+            gain = np.abs(c0 + c1 * S ** 2 + c2 * S ** 4)
+            extra = np.abs(c1 * S ** 2 + c2 * S ** 4).max()
+            S = gain * S
+            ratio *= max(1.0, gain.max() / gain.min())
+            unit = 2.0 ** -52 if dtype == torch.float64 else 2.0 ** -22
+            total += 8 * unit * (1 + np.sqrt(max(m.shape)) / 2) + (2.0 ** -11 * extra / gain.min() if dtype == torch.bfloat16 else 0.0)
+        size = np.linalg.norm(b)
+        # (a result below the type's normal numbers: half of its smallest step for each entry)
+        bound = (_u(dtype) + ratio * total) * size + _least(dtype) * np.sqrt(b.size)
+        assert np.linalg.norm(a - b) <= bound, (np.linalg.norm(a - b) / size, bound / size)
+
+
 def test_orthogonalise_views_and_leading_axes(eng):
     M = torch.randn(2, 3, 20, 12, device="cuda")
     want = eng.orthogonalise(M)
