@@ -123,4 +123,6 @@ static __device__ __forceinline__ long kf_xcd_work(long works) {
   const long per = (works + 7) >> 3;
   return (blockIdx.x & 7) * per + (blockIdx.x >> 3);
 }
-static inline unsigned kf_xcd_grid(long works) { return (unsigned)(8 * ((works + 7) >> 3)); }
+// (the last workgroup has the highest work: none where the division leaves a rest, and then it is not launched.  A launch has fewer than
+// 2^32 threads, and 4 tiles of V of 2^22 - 1 heads, 256 threads each, would come to 2^32 with it)
+static inline unsigned kf_xcd_grid(long works) { return (unsigned)(8 * ((works + 7) >> 3) - (works % 8 != 0)); }

@@ -413,6 +413,24 @@ def test_a_prompt_then_single_tokens(eng, dtype):
     _near(state, rS, n * aS, "state")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_as_many_sequences_as_are_allowed(eng, dtype):
+    """B H = 2^22 - 1 with as many tiles of V as there can be; one token each: S = k v', o = s q k v."""
+    B, V = 2 ** 22 - 1, 100
+    gen = torch.Generator(device="cuda").manual_seed(25)
+    q, k = (torch.randn(B, 1, 1, 1, device="cuda", generator=gen).to(dtype) for _ in range(2))
+    v = torch.randn(B, 1, 1, V, device="cuda", generator=gen).to(dtype)
+    o, state = eng.linear_attention(q, k, v, torch.zeros(1, device="cuda"), scale=0.5)
+    # one rounded product each (the state), and for o the score, rounded as the type is, times v, rounded to it
+    want = k.float() * v.float()
+    assert bool(((state[:, :, 0] - want[:, 0]).abs() <= 2 * U32 * want[:, 0].abs()).all())
+    want = 0.5 * q.double() * k.double() * v.double()
+    assert bool(((o.double() - want).abs() <= (2 * _u(dtype) + 4 * U32) * want.abs() * (1 + _u(dtype)) + 1e-37).all())
+    with pytest.raises(Exception, match="B H"):
+        x = torch.zeros(1, device="cuda", dtype=dtype).expand(2 ** 22, 1, 1, 1)
+        eng.linear_attention(x, x, x, torch.zeros(1, device="cuda"))
+
+
 # ------------------------------------------------------------------------------------------------ orthogonalised updates
 def _amplified(S, coefficients):
     """How far an error of relative size 1 (of |X|_F) in each step's X can have grown at the end: an odd polynomial of a matrix
