@@ -1803,8 +1803,8 @@ extern "C" int kf_orthogonalise(kf_handle* h, int64_t n, int32_t rows, int32_t c
     }
     a.top[s] = top;
     top = quintic_top(a.coef[s], top);
-    if (!(top <= 1.9)) {
-      KF_SET_ERR(h, "kf_orthogonalise: step %d can carry a singular value to %g (at most 1.9)", s, top);
+    if (!(top < 2.0)) {
+      KF_SET_ERR(h, "kf_orthogonalise: step %d can carry a singular value to %g (below 2)", s, top);
       return KF_ERR_ARG;
     }
   }

@@ -6,7 +6,7 @@
 //   * larger, up to 32 bits: tiled products on v_mfma_f32_16x16x32_f16, numbers held in fp16 parts (below)
 //   * larger, fp64: tiled products on v_mfma_f64_16x16x4
 //
-// Numbers in fp16 parts.  The singular values stay within 1.9 (checked on the host), so entries of X, A = X X' and B = b A + c A A are
+// Numbers in fp16 parts.  The singular values stay below 2 (checked on the host), so entries of X, A = X X' and B = b A + c A A are
 // bounded and a power of two for each brings them to the top of fp16's range: hi = fp16(x), lo = fp16(x - hi) hold 22 bits and
 // nothing overflows.  fp32 and fp16 data take three products, hi hi + hi lo + lo hi (2^-22 of the terms is lost), at 1/3 of fp16's rate,
 // five times fp32's.  bf16 data keep X in both parts, which is what the term a X and every later step build on, but multiply hi parts
@@ -357,8 +357,8 @@ static inline int norm_parts(long size) {  // about 16 elements a thread
 static inline size_t norm_bytes(const KfOrthArgs& a) { return kf_seq_round((size_t)a.n * norm_parts((long)a.rows * a.cols) * 8); }
 
 // ------------------------------------------------------------------------------------------------ fp16 parts
-constexpr float SCALE_X = 16384.f;  // 2^14: |x| <= 1.9 comes to 31130 of fp16's 65504
-constexpr float SCALE_A = 8192.f;   // 2^13: |a| <= 1.9^2 comes to 29573
+constexpr float SCALE_X = 16384.f;  // 2^14: |x| < 2 stays below 32768, half of what fp16 holds (what rounding adds has room)
+constexpr float SCALE_A = 8192.f;   // 2^13: |a| < 4 stays below 32768
 
 // Where entry (r, c) of a matrix with rows of ld entries has its hi part: alone (STORED 1), or with the lo parts of 32 columns
 // behind the hi parts of the same 32, one 128-byte line (STORED 2).

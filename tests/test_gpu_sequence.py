@@ -534,6 +534,23 @@ def test_orthogonalise_other_coefficients(eng, shape):
     np.testing.assert_allclose(X, U @ Vh, atol=1e-6)
 
 
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("shape", [(2, 9, 14), (2, 70, 60), (2, 150, 200), (1, 300, 130)], ids=str)
+def test_orthogonalise_with_steps_that_come_close_to_two(eng, shape, dtype):
+    """One singular value where the first step carries it to 1.992 (0.3763), and a last step at 1.99 throughout."""
+    from test_sequence import OPTIMISED
+
+    rng = np.random.default_rng(85)
+    n, r, c = shape
+    d = min(r, c)
+    S = np.abs(rng.standard_normal((n, d))) + 0.1
+    S[:, 0] = 0.3763 / np.sqrt(1 - 0.3763 ** 2) * np.linalg.norm(S[:, 1:], axis=-1)
+    U, V = (np.linalg.qr(rng.standard_normal((n, x, d)))[0] for x in (r, c))
+    M = (U * S[:, None]) @ np.swapaxes(V, -1, -2)
+    _check_orth(eng, M, dtype, OPTIMISED)
+    _check_orth(eng, M, dtype, OPTIMISED + [(1.99, 0.0, 0.0)])
+
+
 def test_orthogonalise_zeros_and_not_a_number(eng):
     for shape in ((3, 8, 8), (3, 70, 80)):
         for dtype in (torch.float32, torch.bfloat16, torch.float64):

@@ -182,6 +182,21 @@ def test_a_quintic_that_is_nearly_a_cubic_is_refused(lib, handle, coef):
     assert b"singular value" in lib.kf_last_error(handle)
 
 
+# a published list of steps, each the best on what the one before leaves; the first reaches 1.992
+OPTIMISED = [(8.28721201814563, -23.595886519098837, 17.300387312530933), (4.107059111542203, -2.9478499167379106, 0.5448431082926601),
+             (3.9486908534822946, -2.908902115962949, 0.5518191394370137), (3.3184196573706015, -2.488488024314874, 0.51004894012372),
+             (2.300652019954817, -1.6689039845747493, 0.4188073119525673), (1.891301407787398, -1.2679958271945868, 0.37680408948524835),
+             (1.875, -1.25, 0.375)]
+
+
+@pytest.mark.parametrize("safety", [1.0, 1.01])
+@pytest.mark.parametrize("rows, cols, dtype", [(96, 96, 1), (96, 96, 2), (96, 96, 0), (300, 200, 3)])
+def test_steps_that_come_close_to_two_are_taken(lib, handle, rows, cols, dtype, safety):
+    coef = [x for a, b, c in OPTIMISED for x in (a / safety, b / safety ** 3, c / safety ** 5)]
+    one, two = C.c_void_p(16), C.c_void_p(1 << 20)
+    assert lib.kf_orthogonalise(handle, 1, rows, cols, dtype, len(OPTIMISED), (C.c_double * len(coef))(*coef), 1e-7, one, two, None, 0, None) == -3
+
+
 def test_the_bound_of_a_step_is_its_polynomials_maximum(lib, handle):
     """Random lists: refused exactly where a fine grid finds a value above the bound in some step.  (The workspace is left out, so that
     a list that is taken ends there.)"""
