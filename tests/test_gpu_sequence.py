@@ -195,6 +195,55 @@ def test_decays_that_grow(eng, dtype):
     _check_backward(eng, p, TYPES[dtype])
 
 
+# many heads: (B, T, G, H, K, V), fixed decays, lengths, and (segments, chunks of each) of the gradient by data type on 256 units
+MANY = [((2, 300, 16, 64, 72, 72), True, [300, 131], (2, 3), (2, 5)),       # 128 x 128, segments summed by the workgroups that need them
+        ((4, 200, 64, 64, 100, 128), True, None, (1, 4), (1, 7)),           # one segment
+        ((2, 1100, 8, 32, 64, 40), True, [1100, 577], (6, 3), (7, 5)),      # 64 x 64
+        ((2, 2500, 16, 16, 32, 24), False, None, (20, 2), (27, 3)),         # 32 x 32, more than 8 segments: summed by a launch of their own
+        ((3, 2100, 3, 12, 20, 32), True, [2100, 0, 1027], (17, 2), (22, 3)),  # the same, ragged
+        ((4, 260, 16, 32, 4, 7), False, [260, 64, 65, 1], (2, 3), (2, 5))]  # rows shorter than 16 bytes
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape, per_token, lengths, split16, split32", MANY, ids=lambda x: str(x) if isinstance(x, tuple) and len(x) == 6 else "")
+def test_several_chunks_in_each_segment(eng, monkeypatch, shape, per_token, lengths, split16, split32, dtype):
+    """Batches of so many heads that a workgroup of the gradient walks several chunks: states kept at every chunk's start, both sums
+    carried from chunk to chunk."""
+    import ctypes as C
+
+    from oracle import sequence_torch as st
+    from pymc_statespace_amd import _lib
+
+    B, T, G, H, K, V = shape
+    t = TYPES[dtype]
+    # the split that the case is for, from what the call asks for: a state for each chunk's start is kept where segments have several
+    chunk = 64 if dtype == "bf16" else 32
+    D = 128 if min(K, V) < 8 else next(d for d in (32, 64, 128) if max(K, V) <= d)
+    segments, each = split16 if dtype == "bf16" else split32
+    if torch.cuda.get_device_properties(0).multi_processor_count == 256:
+        chunks, up = -(-T // chunk), lambda n: -(-n // 256) * 256
+        assert each > 1 and (segments - 1) * each < chunks <= segments * each
+        want = 2 * up(B * H * (segments - 1) * D * D * 4) + up(B * H * segments * 4) + 2 * up(B * H * (segments - 1) * 4) + up(B * H * chunks * D * D * 4) \
+            + (2 * up(B * T * H * K * 4) if G != H else 0) + (0 if per_token else up(B * H * segments * 8))
+        dims, n = _lib.pack_attention_dims(B, T, G, H, K, V, _lib.KF_DTYPE[{"f32": "float32", "f16": "float16", "bf16": "bfloat16"}[dtype]], per_token,
+                                           1.0, *[0] * 12), C.c_size_t()
+        assert eng.lib.kf_linear_attention_workspace(eng._h, dims, 1, C.byref(n)) == 0 and n.value == want
+    # (the oracle's own loops over tokens and sequences would take minutes)
+    for name in ("attention", "attention_gradient"):
+        monkeypatch.setattr(sn, name, lambda *a, f=getattr(st, name): f(*a, device="cuda"))
+    p = _make(19, *shape, t, per_token=per_token)
+    _check_forward(eng, p, t, lengths)
+    _check_backward(eng, p, t, lengths)
+    if lengths is not None:  # the same bits without what lies behind the sequences
+        dev = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        want = _backward(eng, p, t, dev)
+        for b, n in enumerate(lengths):
+            for name in ("q", "k", "v", "g_o") + (("log_decay",) if per_token else ()):
+                p[name][b, n:] = np.nan
+        got = _backward(eng, p, t, dev)
+        assert all(torch.equal(want[n], got[n]) for n in want)
+
+
 def test_no_decay_at_all(eng):
     """log_decay = 0: a plain running sum, the state grows with the length."""
     p = _make(6, 1, 700, 1, 1, 16, 16, torch.float32)

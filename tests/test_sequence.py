@@ -50,6 +50,23 @@ def test_the_oracles_gradient_against_differences(per_token, lengths):
         assert abs(2 * np.sum(grad[name] * step) - want) < 1e-11 * max(1.0, abs(want) / 1e-5), name
 
 
+@pytest.mark.parametrize("per_token", [True, False])
+@pytest.mark.parametrize("lengths", [None, [7, 0], [3, 5]])
+def test_the_batched_oracle_is_the_other(per_token, lengths):
+    from oracle import sequence_torch as st
+
+    rng = np.random.default_rng(5)
+    q, k, v, g, s0 = _problem(rng, G=2, H=4, per_token=per_token)
+    go, gs = rng.standard_normal(v.shape), rng.standard_normal(s0.shape)
+    for first, last in ((s0, gs), (None, None)):
+        for a, b in zip(sn.attention(q, k, v, g, 0.7, first, lengths), st.attention(q, k, v, g, 0.7, first, lengths)):
+            np.testing.assert_allclose(a, b, rtol=1e-13, atol=1e-13)
+        a, b = (m.attention_gradient(q, k, v, g, go, 0.7, first, lengths, last) for m in (sn, st))
+        assert a.keys() == b.keys()
+        for n in a:
+            np.testing.assert_allclose(a[n], b[n], rtol=1e-12, atol=1e-12, err_msg=n)
+
+
 def test_orthogonalise_maps_the_singular_values():
     rng = np.random.default_rng(2)
     for shape in ((5, 9), (9, 5), (6, 6)):
