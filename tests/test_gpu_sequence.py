@@ -652,6 +652,35 @@ def test_orthogonalise_far_below_eps(eng, shape, dtype, rho):
         assert np.linalg.norm(a - b) <= bound, (np.linalg.norm(a - b) / size, bound / size)
 
 
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("shape", [(3, 150, 200), (3, 210, 100)], ids=str)
+def test_orthogonalise_zeros_and_not_a_number_in_tiles(eng, shape, dtype):
+    """The tiled products keep the matrices of a batch apart as the others do."""
+    M = torch.from_numpy(np.random.default_rng(82).standard_normal(shape)).to(dtype).cuda()
+    clean = eng.orthogonalise(M)
+    M[1] = 0.0
+    got = eng.orthogonalise(M)
+    assert not got[1].any() and torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2])
+    for bad in (float("nan"), float("inf")):
+        M[1, 3, 2] = bad
+        got = eng.orthogonalise(M)
+        assert torch.isnan(got[1]).all() and torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("shape", [(90, 200, 260), (90, 260, 200), (172, 200, 260), (172, 260, 200), (1, 600, 700)], ids=str)
+def test_orthogonalise_in_tiles_off_the_diagonal(eng, shape, dtype):
+    """Enough matrices for tiles of 128, with several of them along each side: off the diagonal, stored with their mirror image; 172: the
+    last few of 516 (A, B) and 1032 (X) cut in four, off the diagonal too.  (1, 600, 700): tiles of 64 in bands of 8, the last partial."""
+    _check_orth(eng, np.random.default_rng(83).standard_normal(shape), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_orthogonalise_in_several_bands_of_large_tiles(eng, dtype):
+    """9 x 11 tiles of 128 for each of 6 matrices: a second band of one tile."""
+    _check_orth(eng, np.random.default_rng(84).standard_normal((6, 1100, 1290)), dtype)
+
+
 def test_orthogonalise_views_and_leading_axes(eng):
     M = torch.randn(2, 3, 20, 12, device="cuda")
     want = eng.orthogonalise(M)
