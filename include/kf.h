@@ -509,8 +509,8 @@ KF_API int kf_linear_attention_workspace(kf_handle* h, const kf_attention_dims* 
 /* Linear attention with a decay for each head, over whole sequences:
  *     S_t = exp(log_decay_t) S_{t-1} + k_t v_t',   o_t = s S_t' q_t,   S_0 = s0 (NULL: zero)
  * o [B][T][H][V]; sT [B][H][K][V] fp32, the state behind each sequence's last token (may be NULL).  No output overlaps an input or
- * another output.  log_decay is fp32 and meant to be <= 0 (a positive one is a growth, right while its product over 64 tokens stays in
- * fp32); anything below -1e4, -infinity included, is a reset of the state.  lengths [B] int32 (NULL: all T): tokens from
+ * another output.  log_decay is fp32 and meant to be <= 0 (a positive one is a growth, right while its product over 64 tokens and every
+ * state stay in fp32); anything below -1e4, -infinity included, is a reset of the state.  lengths [B] int32 (NULL: all T): tokens from
  * lengths[b] on (clamped to 0 .. T) are not read, o is zero there and the state stays.  The state, its sums and the decays are held
  * in 32 bits.  For bf16, o is computed from the state and the weighted scores rounded to bf16 (fp16 and fp32: in 32 bits throughout).
  * An infinity or NaN reaches only the outputs that the formula carries it to, those of its own and later tokens of its head. */

@@ -33,7 +33,7 @@ struct Split {
   long works;
   int segments, seg_chunks;
   long chunks;
-  float *adds_s, *adds_r, *factors;  // [B H][segments - 1][D D], [B H][segments] (each segment's whole decay)
+  float *adds_s, *adds_r, *factors;  // [B H][segments - 1][D D], [B H][segments] (the root of each segment's whole decay)
   float *products_s, *products_r;    // [B H][segments - 1]: see kf_attention_scan_kernel
   kf_f32x4* starts;                  // S_0 of every chunk: [B H][chunks][D / 16][threads]
   float *part_q, *part_k;            // [B][T][H][K], where heads share q and k
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
   auto add = [&](kf_f32x4& x, float f, const kf_f32x4* u, int t) {
     const kf_f32x4 y = u[real(t) ? t * TH : 0];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = real(t) ? x[r] * f + y[r] : x[r];
+    for (int r = 0; r < 4; ++r) x[r] = real(t) ? x[r] * f * f + y[r] : x[r];
   };
   kf_f32x4 acc[NT];
 #pragma unroll
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
       for (int t = 0; t < NT; ++t) add(acc[t], f, u, t);
     }
   }
-  float through = 1.f;
+  float through = 1.f;  // the root of the segment's decay
   Stage<C, A, T, D, MODE> rx, ry;
   float rg = 0.f;
   const long steps = last > c0 ? last - c0 : 0;
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
     rx.load(x, xs, at(0) * C, n, a.K);
     ry.load(y, ys, at(0) * C, n, a.V);
     rg = decay_of(at(1));
-    if (w == 0) dec[0].fill(decay_of(at(0)), l < C && at(0) * C + l < n);
+    if (w == 0) dec[0].template fill<!STARTS>(decay_of(at(0)), l < C && at(0) * C + l < n);
   }
   for (long s = 0; s < steps; ++s) {
     if (STARTS) {
@@ -158,10 +158,10 @@ __global__ __launch_bounds__(4 * D) void attention_sweep_kernel(KfAttnArgs a, Sp
     rg = decay_of(at(s + 2));
     rx.load(x, xs, at(next) * C, n, a.K);
     ry.load(y, ys, at(next) * C, n, a.V);
-    if (w == (int)(s % NT)) dec[(s + 1) & 1].fill(g1, l < C && at(s + 1) >= 0 && at(s + 1) * C + l < n);
+    if (w == (int)(s % NT)) dec[(s + 1) & 1].template fill<!STARTS>(g1, l < C && at(s + 1) >= 0 && at(s + 1) * C + l < n);
     const KfChunkDecay<C>& d = dec[s & 1];
     const float fe = d.from_start[C - 1];
-    through *= fe;
+    if (!STARTS) through = kf_root_decay(through * d.root);
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t] *= fe;
 #pragma unroll
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(4 * D, 2) void attention_gradient_kernel(KfAttnArgs
   auto add = [&](kf_f32x4& x, float f, const kf_f32x4* u, int t) {  // as in the sweeps
     const kf_f32x4 y = u[real(t) ? t * TH : 0];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = real(t) ? x[r] * f + y[r] : x[r];
+    for (int r = 0; r < 4; ++r) x[r] = real(t) ? x[r] * f * f + y[r] : x[r];
   };
   kf_f32x4 R[NT];  // rows v, columns k
 #pragma unroll
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(4 * D, 2) void attention_gradient_kernel(KfAttnArgs
       load_start(last - 1);
     }
     rg = decay_of(last - 2);
-    if (w == 0) dec[0].fill(decay_of(last - 1), l < C && (last - 1) * C + l < n);
+    if (w == 0) dec[0].template fill<false>(decay_of(last - 1), l < C && (last - 1) * C + l < n);
   }
   double decay_sum = 0.;
   int turn = 0;
@@ -345,7 +345,7 @@ __global__ __launch_bounds__(4 * D, 2) void attention_gradient_kernel(KfAttnArgs
     const float g1 = rg;
     rg = decay_of(c - 2);
     load(next);
-    if (w == NT - 1) dec[turn ^ 1].fill(g1, l < C && c > 0 && t0 - C + l < n);
+    if (w == NT - 1) dec[turn ^ 1].template fill<false>(g1, l < C && c > 0 && t0 - C + l < n);
     const KfChunkDecay<C>& d = dec[turn];
 
     // scores: tile (it, jt) of A and B, rows j, columns i

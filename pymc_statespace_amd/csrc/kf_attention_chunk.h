@@ -13,19 +13,27 @@ static __device__ __forceinline__ double kf_readlane(double x, int lane) {
   return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), lane), __builtin_amdgcn_readlane(__double2loint(x), lane));
 }
 
+// A segment's decay is handed on as its square root, and a state multiplied by that twice: positive log decays may come to more over a
+// segment than fp32 holds while every state stays inside (a zero one, for instance, which must not meet an infinity).  The root of what
+// does not fit either is the largest number: it takes any state that is not zero out of range, as the growth itself would.
+static __device__ __forceinline__ bool kf_too_large(float x) { return x > 3.402823466e38f; }
+static __device__ __forceinline__ float kf_root_decay(float x) { return kf_too_large(x) ? 3.402823466e38f : x; }
+
 // Decays of one chunk, G_i = sum of the log decays up to and with token i (summed in 64 bits; each exponent is rounded once).
 // No exponent is positive: pairs (i, j) in different 16-token tiles take exp(G_i - G_j) as the product of two factors <= 1 that meet
 // at the end of j's tile, so that only the tiles on the diagonal need an exponential for each pair.
 template <int C>
-struct KfChunkDecay {
+struct alignas(16) KfChunkDecay {  // (its rows are read 16 bytes at a time)
   float from_start[C];            // exp(G_i): from the chunk's start through token i
   float to_end[C];                // exp(G_(C-1) - G_j): from behind token j to the chunk's end
   float to_tile_end[C];           // exp(G_e - G_j), e the last token of j's tile
   float from_tile[C / 16 - 1][C]; // exp(G_i - G_e), e the last token of an earlier tile
   float hi[C], lo[C];             // G in two floats, for the diagonal
+  float root;                     // exp(G_(C-1) / 2), see kf_root_decay
 
   // by one whole wave, lane l with token l; tokens that are not `live` (lanes from C on are not) neither decay nor write
-  __device__ __forceinline__ void fill(float log_decay, bool live) {
+  // (ROOT: `root` too, for what sums up segments)
+  template <bool ROOT> __device__ __forceinline__ void fill(float log_decay, bool live) {
     const int l = threadIdx.x & 63, row = l >> 4;
     double G = live ? (double)kf_clamp_log_decay(log_decay) : 0.0;
     // running sums inside each row of 16 lanes, then over the rows
@@ -47,6 +55,7 @@ struct KfChunkDecay {
       for (int t = 0; t < C / 16 - 1; ++t) {
         from_tile[t][l] = row > t ? __expf((float)(G - end[t])) : 0.f;
       }
+      if (ROOT && l == 0) root = kf_root_decay(__expf((float)(0.5 * end[C / 16 - 1])));
       hi[l] = (float)G;
       lo[l] = (float)(G - (double)hi[l]);
     }
@@ -63,8 +72,8 @@ struct KfChunkDecay {
 };
 
 // What each segment adds to a state (slots 0 .. n - 1 of `cells` 16-byte pieces for each head) into the state that the next segment
-// starts from, in place; products[s]: what becomes of a state from before all of them.  `back`: from the last slot to the first, with
-// the decay of the segment behind each slot.  Up to KF_FUSED_SEGMENTS segments each workgroup sums up what is before it by itself
+// starts from, in place; products[s]: what becomes of a state from before all of them (its square root, like the factors).  `back`: from
+// the last slot to the first, with the decay of the segment behind each slot.  Up to KF_FUSED_SEGMENTS segments each workgroup sums up what is before it by itself
 // (about 0.4 us for each 64 KB); beyond, this kernel (4 to 6 us) is the shorter way and keeps the sum linear in their number.
 constexpr int KF_FUSED_SEGMENTS = 8;
 static __global__ __launch_bounds__(256) void kf_attention_scan_kernel(kf_f32x4* adds_s, kf_f32x4* adds_r, const float* factors, float* products_s,
@@ -97,8 +106,8 @@ static __global__ __launch_bounds__(256) void kf_attention_scan_kernel(kf_f32x4*
     for (int j = 0; j < 8; ++j)
       if (s0 + j < n) {
         const int slot = back ? n - 1 - s0 - j : s0 + j;
-        sum = sum * d[j] + in[j];
-        product *= d[j];
+        sum = sum * d[j] * d[j] + in[j];
+        product = kf_root_decay(product * d[j]);
         a[slot * cells] = sum;
         if (e == 0) products[head * n + slot] = product;
       }

@@ -86,7 +86,15 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
     // (many segments: already summed up, with the products of the decays)
     const bool summed = sp.segments > KF_FUSED_SEGMENTS;
     for (int s = summed && seg ? seg - 1 : 0; s < seg; ++s) {
-      const float f = (summed ? products : factors)[bh * (sp.segments - 1) + s];
+      const float root = (summed ? products : factors)[bh * (sp.segments - 1) + s];
+      float f = root * root;  // (5 x 1000 tokens: 42.5 us, 43.3 with both multiplications each time)
+      if (kf_too_large(f)) {
+#pragma unroll
+        for (int m = 0; m < SM; ++m)
+#pragma unroll
+          for (int t = 0; t < SN; ++t) S[m][t] *= root;
+        f = root;
+      }
       const kf_f32x4* u = reinterpret_cast<const kf_f32x4*>(adds) + (cell + (long)s * sp.v_tiles + vt) * (KP * VT / 4) + tid;
 #pragma unroll
       for (int m = 0; m < SM; ++m)
@@ -94,7 +102,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
         for (int t = 0; t < SN; ++t) S[m][t] = S[m][t] * f + u[(m * SN + t) * 256];
     }
   }
-  float through = 1.f;
+  float through = 1.f;  // the root of the segment's decay
 
   typename Row::Raw rk[KK], rv[VT / 32], rq[KK];  // the next chunk's, as loaded
   float rg = 0.f;                                  // and the log decay of one token of the chunk behind it
@@ -139,7 +147,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
     rg = log_decay(c0 + 1);
     load(c0);
     if (OUT) load_q(c0);
-    if (w == 0) dec[c0 & 1].fill(first, c0 * KF_CHUNK + l < n);
+    if (w == 0) dec[c0 & 1].template fill<!OUT>(first, c0 * KF_CHUNK + l < n);
     if (OUT) put_state();
   }
   for (long c = c0; c < end; ++c) {
@@ -152,7 +160,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
     const float g1 = rg;
     rg = log_decay(c + 2);
     load(next);
-    if (w == (int)(c & 3)) dec[(c + 1) & 1].fill(g1, (c + 1) * KF_CHUNK + l < n);
+    if (w == (int)(c & 3)) dec[(c + 1) & 1].template fill<!OUT>(g1, (c + 1) * KF_CHUNK + l < n);
     const KfChunkDecay<KF_CHUNK>& D = dec[c & 1];
 
     if (OUT) {
@@ -291,7 +299,7 @@ __global__ __launch_bounds__(256, 2) void attention_chunk_kernel(KfAttnArgs a, K
 
     // the state at the chunk's end
     const float fe = D.from_start[KF_CHUNK - 1];
-    through *= fe;
+    if (!OUT) through = kf_root_decay(through * D.root);
 #pragma unroll
     for (int m = 0; m < SM; ++m)
 #pragma unroll

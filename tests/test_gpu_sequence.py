@@ -244,6 +244,30 @@ def test_several_chunks_in_each_segment(eng, monkeypatch, shape, per_token, leng
         assert all(torch.equal(want[n], got[n]) for n in want)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("H", [2, 64])
+def test_a_growth_that_nothing_takes_part_in(eng, monkeypatch, H, dtype):
+    """Decays of e^0.5 a token over 1500 tokens: far more than fp32 holds over a segment or all of them, but the state is zero until token
+    700 and after the reset at 800, and so is what flows back from behind it and to before the reset at 690.  (H: segments summed by a
+    launch of their own, and by the workgroups that need them.)"""
+    from oracle import sequence_torch as st
+
+    for name in ("attention", "attention_gradient"):
+        monkeypatch.setattr(sn, name, lambda *a, f=getattr(st, name): f(*a, device="cuda"))
+    p = _make(26, 1, 1500, H, H, 24, 40, TYPES[dtype], init=False)
+    p["log_decay"] = np.random.default_rng(27).uniform(0.48, 0.52, p["log_decay"].shape).astype(np.float32).astype(np.float64)
+    p["log_decay"][:, [690, 800]] = -np.inf
+    p["k"][:, :700] = p["k"][:, 780:] = 0.0
+    p["g_o"][:, :700] = p["g_o"][:, 800:] = 0.0
+    if dtype == "f16":  # (e^50 does not fit its outputs: the state and its gradient, which are fp32, by values that keep them small)
+        for x in ("k", "g_o"):
+            p[x] = torch.from_numpy(p[x] * 2.0 ** -14).half().double().numpy()
+        p["log_decay"][:, 700:800] *= 0.25
+        p["log_decay"] = p["log_decay"].astype(np.float32).astype(np.float64)
+    _check_forward(eng, p, TYPES[dtype])
+    _check_backward(eng, p, TYPES[dtype])
+
+
 def test_no_decay_at_all(eng):
     """log_decay = 0: a plain running sum, the state grows with the length."""
     p = _make(6, 1, 700, 1, 1, 16, 16, torch.float32)
