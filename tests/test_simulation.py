@@ -58,6 +58,27 @@ def test_simulation_reference_signature_and_statistics():
         assert_allclose(sims[:, t].mean(0), mus.reshape(n, k)[t], atol=0.06)
 
 
+def test_simulation_statistics_in_standard_errors():
+    """Means and covariances of S draws within five of their standard errors (a normal number is outside of that once in 1.7 million;
+    the draws are the same in every run)."""
+    import torch
+
+    from pymc_statespace_amd.simulation import conditional_simulation
+
+    rng = np.random.default_rng(1)
+    n, k, S = 3, 4, 20000
+    A = rng.standard_normal((1, n, k, k))
+    covs = A @ np.swapaxes(A, -1, -2) + 0.5 * np.eye(k)
+    mus = rng.standard_normal((1, n * k))
+    sims = conditional_simulation(mus, covs, n, k, n_simulations=S, generator=torch.Generator(device="cuda").manual_seed(3))
+    for t in range(n):
+        c, mu = covs[0, t], mus.reshape(n, k)[t]
+        var = np.diagonal(c)
+        assert (np.abs(sims[:, t].mean(0) - mu) <= 5 * np.sqrt(var / S)).all()
+        # the variance of one term (x_i - mu_i)(x_j - mu_j) is c_ii c_jj + c_ij^2
+        assert (np.abs(np.cov(sims[:, t].T) - c) <= 5 * np.sqrt((np.outer(var, var) + c * c) / S)).all()
+
+
 def test_simulation_singular_covariance_needs_jitter():
     """Filtered covariances with H = 0 are exactly singular: the reference adds a jitter for
     this; without it the factorisation is flagged."""
