@@ -81,9 +81,10 @@ def _newton_schulz(coefficients, steps):
         return steps, (C.c_double * (3 * steps))(*(coefficients * steps))  # (as below, without numpy's 3 us)
     c = np.asarray(coefficients, dtype=np.float64)
     if c.shape == (3,):
-        if not 1 <= int(steps) <= most:
-            raise ValueError(f"steps must be between 1 and {most}")
-        c = np.broadcast_to(c, (int(steps), 3))
+        count = int(steps)
+        if count != steps or not 1 <= count <= most:
+            raise ValueError(f"steps must be a whole number between 1 and {most}")
+        c = np.broadcast_to(c, (count, 3))
     if c.ndim != 2 or c.shape[1] != 3 or not 1 <= c.shape[0] <= most:
         raise ValueError(f"coefficients: (a, b, c), or 1 to {most} of them")
     return c.shape[0], (C.c_double * (3 * c.shape[0]))(*c.ravel().tolist())

@@ -293,3 +293,20 @@ def test_matrices_that_the_engine_refuses(engine):
         engine.orthogonalise(torch.zeros(3, 3), steps=17)
     with pytest.raises(ValueError):
         engine.orthogonalise(torch.zeros(3, 3), coefficients=[(1.0, 2.0)])
+
+
+@pytest.mark.parametrize("steps", [2.5, "3", None, float("nan")])
+@pytest.mark.parametrize("coefficients", [(1.5, -0.5, 0.0), [1.5, -0.5, 0.0]])
+def test_a_number_of_steps_that_is_not_whole_is_refused(engine, steps, coefficients):
+    with pytest.raises((TypeError, ValueError)):
+        engine.orthogonalise(torch.zeros(3, 3), steps=steps, coefficients=coefficients)
+
+
+def test_steps_as_any_whole_number():
+    from pymc_statespace_amd.engine import _newton_schulz
+
+    want = [1.5, -0.5, 0.25] * 3
+    for steps in (3, 3.0, np.int64(3), torch.tensor(3)):
+        for c in ((1.5, -0.5, 0.25), [1.5, -0.5, 0.25], np.array([1.5, -0.5, 0.25])):
+            n, coef = _newton_schulz(c, steps)
+            assert n == 3 and list(coef) == want
