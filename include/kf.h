@@ -540,7 +540,8 @@ KF_API int kf_linear_attention_step(kf_handle* h, const kf_attention_dims* dims,
  *     X = M / (|M|_F + eps);   for each step (a, b, c):   A = X X',   X <- a X + (b A + c A A) X
  * (on the transpose where rows > cols).  coefficients: HOST double[n_steps][3].  The singular values of X start in [0, 1] and each
  * goes through the polynomials a s + b s^3 + c s^5; a list that can carry one of them to 2 or above is refused (KF_ERR_ARG).
- * X: the type and shape of M, not overlapping it.  1 <= n_steps <= 16.  The same inputs give the same bits. */
+ * |M|_F is the root of a sum in 64 bits: KF_DTYPE_F64 entries beyond about 1e150, whose squares do not fit, give zeros, and below 1e-150
+ * count as nothing beside eps.  X: the type and shape of M, not overlapping it.  1 <= n_steps <= 16.  The same inputs give the same bits. */
 #define KF_ORTHOGONALISE_STEPS_MAX 16
 KF_API int kf_orthogonalise_workspace(kf_handle* h, int64_t n, int32_t rows, int32_t cols, int32_t dtype, size_t* bytes);
 KF_API int kf_orthogonalise(kf_handle* h, int64_t n, int32_t rows, int32_t cols, int32_t dtype, int32_t n_steps,

@@ -10,10 +10,11 @@
 // weighted keys enter it in three parts (KfSplit).
 //
 // Measured: 4 x 2048 tokens, 16 heads of 128 x 128, bf16: 25 + 46 us for 139 MB (30 us at the 4.7 TB/s of a large copy).  32768 tokens, 32
-// heads of 128 x 64: 88 + 7 + 153 us for 408 MB (87 us).  5 x 1000 ragged tokens, 6 heads of 72 x 56, fp32: 12 + 32 us.  The second
-// launch takes 33 us of its 46 with its loads, stores and barriers alone; what the rest adds is issue: two waves on a SIMD (220
-// registers) spend 46 % of its cycles on vector instructions -- 290 of 670 for each chunk cut the weighted keys --, the matrix pipe is
-// busy 23 %, LDS 18 %.  A third wave (168 registers) spills and gains nothing.
+// heads of 128 x 64: 88 + 7 + 153 us for 408 MB (87 us).  5 x 1000 ragged tokens, 6 heads of 72 x 56, fp32: 12 + 32 us.  The first case in
+// fp16 205 us, in fp32 208 (eight fp32 instructions for one of bf16); its 16 heads as 4 x 4, by the 128-wide kernel with loads of single
+// elements, 48 in bf16.  The first case's second launch takes 33 us of its 46 with its loads, stores and barriers alone; what the rest adds
+// is issue: two waves on a SIMD (220 registers) spend 46 % of its cycles on vector instructions -- 290 of 670 for each chunk cut the
+// weighted keys --, the matrix pipe is busy 23 %, LDS 18 %.  A third wave (168 registers) spills and gains nothing.
 #include "kf_attention_chunk.h"
 
 namespace {

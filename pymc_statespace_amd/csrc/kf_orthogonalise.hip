@@ -18,7 +18,7 @@
 // Y = 2^k X a step is a Y + (4^-k b (YY') + 16^-k c (YY')^2) Y.  k = 0 multiplies by 1: no bit of other matrices changes.
 //
 // Measured: one 4096 x 4096 in fp32 3.7 ms, at 1101 TFLOP/s (the fp16 rate of a large library product) its 4.1 TFLOP take 3.75 ms; its fp32
-// library products 14.5 ms.  Four of 768 x 2048 in bf16 221 us, 74 at that rate: with 312 tiles of 64 (A, B) and 384 of 128 (X) for 256
+// library products 14.5 ms.  Four of 768 x 2048 in fp32 or fp16 387 us, in bf16 224, 74 at that rate: with 312 tiles of 64 (A, B) and 384 of 128 (X) for 256
 // compute units, the units that have two bound each product by the 64 bytes a cycle they can read, 15 + 8 + 22 us a step.
 #include "kf_sequence.h"
 
@@ -157,7 +157,8 @@ static inline bool fits_wave(const KfOrthArgs& a) { return (a.rows <= 16 && a.co
 // pieces apart: neighbouring rows meet different banks.  Where A has fewer tiles than there are waves the sum over L is cut into
 // `slices`, which meet in LDS.  Measured against the tiled products below, fp32: 256 matrices of 24 x 24 11 and 143 us, 256 of 64 x 64 42 and
 // 145, 256 of 64 x 250 79 and 189, one of 64 x 250 71 and 63, one of 80 x 150 69 and 75; fp64: 256 of 80 x 80 74 and 510 us.  Bound by the
-// waits between its three products a step, each short: the matrix pipe is busy 10 us of a 64 x 64 matrix's 40.
+// waits between its three products a step, each short: the matrix pipe is busy 10 us of a 64 x 64 matrix's 40.  (8 waves of 16 tiles, for
+// more than 64 tiles of X in 32 bits, spill 5 of their 256 registers.)
 template <typename C> struct ChipRow { static __host__ __device__ constexpr int stride(int n) { return sizeof(C) == 8 ? (n & ~1) | 2 : (n & ~3) | 4; } };
 
 // WAVES x HELD tiles of X at most, HELD for each wave.

@@ -781,7 +781,9 @@ class KalmanEngine:
         -> (o (B,T,H,V) in the type of q, state (B,H,K,V) fp32 behind each sequence's last token).
         q, k (B,T,G,K), v (B,T,H,V): float32, bfloat16 or float16, one type; head h reads group h // (H // G); K, V <= 128.
         log_decay (B,T,H), or (H,) for fixed decays: fp32, <= 0 (-inf resets the state).  scale: K ** -0.5 by default.
-        initial_state (B,H,K,V): what an earlier call left.  lengths (B,): tokens from there on are not read (o is zero there)."""
+        initial_state (B,H,K,V): what an earlier call left.  lengths (B,): tokens from there on are not read (o is zero there).
+        Autograd does not see the call: the outputs carry no gradient, also where inputs require one.  To train through it, wrap it and
+        ``linear_attention_backward`` in a ``torch.autograd.Function``."""
         d, sizes, q, k, v, g = self._attention_args(q, k, v, log_decay, scale)
         s0 = self._seq_f32(initial_state, "initial_state", sizes)
         lengths = self._seq_i32(lengths, "lengths", sizes[0])
@@ -816,7 +818,7 @@ class KalmanEngine:
     def linear_attention_step(self, q, k, v, log_decay, state, *, scale=None, slots=None, state_out=None):
         """kf_linear_attention_step: one token of each sequence, its state in a pool -> (o (B,H,V), info (B,) int32).
         q, k (B,G,K), v (B,H,V), log_decay (B,H) or (H,); state (N,H,K,V) fp32 is advanced in place, or into ``state_out`` (slots
-        that no row names are not touched).  slots (B,): the pool's entry of each row (None: row b has entry b); a negative one is an
+        that no row names are not touched; autograd does not see the call).  slots (B,): the pool's entry of each row (None: row b has entry b); a negative one is an
         empty row (o zero), one >= N as well, with info 1; rows with the same slot are consecutive tokens of that sequence."""
         d, (B, H, K, V), q, k, v, g = self._attention_args(q, k, v, log_decay, scale, ndim=3)
         N = state.shape[0] if getattr(state, "ndim", 0) else 0
@@ -840,7 +842,9 @@ class KalmanEngine:
         """kf_orthogonalise: each matrix of M (..., rows, cols) moved towards its orthogonal factor by Newton-Schulz products,
         X = M / (|M|_F + eps), then X <- a X + (b A + c A A) X with A = X X' (on the transpose where rows > cols); the type of M
         (float64, float32, bfloat16, float16).  ``coefficients``: one (a, b, c) used ``steps`` times, or a list of them, one for each
-        step.  For instance an update of weights from their gradient, or of a batch of transition matrices from ``value_and_grad``'s."""
+        step; one that can carry a singular value to 2 is refused.  For instance an update of weights from their gradient, or of a batch
+        of transition matrices from ``value_and_grad``'s.  Autograd does not see the call.  (float64: entries beyond about 1e150, whose
+        squares do not fit, give zeros.)"""
         t = M if isinstance(M, torch.Tensor) else torch.as_tensor(np.ascontiguousarray(M))
         code = _SEQ_DTYPES.get(t.dtype)
         if code is None:
